@@ -214,6 +214,80 @@ int mxfp4_kv_write(const void* k, const void* v, uint8_t* kvk, uint8_t* kvv, con
                    int M, int Hkv, int D, int max_pos, void* stream);
 
 /* ---------------------------------------------------------------------
+ * The KV cache in MXFP4: write, read back, attention.  No counterpart in the
+ * reference, whose cache is FP8 (mxfp4_kv_write / mxfp4_attn_decode above): a
+ * head row of 128 takes 68 bytes here, 128 there.  Unlike those, the entries
+ * take several sequences, paged or not, head dimensions of 64 and 128 and any
+ * number of query heads per kv head.
+ *
+ * The cache (every entry's kq .. max_pages):
+ *   kq, vq     u8 (n_pages, Hkv, page, D/2), ks, vs u8 (n_pages, Hkv, page,
+ *              D/32): a head row is the library's MXFP4 row (above); 16-byte
+ *              aligned; D = 64 or 128; page a multiple of 16
+ *   pages      device int32 (B, max_pages), a power-of-two page: position p of
+ *              sequence b is row p % page of page pages[b][p / page]; entries
+ *              outside [0, n_pages) are no page (-1 for what is not handed
+ *              out yet).  NULL: sequence b is page b (n_pages >= B, max_pages
+ *              unused)
+ * A sequence has positions 0 .. max_pos - 1, max_pos = page (pages NULL) or
+ * max_pages * page, at most 2^30.  dpos: device int32 (B), token m of sequence
+ * b sits at dpos[b] + m; read on the device, so a captured graph follows it.
+ * A slot of the batch that is empty has dpos[b] <= -M.
+ * Scale code 255 is no scale (the quantizer writes 0 .. 253) and reads as NaN.
+ *
+ * mxfp4_kv4_write: k, v (B*M tokens, ldk / ldv elements apart, Hkv*D contiguous
+ * elements each) of src_dtype (MXFP4_DT_*) -> MXFP4 rows, bit-exact to
+ * mxfp4_quantize_rows.  Tokens outside the cache, or on no page, write nothing.
+ * Two tokens of one call that share a row (a table that names a page twice, where
+ * it is written) leave a mixture of both there.
+ */
+int mxfp4_kv4_write(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq, uint8_t* ks,
+                    uint8_t* vq, uint8_t* vs, const int32_t* pages, int n_pages, int page, int max_pages,
+                    const int32_t* dpos, int B, int M, int Hkv, int D, void* stream);
+
+/* mxfp4_kv4_read: positions start[b] .. start[b] + n - 1 of every sequence
+ * (start device int32 (B), NULL: 0) as k, v (B, n, Hkv, D) of dst_dtype,
+ * 16-byte aligned.  bf16 and fp32 hold every value exactly as far as they reach
+ * (past it: infinite); fp16 is rounded to nearest even.  Zeros where a position
+ * lies outside the cache or on no page. */
+int mxfp4_kv4_read(const uint8_t* kq, const uint8_t* ks, const uint8_t* vq, const uint8_t* vs, const int32_t* pages,
+                   int n_pages, int page, int max_pages, const int32_t* start, void* k, void* v, int dst_dtype, int B,
+                   int n, int Hkv, int D, void* stream);
+
+/* mxfp4_qk_norm_rope_kv4: mxfp4_qk_norm_rope_kv with this cache: qkv fp32 (B*M,
+ * (Hq + 2 Hkv) * D) -> q_out bf16 (B*M, Hq, D), the same bits as there, and k
+ * and bf16(v) to the cache, the bits of mxfp4_kv4_write of those bf16 rows.
+ * D = 128. */
+int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k_norm_w, float eps, float theta,
+                           uint8_t* kq, uint8_t* ks, uint8_t* vq, uint8_t* vs, const int32_t* pages, int n_pages,
+                           int page, int max_pages, const int32_t* dpos, int B, int M, int Hq, int Hkv, int D,
+                           void* q_out, void* stream);
+
+/* mxfp4_attn_kv4: o = softmax(q K^T / sqrt(D)) V for M tokens of each sequence,
+ * token m of sequence b over positions 0 .. dpos[b] + m of its cache, without
+ * those on no page.
+ *   q          bf16 or fp16 (q_dtype), B*M tokens ldq elements apart (a multiple
+ *              of 8, q 16-byte aligned), Hq * D contiguous elements each; Hq a
+ *              multiple of Hkv
+ *   o          (B*M, Hq, D) of o_dtype (MXFP4_DT_*), 16-byte aligned, or NULL
+ *   oq, os     the MXFP4 rows of bf16(o), u8 (B*M, Hq*D/2) and (B*M, Hq*D/32), or
+ *              both NULL
+ *   workspace  16-byte aligned, mxfp4_attn_kv4_workspace_size(B, M, Hq, Hkv, D,
+ *              max_pos) bytes (0: may be NULL); nothing persists, but calls that
+ *              share one must be stream-ordered
+ * Sums and softmax in fp32.  A token outside [0, max_pos), or one that sees no
+ * position, gets zeros.  What the cache holds past dpos[b] + M - 1 is without
+ * effect, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
+ * The sums of a token are rounded in an order that depends on the batch's
+ * lengths, not on when the workgroups run: the same call gives the same bits.
+ */
+size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos);
+int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,
+                   const uint8_t* vs, const int32_t* pages, int n_pages, int page, int max_pages, const int32_t* dpos,
+                   void* o, int o_dtype, uint8_t* oq, uint8_t* os, int B, int M, int Hq, int Hkv, int D,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
  * Fused decode MoE layer, one launch per layer, batch 1.
  * Replaces the per-layer sequence prequant -> moe_gateup -> moe_down ->
  * moe_combine -> `x + moe.bfloat16()` of runtime/model_runner_v2.py:185-208

@@ -78,6 +78,15 @@ SIGNATURES = {
     "mxfp4_attn_decode_fused": (_c_i, [_c_p, _c_p, _c_p, ctypes.c_float, ctypes.c_float, _c_p, _c_p, _c_p, _c_p,
                                        _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_sz, _c_p]),
     "mxfp4_kv_write": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_p]),
+    "mxfp4_kv4_write": (_c_i, [_c_p, _c_p, _c_i, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_p,
+                               _c_i, _c_i, _c_i, _c_i, _c_p]),
+    "mxfp4_kv4_read": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i,
+                              _c_i, _c_p]),
+    "mxfp4_qk_norm_rope_kv4": (_c_i, [_c_p, _c_p, _c_p, ctypes.c_float, ctypes.c_float, _c_p, _c_p, _c_p, _c_p, _c_p,
+                                      _c_i, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_p]),
+    "mxfp4_attn_kv4_workspace_size": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "mxfp4_attn_kv4": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_i, _c_p,
+                              _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_sz, _c_p]),
     "mxfp4_moe_group": (_c_i, [_c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p]),
     "mxfp4_route_topk": (_c_i, [_c_p, _c_i64, _c_i, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p]),
     "mxfp4_route_tables": (_c_i, [_c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i,

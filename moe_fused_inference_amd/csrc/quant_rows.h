@@ -47,7 +47,31 @@ __device__ __forceinline__ void load8(const void* x, int64_t base, int k0, int K
     }
 }
 
+// MXFP4 of eight consecutive values of a 32-block, the block's other values in
+// the lane's quad: the packed nibbles and the block's scale code.
 // RND: 0 none, 1 round each element to fp16 first, 2 to bf16 first.
+template <int SRC, int RND>
+__device__ __forceinline__ uint32_t quantize8(float (&v)[8], uint32_t& code) {
+    if (RND == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mx::round_to_f16(v[i]);
+    }
+    if (RND == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mx::bf16_to_f32(mx::f32_to_bf16_rne(v[i]));
+    }
+    float am = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) am = fmaxf(am, __builtin_fabsf(v[i]));
+    // the block's four lanes: quad max by DPP
+    am = fmaxf(am, mx::dpp<mx::kDppQuadXor1>(am));
+    am = fmaxf(am, mx::dpp<mx::kDppQuadXor2>(am));
+    code = mx::e8m0_code(am);
+    // fp32 input without rounding keeps the software codes (up to 24 significant bits)
+    return (SRC == MXFP4_DT_F32 && RND == 0) ? mx::e2m1_pack8(v, mx::e8m0_inv_scale(code))
+                                             : mx::e2m1_pack8_short(v, mx::e8m0_inv_scale(code));
+}
+
 // Unit u (elements 8u .. 8u+7) of row `row`; rows >= M and units past the
 // row's Kp/8 write nothing.  Needs the four lanes of a 32-block in one quad.
 template <int SRC, int RND>
@@ -65,24 +89,8 @@ __device__ __forceinline__ void quantize_unit(const void* __restrict__ x, int64_
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     }
-    if (RND == 1) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = mx::round_to_f16(v[i]);
-    }
-    if (RND == 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = mx::bf16_to_f32(mx::f32_to_bf16_rne(v[i]));
-    }
-    float am = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) am = fmaxf(am, __builtin_fabsf(v[i]));
-    // the block's four lanes: quad max by DPP
-    am = fmaxf(am, mx::dpp<mx::kDppQuadXor1>(am));
-    am = fmaxf(am, mx::dpp<mx::kDppQuadXor2>(am));
-    const uint32_t code = mx::e8m0_code(am);
-    // fp32 input without rounding keeps the software codes (up to 24 significant bits)
-    const uint32_t packed = (SRC == MXFP4_DT_F32 && RND == 0) ? mx::e2m1_pack8(v, mx::e8m0_inv_scale(code))
-                                                              : mx::e2m1_pack8_short(v, mx::e8m0_inv_scale(code));
+    uint32_t code;
+    const uint32_t packed = quantize8<SRC, RND>(v, code);
     if (valid) {
         *reinterpret_cast<uint32_t*>(q + row * (int64_t)(Kp >> 1) + (u << 2)) = packed;
         if ((u & 3) == 0) s[row * (int64_t)(Kp >> 5) + (u >> 2)] = (uint8_t)code;

@@ -6,6 +6,8 @@
 //   decode  -- mxfp4_decode_ext  (src/ext/mxfp4_decode_binding.cpp:44-243):
 //              prequant, lin_pq, moe_gateup, moe_down, moe_combine,
 //              moe_gateup_tab, moe_down_tab, attn_decode, kv_write
+// and a third of this library's own:
+//   kv4     -- the MXFP4 KV cache: write, read, attn, attn_mx (kv4.py)
 // Names, argument order and meaning, output shapes and dtypes, and the
 // argument-check messages are the reference's.  Each op is a thin shim:
 // checks, torch allocations on the input's device (caching allocator), then
@@ -257,6 +259,158 @@ void kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor kvk, torch::Tensor
           "kv_write");
 }
 
+// ---- the MXFP4 KV cache (kv4.py) -----------------------------------------------
+
+// The cache tensors and where the batch's sequences lie in them, checked:
+// kq, vq u8 (n_pages, Hkv, page, D/2), ks, vs u8 (n_pages, Hkv, page, D/32),
+// pages int32 (B, max_pages) or none, at (dpos or start) int32 (B) or none.
+struct Kv4 {
+    uint8_t *kq, *ks, *vq, *vs;
+    const int32_t* pages;
+    const int32_t* at;
+    int n_pages, page, max_pages, B, Hkv, D;
+};
+
+int as_int(int64_t v, const char* msg) {
+    require(v >= 0 && v <= 0x7FFFFFFF, msg);
+    return (int)v;
+}
+
+Kv4 kv4_cache(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq, const torch::Tensor& vs,
+              const c10::optional<torch::Tensor>& pages, const c10::optional<torch::Tensor>& at, const char* at_msg) {
+    require(kq.is_cuda() && ks.is_cuda() && vq.is_cuda() && vs.is_cuda(), "cache tensors must be cuda");
+    require(kq.scalar_type() == torch::kUInt8 && ks.scalar_type() == torch::kUInt8 && vq.scalar_type() == torch::kUInt8 &&
+                vs.scalar_type() == torch::kUInt8,
+            "cache tensors must be uint8");
+    require(kq.dim() == 4 && ks.dim() == 4 && vq.sizes() == kq.sizes() && vs.sizes() == ks.sizes() &&
+                ks.size(0) == kq.size(0) && ks.size(1) == kq.size(1) && ks.size(2) == kq.size(2) &&
+                ks.size(3) * 16 == kq.size(3),
+            "kq/vq must be (n_pages,Hkv,page,D/2), ks/vs (n_pages,Hkv,page,D/32)");
+    require(kq.is_contiguous() && ks.is_contiguous() && vq.is_contiguous() && vs.is_contiguous(),
+            "cache tensors must be contiguous");
+    const auto dev = kq.device();
+    require(ks.device() == dev && vq.device() == dev && vs.device() == dev, "cache tensors must be on one device");
+    Kv4 c{u8m(kq), u8m(ks), u8m(vq), u8m(vs), nullptr, nullptr, 0, 0, 0, 0, 0, 0};
+    c.n_pages = as_int(kq.size(0), "too many pages");
+    c.Hkv = as_int(kq.size(1), "too many heads");
+    c.page = as_int(kq.size(2), "page too long");
+    c.D = as_int(kq.size(3) * 2, "head_dim too large");
+    c.B = c.n_pages;
+    if (pages.has_value()) {
+        require(pages->scalar_type() == torch::kInt32 && pages->dim() == 2 && pages->is_contiguous() && pages->device() == dev,
+                "pages must be a contiguous int32 (B,max_pages) tensor on the cache's device");
+        c.pages = static_cast<const int32_t*>(pages->data_ptr());
+        c.B = as_int(pages->size(0), "too many sequences");
+        c.max_pages = as_int(pages->size(1), "too many pages");
+    }
+    if (at.has_value()) {
+        require(at->scalar_type() == torch::kInt32 && at->is_contiguous() && at->device() == dev && at->numel() == c.B, at_msg);
+        c.at = static_cast<const int32_t*>(at->data_ptr());
+    }
+    return c;
+}
+
+// (B,M,H,D) of the cache's device whose tokens lie at one stride, H*D contiguous: itself, or a copy.
+torch::Tensor token_rows(const torch::Tensor& t) {
+    const bool ok = t.stride(3) == 1 && t.stride(2) == t.size(3) && t.stride(1) >= t.size(2) * t.size(3) &&
+                    (t.size(0) == 1 || t.stride(0) == t.size(1) * t.stride(1));
+    return ok ? t : t.contiguous();
+}
+int64_t token_stride(const torch::Tensor& t) {
+    return t.size(1) > 1 ? t.stride(1) : t.size(0) > 1 ? t.stride(0) : t.size(2) * t.size(3);
+}
+bool is_float16s(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kHalf; }
+
+void kv4_write(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& kq, const torch::Tensor& ks,
+               const torch::Tensor& vq, const torch::Tensor& vs, const torch::Tensor& dpos,
+               const c10::optional<torch::Tensor>& pages) {
+    const Kv4 c = kv4_cache(kq, ks, vq, vs, pages, dpos, "dpos must be a contiguous int32 (B,) tensor on the cache's device");
+    require(k.device() == kq.device() && v.device() == kq.device(), "k/v must be on the cache's device");
+    require((is_float16s(k) || k.scalar_type() == torch::kFloat32) && v.scalar_type() == k.scalar_type(),
+            "k/v must be bfloat16, float16 or float32, both of one type");
+    require(k.dim() == 4 && v.sizes() == k.sizes() && k.size(0) == c.B && k.size(2) == c.Hkv && k.size(3) == c.D,
+            "k/v must be (B,M,Hkv,D)");
+    const int M = as_int(k.size(1), "too many tokens");
+    if (M == 0 || c.B == 0) return;
+    const c10::DeviceGuard guard(kq.device());
+    const torch::Tensor kc = token_rows(k), vc = token_rows(v);
+    check(mxfp4_kv4_write(kc.data_ptr(), vc.data_ptr(), dtype_code(kc.scalar_type()), token_stride(kc), token_stride(vc), c.kq,
+                          c.ks, c.vq, c.vs, c.pages, c.n_pages, c.page, c.max_pages, c.at, c.B, M, c.Hkv, c.D, stream_of(kq)),
+          "kv4_write");
+}
+
+std::vector<torch::Tensor> kv4_read(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq,
+                                    const torch::Tensor& vs, int64_t n_, const c10::optional<torch::Tensor>& start,
+                                    const c10::optional<torch::Tensor>& pages, const py::object& dtype) {
+    const Kv4 c = kv4_cache(kq, ks, vq, vs, pages, start, "start must be a contiguous int32 (B,) tensor on the cache's device");
+    const auto dt = torch::python::detail::py_object_to_dtype(dtype);
+    require(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32, "dtype must be bfloat16, float16 or float32");
+    const int n = as_int(n_, "n must not be negative");
+    const c10::DeviceGuard guard(kq.device());
+    auto k = torch::empty({c.B, n, c.Hkv, c.D}, kq.options().dtype(dt));
+    auto v = torch::empty({c.B, n, c.Hkv, c.D}, kq.options().dtype(dt));
+    if (n != 0 && c.B != 0) {
+        check(mxfp4_kv4_read(c.kq, c.ks, c.vq, c.vs, c.pages, c.n_pages, c.page, c.max_pages, c.at, k.data_ptr(), v.data_ptr(),
+                             dtype_code(dt), c.B, n, c.Hkv, c.D, stream_of(kq)),
+              "kv4_read");
+    }
+    return {k, v};
+}
+
+// The attention of q (B,M,Hq,D) over the cache into o and / or oq, os (undefined: not wanted).
+void kv4_attn_into(const torch::Tensor& q, const Kv4& c, const torch::Tensor& kq, const torch::Tensor& o,
+                   const torch::Tensor& oq, const torch::Tensor& os) {
+    const int M = (int)q.size(1), Hq = (int)q.size(2);
+    const torch::Tensor qc0 = token_rows(q);
+    const bool aligned = (reinterpret_cast<uintptr_t>(qc0.data_ptr()) & 15) == 0 && token_stride(qc0) % 8 == 0;
+    const torch::Tensor qc = aligned ? qc0 : qc0.clone(at::MemoryFormat::Contiguous);
+    const int64_t max_pos = c.pages ? (int64_t)c.max_pages * c.page : c.page;
+    require(max_pos <= (1ll << 30), "attn_decode4: more than 2^30 positions a sequence");
+    const size_t wsb = mxfp4_attn_kv4_workspace_size(c.B, M, Hq, c.Hkv, c.D, (int)max_pos);
+    torch::Tensor ws;
+    if (wsb) ws = torch::empty({(int64_t)wsb}, kq.options());
+    check(mxfp4_attn_kv4(qc.data_ptr(), dtype_code(qc.scalar_type()), token_stride(qc), c.kq, c.ks, c.vq, c.vs, c.pages,
+                         c.n_pages, c.page, c.max_pages, c.at, o.defined() ? o.data_ptr() : nullptr,
+                         o.defined() ? dtype_code(o.scalar_type()) : 2, oq.defined() ? u8m(oq) : nullptr,
+                         os.defined() ? u8m(os) : nullptr, c.B, M, Hq, c.Hkv, c.D, wsb ? ws.data_ptr() : nullptr, wsb,
+                         stream_of(kq)),
+          "attn_decode4");
+}
+
+Kv4 kv4_attn_args(const torch::Tensor& q, const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq,
+                  const torch::Tensor& vs, const torch::Tensor& dpos, const c10::optional<torch::Tensor>& pages) {
+    const Kv4 c = kv4_cache(kq, ks, vq, vs, pages, dpos, "dpos must be a contiguous int32 (B,) tensor on the cache's device");
+    require(q.device() == kq.device() && is_float16s(q), "q must be bfloat16 or float16 on the cache's device");
+    require(q.dim() == 4 && q.size(0) == c.B && q.size(3) == c.D && q.size(2) > 0 && q.size(2) % c.Hkv == 0,
+            "q must be (B,M,Hq,D), Hq a multiple of Hkv");
+    as_int(q.size(1), "too many tokens");
+    as_int(q.size(2), "too many heads");
+    return c;
+}
+
+torch::Tensor kv4_attn(const torch::Tensor& q, const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq,
+                       const torch::Tensor& vs, const torch::Tensor& dpos, const c10::optional<torch::Tensor>& pages,
+                       const py::object& dtype) {
+    const Kv4 c = kv4_attn_args(q, kq, ks, vq, vs, dpos, pages);
+    const auto dt = torch::python::detail::py_object_to_dtype(dtype);
+    require(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32, "dtype must be bfloat16, float16 or float32");
+    const c10::DeviceGuard guard(kq.device());
+    auto o = torch::empty(q.sizes(), q.options().dtype(dt));
+    if (o.numel() != 0) kv4_attn_into(q, c, kq, o, torch::Tensor(), torch::Tensor());
+    return o;
+}
+
+std::vector<torch::Tensor> kv4_attn_mx(const torch::Tensor& q, const torch::Tensor& kq, const torch::Tensor& ks,
+                                       const torch::Tensor& vq, const torch::Tensor& vs, const torch::Tensor& dpos,
+                                       const c10::optional<torch::Tensor>& pages) {
+    const Kv4 c = kv4_attn_args(q, kq, ks, vq, vs, dpos, pages);
+    const c10::DeviceGuard guard(kq.device());
+    const int64_t T = q.size(0) * q.size(1), row = q.size(2) * q.size(3);
+    auto oq = torch::empty({T, row / 2}, kq.options()), os = torch::empty({T, row / 32}, kq.options());
+    if (T != 0) kv4_attn_into(q, c, kq, torch::Tensor(), oq, os);
+    return {oq, os};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(mxfp4_ext, m) {
@@ -275,4 +429,13 @@ PYBIND11_MODULE(mxfp4_ext, m) {
     dec.def("moe_down_tab", &moe_down_tab, "fused silu-down from device pointer tables");
     dec.def("attn_decode", &attn_decode, "decode attention over an E4M3 KV cache -> f32 (M,Hq,D)");
     dec.def("kv_write", &kv_write, "E4M3 KV write of M tokens at rows dpos+m");
+    auto k4 = m.def_submodule("kv4", "the MXFP4 KV cache");
+    k4.def("write", &kv4_write, py::arg("k"), py::arg("v"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"),
+           py::arg("dpos"), py::arg("pages"), "k, v (B,M,Hkv,D) -> MXFP4 rows at dpos[b]+m");
+    k4.def("read", &kv4_read, py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("n"), py::arg("start"),
+           py::arg("pages"), py::arg("dtype"), "positions start[b] .. start[b]+n-1 -> [k, v] (B,n,Hkv,D)");
+    k4.def("attn", &kv4_attn, py::arg("q"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("dpos"),
+           py::arg("pages"), py::arg("dtype"), "attention over the MXFP4 cache -> (B,M,Hq,D)");
+    k4.def("attn_mx", &kv4_attn_mx, py::arg("q"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("dpos"),
+           py::arg("pages"), "attn as the MXFP4 rows of its bf16 rounding -> [oq, os]");
 }
