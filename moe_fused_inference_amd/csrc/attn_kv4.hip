@@ -28,6 +28,9 @@
 #include "mx_device.h"
 #include "mx_host.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 using kv4::Cache;
@@ -36,7 +39,10 @@ constexpr int kUnit = 32;              // positions per wave and step
 constexpr float kSlack = 8.0f;         // a term is at most 2^8
 constexpr float kWide = 262144.0f;     // a reference past it: an exponent's rounding is up to 2^-6 and more
 constexpr float kNone = -3e38f;        // the reference of a row that has seen nothing: exp2(-inf - kNone) = 0
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 constexpr int kMaxRT = 2;              // 16-row tiles per workgroup
+constexpr int kFew = 32;               // shares of a sequence that four waves merge at once
+constexpr int kMinShare = 4;           // units, one a wave
 constexpr int kParts = 3;              // bf16 parts of a probability
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -55,71 +61,81 @@ struct Args {
     const int32_t* dpos;
     float* part;
     mxa::Out out;
-    int B, M, Hq, G, shares;     // shares: how many there may be, over the batch
+    int B, M, Hq, G, shares, wanted;   // shares: how many there may be, over the batch
     float scale;                 // log2(e) / sqrt(D)
 };
 
-// Units of sequence b, and what a share holds: equal whole rounds of the four waves.
-__device__ __forceinline__ int units_of(const Args& a, int b) {
+// Units of sequence b.
+__device__ __forceinline__ uint32_t units_of(const Args& a, int b) {
     const int64_t n = (int64_t)a.dpos[b] + a.M;
-    const int np = (int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos);
-    return (np + kUnit - 1) / kUnit;
+    return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
 }
-__device__ __forceinline__ int share_of(int64_t units, int wanted) {
-    const int64_t per = (units + wanted - 1) / wanted;
-    return (int)(per < 4 ? 4 : (per + 3) & ~3ll);
-}
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+// Inclusive prefix sums over the wave (every lane active).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr 1, 2, 4, 8: within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15: row 0's total to row 1, 2's to 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast 31: the first half's to the second
     return v;
 }
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ uint32_t shares_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
 
-// The share's units, and for share number `at` of the batch its sequence b and its
-// number there, or for at < 0 the first share of sequence b.  Every wave finds them
-// by itself: a lane per sequence, sums over the wave.
+// Units of a share for `total` units in the batch: a.wanted of them, in whole rounds of
+// the four waves, two rounds at least from 32 shares a sequence on (fewer records to
+// merge; one token, us with at least 1 / 2 rounds: 4096 positions 8.2 / 9.0, 8000 9.8 /
+// 9.1, 32000 16.4 / 13.5).
+__device__ __forceinline__ uint32_t share_units(uint64_t total, const Args& a) {
+    const uint32_t per = (uint32_t)((total + a.wanted - 1) / a.wanted + 3) & ~3u;
+    return max(per, total > (uint64_t)kFew * kMinShare * a.B ? 2u * kMinShare : (uint32_t)kMinShare);
+}
+
+// What a share holds -- the same whole rounds of the four waves for every sequence, so
+// few units that the batch has at most a.wanted shares, or a few more -- and for share
+// number `at` of the batch its sequence b and its number s there, or for at < 0 the
+// batch's number of sequence b's first share.  Every wave finds them by itself: a lane
+// per sequence, sums over the wave.  All uniform.
 struct Place {
     int per, b, s, first;
 };
 __device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
     const int lane = threadIdx.x & 63;
-    const int wanted = a.shares - a.B;      // the rounding up costs at most one a sequence
+    auto units = [&](int b0) { return b0 + lane < a.B ? units_of(a, b0 + lane) : 0u; };
     if (a.B == 1) {
-        const int nu = units_of(a, 0);
-        p.per = share_of(nu, wanted);
-        p.first = 0;
-        p.b = 0;
+        const uint32_t nu = units_of(a, 0);
+        p.per = (int)share_units(nu, a);
+        p.first = p.b = 0;
         p.s = at;
-        return at < 0 || at * (int64_t)p.per < nu;
+        return at < 0 || (int64_t)at * p.per < nu;
     }
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) total += b0 + lane < a.B ? units_of(a, b0 + lane) : 0;
-    p.per = share_of(wave_sum(total), wanted);
+    const uint32_t u0 = units(0);
+    uint64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) total += last_lane(wave_scan(b0 ? units(b0) : u0));
+    uint32_t per = share_units(total, a);
+    for (int i = 0; i < 3; ++i) {      // a sequence's last share is a part of one: longer ones until they are few enough
+        uint32_t n = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) n += last_lane(wave_scan(shares_of(b0 ? units(b0) : u0, per)));
+        if (n <= (uint32_t)a.wanted) break;
+        per = max(per + 4, (uint32_t)((uint64_t)per * n / a.wanted + 3) & ~3u);
+    }
+    p.per = (int)per;
     int before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int ns = b0 + lane < a.B ? (units_of(a, b0 + lane) + p.per - 1) / p.per : 0;
-        int upto = ns;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(upto, o);
-            if (lane >= o) upto += t;
-        }
-        if (at < 0) {
-            if (p.b < b0 + 64) {
-                p.first = before + __builtin_amdgcn_readlane(upto - ns, p.b - b0);
-                return true;
-            }
-        } else {
+        const int ns = (int)shares_of(b0 ? units(b0) : u0, per), upto = (int)wave_scan(ns);
+        int l = p.b - b0;
+        if (at >= 0) {
             const uint64_t past = __ballot(before + upto > at);
-            if (past) {
-                const int l = (int)__builtin_ctzll(past);
-                p.b = b0 + l;
-                p.first = before + __builtin_amdgcn_readlane(upto - ns, l);
-                p.s = at - p.first;
-                return true;
-            }
+            l = past ? (int)__builtin_ctzll(past) : 64;
         }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        if (l < 64) {
+            p.b = b0 + l;
+            p.first = before + __builtin_amdgcn_readlane(upto - ns, l);
+            p.s = at - p.first;
+            return true;
+        }
+        before += (int)last_lane(upto);
     }
     return false;
 }
@@ -129,12 +145,11 @@ __device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
 // V: positions 16 t + 4 lq + i, columns D/16 l16 ..; a position's codes as one word.
 template <int D>
 struct Raw {
-    typedef uint32_t kvec __attribute__((ext_vector_type(D / 32)));
-    typedef uint32_t svec __attribute__((ext_vector_type(D / 32)));   // four positions' codes
-    kvec k[2];
+    typedef uint32_t vec __attribute__((ext_vector_type(D / 32)));
+    vec k[2];
     uint32_t ks[2];
     uint32_t v[8];
-    svec vs[2];
+    vec vs[2];      // four positions' codes
 };
 
 // Lane offsets into a tile's rows, in bytes.
@@ -150,65 +165,56 @@ struct Lane {
     }
 };
 
+// row[t]: tile t's first head row (uniform).
 template <int D>
-__device__ __forceinline__ void load_k(Raw<D>& r, const Cache& c, const int64_t (&row)[2], const Lane<D>& o) {
+__device__ __forceinline__ void load_k(Raw<D>& r, const Cache& c, const uint32_t (&row)[2], const Lane<D>& o) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        r.k[t] = *reinterpret_cast<const typename Raw<D>::kvec*>(c.kq + row[t] * (D / 2) + o.k);
-        r.ks[t] = *(c.ks + row[t] * (D / 32) + o.ks);
+        r.k[t] = *reinterpret_cast<const typename Raw<D>::vec*>(c.kq + (uint64_t)row[t] * (D / 2) + o.k);
+        r.ks[t] = *(c.ks + (uint64_t)row[t] * (D / 32) + o.ks);
     }
 }
 template <int D>
-__device__ __forceinline__ void load_v(Raw<D>& r, const Cache& c, const int64_t (&row)[2], const Lane<D>& o) {
+__device__ __forceinline__ void load_v(Raw<D>& r, const Cache& c, const uint32_t (&row)[2], const Lane<D>& o) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const uint8_t* p = c.vq + row[t] * (D / 2);
+        const uint8_t* p = c.vq + (uint64_t)row[t] * (D / 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (D == 128) r.v[4 * t + i] = *reinterpret_cast<const uint32_t*>(p + (o.v + i * (D / 2)));
             else r.v[4 * t + i] = *reinterpret_cast<const uint16_t*>(p + (o.v + i * (D / 2)));
         }
-        r.vs[t] = *reinterpret_cast<const typename Raw<D>::svec*>(c.vs + row[t] * (D / 32) + o.vs);
+        r.vs[t] = *reinterpret_cast<const typename Raw<D>::vec*>(c.vs + (uint64_t)row[t] * (D / 32) + o.vs);
     }
 }
 
-// MFMA operands: kd[tile][kt] (positions x 8 dimensions), vd[c] (columns D/16 l16 + c x 8 positions).
+// The scales of the lane's eight V positions, for the packed conversions, which read
+// the exponent field alone: the code rotated there, its neighbours around it.
 template <int D>
-__device__ __forceinline__ void decode_k(const Raw<D>& r, uint4 (&kd)[2][D / 32]) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int kt = 0; kt < D / 32; ++kt) kd[t][kt] = kv4::eight_bf16(r.k[t][kt], kv4::scale_of(r.ks[t]));
-}
-template <int D>
-__device__ __forceinline__ void decode_v(const Raw<D>& r, uint4 (&vd)[D / 16]) {
+__device__ __forceinline__ void v_scales(const Raw<D>& r, float (&s)[8]) {
     const int l16 = threadIdx.x & 15;
-    uint32_t o[D / 16][4];
+    const uint32_t turn = (D == 128 ? 8 * (l16 >> 2) : 8 * (l16 >> 3)) + 9;
 #pragma unroll
-    for (int p2 = 0; p2 < 4; ++p2) {       // positions 2 p2, 2 p2 + 1 of the lane's eight
-        uint32_t x[2][D / 32];             // a position's columns, two a word
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w = D == 128 ? r.vs[i >> 2][i & 3] : r.vs[i >> 2][(i & 3) >> 1];
+        s[i] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, D == 64 && (i & 1) ? turn + 16 : turn));
+    }
+}
+// MFMA operands of four column tiles: columns D/16 l16 + 4 H + c x the lane's eight positions.
+template <int H>
+__device__ __forceinline__ void decode_v(const uint32_t (&v)[8], const float (&s)[8], uint4 (&vd)[4]) {
+    uint32_t o[4][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int i = 2 * p2 + j;
-            uint32_t code;
-            if constexpr (D == 128) code = (r.vs[i >> 2][i & 3] >> (8 * (l16 >> 2))) & 0xFFu;
-            else code = (r.vs[i >> 2][(i & 3) >> 1] >> (16 * (i & 1) + 8 * (l16 >> 3))) & 0xFFu;
-            const float s = kv4::scale_of(code);
-            x[j][0] = kv4::pair_bf16<0>(r.v[i], s);
-            x[j][1] = kv4::pair_bf16<1>(r.v[i], s);
-            if constexpr (D == 128) {
-                x[j][2] = kv4::pair_bf16<2>(r.v[i], s);
-                x[j][3] = kv4::pair_bf16<3>(r.v[i], s);
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-            o[2 * w][p2] = __builtin_amdgcn_perm(x[1][w], x[0][w], 0x05040100u);
-            o[2 * w + 1][p2] = __builtin_amdgcn_perm(x[1][w], x[0][w], 0x07060302u);
-        }
+    for (int p2 = 0; p2 < 4; ++p2) {       // positions 2 p2, 2 p2 + 1
+        const uint32_t a0 = kv4::pair_bf16<2 * H>(v[2 * p2], s[2 * p2]), a1 = kv4::pair_bf16<2 * H + 1>(v[2 * p2], s[2 * p2]);
+        const uint32_t b0 = kv4::pair_bf16<2 * H>(v[2 * p2 + 1], s[2 * p2 + 1]), b1 = kv4::pair_bf16<2 * H + 1>(v[2 * p2 + 1], s[2 * p2 + 1]);
+        o[0][p2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+        o[1][p2] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+        o[2][p2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+        o[3][p2] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
     }
 #pragma unroll
-    for (int cc = 0; cc < D / 16; ++cc) vd[cc] = make_uint4(o[cc][0], o[cc][1], o[cc][2], o[cc][3]);
+    for (int c = 0; c < 4; ++c) vd[c] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
 }
 
 // Eight fp32 terms as bf16 parts whose sum each is (8 bits a part, rounded to nearest, the rest exact).
@@ -227,6 +233,14 @@ __device__ __forceinline__ void parts(float (&t)[8], uint4 (&p)[N]) {
         }
         p[j] = make_uint4(o[0], o[1], o[2], o[3]);
     }
+}
+
+// The largest of three, a NaN among them left out (as fmaxf, whose operands the
+// compiler would first pass through an instruction each).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 // a * b rounded, minus c: not one fma.
@@ -260,239 +274,231 @@ __device__ __forceinline__ void q_parts(uint4 w, uint4 (&p)[NQ]) {
     }
 }
 
-template <int D, int RT, int NQ, bool ONE>
-__global__ __launch_bounds__(256, 2) void attn_kv4_kernel(Args a) {
+template <int D, int RT, int NQ, bool ONE, int NW>
+__global__ __launch_bounds__(64 * NW, RT == 1 ? 4 : 2) void attn_kv4_kernel(Args a) {
     constexpr int R = 16 * RT, KT = D / 32, CT = D / 16;
-    __shared__ __align__(16) uint16_t qs[RT > 1 ? NQ * R : 1][D + 8];
-    __shared__ __align__(16) float mo[4][16][D + 4];
-    __shared__ float mm[4][16], ml[4][16];
+    // q, and after the last unit the waves' sums
+    __shared__ union Lds {
+        alignas(16) uint16_t qs[NQ * R][D + 8];
+        alignas(16) float mo[NW][16][D + 4];
+    } lds;
+    auto& qs = lds.qs;
+    auto& mo = lds.mo;
+    __shared__ float mm[NW][16], ml[NW][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lq = lane >> 4;
     const int g = blockIdx.y, r0 = blockIdx.z * R, G = a.G;
     const int rows = a.M * G;
-    Place pl;
+    int b = 0, u0 = 0, u1 = INT32_MAX;
     if constexpr (ONE) {
-        pl.b = blockIdx.x;
-        pl.s = 0;
+        b = blockIdx.x;
     } else {
+        Place pl;
         if (!find_share(a, blockIdx.x, pl)) return;        // uniform
-    }
-    const int b = pl.b;
-    const int64_t base = a.dpos[b];
-    const int64_t last = base + a.M - 1 < a.c.max_pos - 1 ? base + a.M - 1 : a.c.max_pos - 1;   // positions past it are no one's
-    int u0 = 0, u1 = (int)((last + kUnit) / kUnit);
-    if constexpr (!ONE) {
+        b = pl.b;
         u0 = pl.s * pl.per;
-        u1 = min(u1, u0 + pl.per);
+        u1 = u0 + pl.per;
     }
-    // the group's last token sees no further
-    const int64_t lim_min = base + r0 / G;                  // the first token of the group sees up to here
-    const int64_t lim_max = base + (min(r0 + R, rows) - 1) / G;
-    u1 = (int)(lim_max < (int64_t)u1 * kUnit ? (lim_max + kUnit) / kUnit : u1);
+    // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
+    const int64_t base = __builtin_amdgcn_readfirstlane(a.dpos[b]);
+    auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
+    const int last = min(clamped(base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
+    const int lim_min = clamped(base + r0 / G);                          // the group's first token sees up to here
+    const int lim_max = min(clamped(base + (min(r0 + R, rows) - 1) / G), a.c.max_pos - 1);   // its last one
+    u1 = min(u1, (lim_max + kUnit) / kUnit);
     if (!ONE && u0 >= u1) return;                           // no record: the merge reads none
-    // the pages of the wave's units u0 + wave + 4 j, j = lane, tiles 0 and 1 (-1: none)
-    int pid[2];
-    auto load_pages = [&](int j0) {
+    // q, whose parts go to LDS once the first units' loads are on their way
+    const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
+    constexpr int NT = 64 * NW, QN = (R * (D / 8) + NT - 1) / NT;
+    uint4 qw[QN];
+#pragma unroll
+    for (int i = 0; i < QN; ++i) {
+        const int r = r0 + (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+        qw[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows && (R * (D / 8) % NT == 0 || tid + NT * i < R * (D / 8)))
+            qw[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)(r / G) * a.ldq + (r % G) * D + 8 * ch);
+    }
+    // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
+    uint32_t first[2];
+    auto find_rows = [&](int j0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int64_t pos = ((int64_t)u0 + wave + 4 * (j0 + lane)) * kUnit + 16 * t;
-            pid[t] = -1;
+            const int64_t pos = ((int64_t)u0 + wave + NW * (j0 + lane)) * kUnit + 16 * t;
+            first[t] = kNoRow;
             if (pos < a.c.max_pos) {
-                pid[t] = b;
-                if (a.c.pages) {
-                    const int id = a.c.pages[(int64_t)b * a.c.max_pages + (pos >> a.c.lg)];
-                    pid[t] = (uint32_t)id < (uint32_t)a.c.n_pages ? id : -1;
-                }
+                const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
+                first[t] = row < 0 ? kNoRow : (uint32_t)row;
             }
         }
     };
     const Lane<D> off(lane);
-    // unit u, the wave's j-th: its tiles' first head rows, and which of them exist
-    auto locate = [&](int u, int j, int64_t (&row)[2]) -> int {
-        int there = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int id = __builtin_amdgcn_readlane(pid[t], j & 63);
-            const int pos = u * kUnit + 16 * t;
-            const int in = a.c.pages ? pos & (a.c.page - 1) : pos;
-            there |= id >= 0 ? 1 << t : 0;
-            row[t] = id >= 0 ? ((int64_t)id * a.c.Hkv + g) * a.c.page + in : (int64_t)g * a.c.page;
-        }
-        return there;
+    // the wave's j-th unit: its tiles' rows, and which of them exist
+    auto locate = [&](int j, uint32_t (&row)[2]) -> int {
+        const uint32_t r0 = __builtin_amdgcn_readlane(first[0], j & 63), r1 = __builtin_amdgcn_readlane(first[1], j & 63);
+        row[0] = r0 == kNoRow ? 0 : r0;
+        row[1] = r1 == kNoRow ? 0 : r1;
+        return (r0 == kNoRow ? 0 : 1) | (r1 == kNoRow ? 0 : 2);
     };
-    // q: one tile's operands straight into registers, more through LDS.  zero[rt]: 0, or
-    // NaN where the row holds an infinity or a NaN (then so is its output)
-    const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
-    auto q_row = [&](int r) { return qb + (int64_t)(r / G) * a.ldq + (r % G) * D; };
-    uint4 q1[RT > 1 ? 1 : KT][NQ];
-    float zero[RT];
+    Raw<D> r;
+    int there = 0;
+    if (u0 + wave < u1) {
+        uint32_t row[2];
+        find_rows(0);
+        there = locate(0, row);
+        load_k(r, a.c, row, off);
+        load_v(r, a.c, row, off);
+    }
     auto check = [](uint4 w) {
         const uint32_t x[4] = {w.x, w.y, w.z, w.w};
         float z = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint16_t e = (uint16_t)(x[i / 2] >> (16 * (i & 1)));
-            z = fmaf(NQ == 1 ? mx::bf16_to_f32(e) : mx::f16_to_f32(e), 0.0f, z);
-        }
+        for (int i = 0; i < 8; ++i) z = fmaf(mx::bf16_to_f32((uint16_t)(x[i / 2] >> (16 * (i & 1)))), 0.0f, z);
         return z;
     };
-    if constexpr (RT == 1) {
-        zero[0] = 0.0f;
-        const uint16_t* row = q_row(min(r0 + l16, rows - 1)) + (D / 4) * lq;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            uint4 w = *reinterpret_cast<const uint4*>(row + 8 * kt);
-            if (r0 + l16 >= rows) w = make_uint4(0, 0, 0, 0);
-            zero[0] += check(w);
-            q_parts<NQ>(w, q1[kt]);
-        }
-        zero[0] = over_lq<false>(zero[0]);
-    } else {
-        for (int i = tid; i < R * (D / 8); i += 256) {
-            const int r = i / (D / 8), ch = i % (D / 8);
-            uint4 w = make_uint4(0, 0, 0, 0), p[NQ];
-            if (r0 + r < rows) w = *reinterpret_cast<const uint4*>(q_row(r0 + r) + 8 * ch);
-            q_parts<NQ>(w, p);
+    for (int i = 0; i < QN; ++i) {
+        const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+        uint4 p[NQ];
+        q_parts<NQ>(qw[i], p);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) *reinterpret_cast<uint4*>(&qs[j * R + r][8 * ch]) = p[j];
-        }
+        for (int j = 0; j < NQ; ++j)
+            if (R * (D / 8) % NT == 0 || r < R) *reinterpret_cast<uint4*>(&qs[j * R + r][8 * ch]) = p[j];
     }
-    // the lane's query of tile rt: row r0 + 16 rt + l16; rows that are none see everything and write nothing
-    int64_t lim[RT];
+    __syncthreads();
+    // 0, or NaN where the row holds an infinity or a NaN (then so is its output)
+    float zero[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + 16 * rt + l16;
-        lim[rt] = r < rows ? base + r / G : INT64_MAX;
+        zero[rt] = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) zero[rt] += check(*reinterpret_cast<const uint4*>(&qs[16 * rt + l16][(D / 4) * lq + 8 * kt]));
+        zero[rt] = over_lq<false>(zero[rt]);
     }
+    // the lane's query of tile rt: row r0 + 16 rt + l16; rows that are none see everything and write nothing
+    int lim[RT];
     float m[RT], l[RT];
     bool wide[RT];   // uniform: a row's reference is past kWide
     mx::v4f acc[RT][CT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+        const int r = r0 + 16 * rt + l16;
+        lim[rt] = r < rows ? clamped(base + r / G) : 1 << 30;
         m[rt] = kNone;
         l[rt] = 0.0f;
         wide[rt] = false;
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[rt][c] = mx::v4f{0.f, 0.f, 0.f, 0.f};
     }
-    if constexpr (RT > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            zero[rt] = 0.0f;
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const uint4 w = *reinterpret_cast<const uint4*>(&qs[16 * rt + l16][(D / 4) * lq + 8 * kt]);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) zero[rt] = fmaf(mx::bf16_to_f32((uint16_t)(x[i / 2] >> (16 * (i & 1)))), 0.0f, zero[rt]);
-            }
-            zero[rt] = over_lq<false>(zero[rt]);
-        }
-    }
-    Raw<D> raw;
-    int there = 0;
-    if (u0 + wave < u1) {
-        int64_t row[2];
-        load_pages(0);
-        there = locate(u0 + wave, 0, row);
-        load_k(raw, a.c, row, off);
-        load_v(raw, a.c, row, off);
-    }
-    for (int u = u0 + wave, j = 0; u < u1; u += 4, ++j) {
-        const int64_t p0 = (int64_t)u * kUnit;
-        const bool more = u + 4 < u1;
-        int64_t next[2] = {0, 0};
+    // Unit u, the wave's j-th.  `more`: the wave's next one is loaded meanwhile (decided in the code, not by a branch:
+    // behind one the compiler waits for the older loads as if these had not been issued, that is for all)
+    auto unit = [&](int u, int j, auto more_) {
+        constexpr bool more = decltype(more_)::value;
+        const int p0 = u * kUnit;
+        uint32_t next[2];
         int there_next = 0;
-        if (more) {
-            if (((j + 1) & 63) == 0) load_pages(j + 1);
-            there_next = locate(u + 4, j + 1, next);
+        if constexpr (more) {
+            if (((j + 1) & 63) == 0) find_rows(j + 1);
+            there_next = locate(j + 1, next);
         }
-        uint4 kd[2][KT];
-        decode_k(raw, kd);
-        if (more) load_k(raw, a.c, next, off);
+        mx::v4f s[RT][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            uint4 kd[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) kd[kt] = kv4::eight_bf16(r.k[t][kt], kv4::scale_of(r.ks[t]));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                s[rt][t] = mx::v4f{zero[rt], zero[rt], zero[rt], zero[rt]};
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        const uint4 qf = *reinterpret_cast<const uint4*>(&qs[n * R + 16 * rt + l16][(D / 4) * lq + 8 * kt]);
+                        s[rt][t] = mfma_bf16(kd[kt], qf, s[rt][t]);
+                    }
+            }
+        }
+        if constexpr (more) load_k(r, a.c, next, off);
+        // s[rt][t][i]: position p0 + 16 t + 4 lq + i
         uint4 p[RT][kParts];
-        const bool masked = p0 + kUnit - 1 > lim_min || there != 3;   // uniform
+        const bool masked = __builtin_amdgcn_readfirstlane(p0 + kUnit - 1 > lim_min || there != 3);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            if (rt > 0 && r0 + 16 * rt >= rows) break;
-            mx::v4f s[2];
-            s[0] = s[1] = mx::v4f{zero[rt], zero[rt], zero[rt], zero[rt]};
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    uint4 qf;
-                    if constexpr (RT == 1) qf = q1[kt][n];
-                    else qf = *reinterpret_cast<const uint4*>(&qs[n * R + 16 * rt + l16][(D / 4) * lq + 8 * kt]);
-                    s[0] = mfma_bf16(kd[0][kt], qf, s[0]);
-                    s[1] = mfma_bf16(kd[1][kt], qf, s[1]);
-                }
-            // s[t][i]: position p0 + 16 t + 4 lq + i
             if (masked) {
+                int sees = lim[rt] - p0 - 4 * lq;    // -1 or less: none of the lane's positions
+                asm volatile("" : "+v"(sees));       // (nothing below it is computed ahead of the branch)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (!(there >> t & 1) || p0 + 16 * t + 4 * lq + i > lim[rt]) s[t][i] = -INFINITY;
+                        if (!(there >> t & 1) || 16 * t + i > sees) s[rt][t][i] = -INFINITY;
             }
-            const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            const float top = max3(max3(s[rt][0][0], s[rt][0][1], s[rt][0][2]), max3(s[rt][0][3], s[rt][1][0], s[rt][1][1]),
+                                   max3(s[rt][1][2], s[rt][1][3], s[rt][1][3]));
             if (__ballot(top * a.scale > m[rt] + kSlack)) {
                 const float mn = fmaxf(m[rt], over_lq<true>(top) * a.scale);
-                if (u != u0 + wave) {
-                    const float al = __builtin_amdgcn_exp2f(m[rt] - mn);
-                    l[rt] *= al;
+                const float al = __builtin_amdgcn_exp2f(m[rt] - mn);
+                l[rt] *= al;
 #pragma unroll
-                    for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CT; ++c)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[rt][c][i] *= al;
-                }
+                    for (int i = 0; i < 4; ++i) acc[rt][c][i] *= al;
                 m[rt] = mn;
                 wide[rt] = __ballot(fabsf(mn) > kWide && mn != kNone) != 0ull;
             }
             float t[8];
             if (!wide[rt]) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = fmaf(s[i >> 2][i & 3], a.scale, -m[rt]);
+                for (int i = 0; i < 8; ++i) t[i] = fmaf(s[rt][i >> 2][i & 3], a.scale, -m[rt]);
             } else {   // the rounded product, as in m: the fma's would differ from it by more than a term
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = mul_then_sub(s[i >> 2][i & 3], a.scale, m[rt]);
+                for (int i = 0; i < 8; ++i) t[i] = mul_then_sub(s[rt][i >> 2][i & 3], a.scale, m[rt]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(t[i]);
             l[rt] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
             parts<kParts>(t, p[rt]);
         }
-        if (masked) {   // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
+        __builtin_amdgcn_sched_barrier(0);   // 128 registers, four waves a SIMD: no operand of the second product before here,
+        float vs[8];
+        v_scales(r, vs);
+        if (masked) {
+            // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
+            int sees = last - p0 - 4 * lq;
+            asm volatile("" : "+v"(sees));
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (!(there >> (i >> 2) & 1) || p0 + 16 * (i >> 2) + 4 * lq + (i & 3) > last) {
-                    raw.v[i] = 0;
-                    if constexpr (D == 128) raw.vs[i >> 2][i & 3] = 0x7F7F7F7Fu;
-                    else raw.vs[i >> 2][(i & 3) >> 1] = (i & 1) ? (raw.vs[i >> 2][(i & 3) >> 1] & 0xFFFFu) | 0x7F7F0000u
-                                                                : (raw.vs[i >> 2][(i & 3) >> 1] & 0xFFFF0000u) | 0x7F7Fu;
+                if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) {
+                    r.v[i] = 0;
+                    vs[i] = 1.0f;
                 }
         }
-        uint4 vd[CT];
-        decode_v(raw, vd);
-        if (more) load_v(raw, a.c, next, off);
+        auto product = [&](auto half) {
+            constexpr int H = decltype(half)::value;
+            uint4 vd[4];
+            decode_v<H>(r.v, vs, vd);
+            if constexpr (H == CT / 4 - 1 && more) load_v(r, a.c, next, off);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int k = kParts - 1; k >= 0; --k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[rt][4 * H + c] = mfma_bf16(vd[c], p[rt][k], acc[rt][4 * H + c]);
+        };
+        product(std::integral_constant<int, 0>{});
+        __builtin_amdgcn_sched_barrier(0);   // and one half's at a time
+        if constexpr (CT == 8) product(std::integral_constant<int, 1>{});
         there = there_next;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (rt > 0 && r0 + 16 * rt >= rows) break;
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int k = kParts - 1; k >= 0; --k) acc[rt][c] = mfma_bf16(vd[c], p[rt][k], acc[rt][c]);
-        }
-    }
-    // the four waves' sums of each tile in LDS, then one record (or the output) per
+    };
+    int u = u0 + wave, j = 0;
+    for (; u + NW < u1; u += NW, ++j) unit(u, j, std::true_type{});
+    if (u < u1) unit(u, j, std::false_type{});
+    // the waves' sums of each tile in LDS, then one record (or the output) per
     // row: acc[rt][c][i] is column D/16 (4 lq + i) + c of query l16
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        if (rt > 0) __syncthreads();
+        __syncthreads();
         const float ls = over_lq<false>(l[rt]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -508,15 +514,17 @@ __global__ __launch_bounds__(256, 2) void attn_kv4_kernel(Args a) {
         // thread: CT columns of a row (8 of 128, 4 of 64)
         const int qr = tid >> 4, c0 = CT * (tid & 15);
         const int rr = r0 + 16 * rt + qr;
-        if (rr >= rows) continue;
+        if (tid >= 256 || rr >= rows) continue;
         const int64_t pos = base + rr / G;
-        if (!ONE && (pos < 0 || pos >= a.c.max_pos || (int64_t)u0 * kUnit > pos)) continue;   // no record: the merge reads none
-        const float gm = fmaxf(fmaxf(mm[0][qr], mm[1][qr]), fmaxf(mm[2][qr], mm[3][qr]));
+        if (!ONE && (pos < 0 || pos >= a.c.max_pos || u0 * kUnit > pos)) continue;   // no record: the merge reads none
+        float gm = mm[0][qr];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) gm = fmaxf(gm, mm[w][qr]);
         float o[CT], den = 0.0f;
 #pragma unroll
         for (int c = 0; c < CT; ++c) o[c] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float wt = __builtin_amdgcn_exp2f(mm[w][qr] - gm);
             den = fmaf(wt, ml[w][qr], den);
 #pragma unroll
@@ -543,14 +551,15 @@ __global__ __launch_bounds__(256, 2) void attn_kv4_kernel(Args a) {
     }
 }
 
-// Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b), 4 waves a
-// quarter of the records each, a lane D / 64 columns.
-template <int D>
-__global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Args a) {
-    constexpr int C = D / 64;
+// Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b): the row's
+// records dealt to NW waves, eight loaded at a time (one memory latency for up to
+// 8 NW), each with a running reference; a lane holds D / 64 columns.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
+    constexpr int C = D / 64, CT = D / 16, N = 8;
     typedef float cvec __attribute__((ext_vector_type(C)));
-    __shared__ float red[4], dred[4];
-    __shared__ float nred[4][D];
+    __shared__ float mm[NW], ml[NW];
+    __shared__ __align__(16) float mo[NW][D];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = a.M * a.G;
@@ -559,45 +568,66 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Args a) {
     find_share(a, -1, p);
     const int g = blockIdx.x / rows, r = blockIdx.x - g * rows;
     const int64_t pos = (int64_t)a.dpos[p.b] + r / a.G;
-    const int ns = pos < 0 || pos >= a.c.max_pos ? 0 : (int)(pos / ((int64_t)p.per * kUnit)) + 1;   // shares of positions 0 .. pos
-    const float* rec = a.part + ((int64_t)blockIdx.x * a.shares + p.first) * (D + 4);
-    float gm = kNone;
-    for (int i = tid; i < ns; i += 256) gm = fmaxf(gm, rec[(int64_t)i * (D + 4)]);
-    gm = mx::wave_reduce_dpp<true>(gm);
-    if (lane == 0) red[wave] = gm;
-    __syncthreads();
-    gm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float den = 0.0f;
-    cvec num = 0.0f;
-#pragma unroll 8
-    for (int i = wave; i < ns; i += 4) {
-        const float* x = rec + (int64_t)i * (D + 4);
-        const float2 st = *reinterpret_cast<const float2*>(x);
-        const cvec v = *reinterpret_cast<const cvec*>(x + 4 + C * lane);
-        const float w = __builtin_amdgcn_exp2f(st.x - gm);
-        den = fmaf(w, st.y, den);
+    const int ns = __builtin_amdgcn_readfirstlane(
+        pos < 0 || pos >= a.c.max_pos ? 0 : (int)(pos / kUnit) / p.per + 1);   // shares of positions 0 .. pos
+    const float* rec = a.part + ((int64_t)blockIdx.x * a.shares + __builtin_amdgcn_readfirstlane(p.first)) * (D + 4);
+    float m = kNone, l = 0.0f;
+    cvec o = 0.0f;
+    for (int i0 = wave; i0 < ns; i0 += N * NW) {
+        float2 st[N];
+        cvec v[N];
 #pragma unroll
-        for (int c = 0; c < C; ++c) num[c] = fmaf(w, v[c], num[c]);
+        for (int k = 0; k < N; ++k) {
+            const float* x = rec + (int64_t)min(i0 + k * NW, ns - 1) * (D + 4);
+            st[k] = *reinterpret_cast<const float2*>(x);
+            v[k] = *reinterpret_cast<const cvec*>(x + 4 + C * lane);
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) top = i0 + k * NW < ns ? fmaxf(top, st[k].x) : top;
+        const float al = __builtin_amdgcn_exp2f(m - top);
+        l *= al;
+        o *= al;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (i0 + k * NW < ns) {
+                const float w = __builtin_amdgcn_exp2f(st[k].x - m);
+                l = fmaf(w, st[k].y, l);
+#pragma unroll
+                for (int c = 0; c < C; ++c) o[c] = fmaf(w, v[k][c], o[c]);
+            }
+        }
     }
-    *reinterpret_cast<cvec*>(&nred[wave][C * lane]) = num;
-    if (lane == 0) dred[wave] = den;
+    *reinterpret_cast<cvec*>(&mo[wave][C * lane]) = o;
+    if (lane == 0) {
+        mm[wave] = m;
+        ml[wave] = l;
+    }
     __syncthreads();
-    constexpr int CT = D / 16;
     if (tid >= 16) return;
-    den = (dred[0] + dred[1]) + (dred[2] + dred[3]);
+    float gm = mm[0], den = 0.0f, x[CT];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) gm = fmaxf(gm, mm[w]);
+#pragma unroll
+    for (int c = 0; c < CT; ++c) x[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const float wt = __builtin_amdgcn_exp2f(mm[w] - gm);
+        den = fmaf(wt, ml[w], den);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) x[c] = fmaf(wt, mo[w][CT * tid + c], x[c]);
+    }
     const bool none = den == 0.0f;    // no position, or none on a page: zeros
     const float inv = 1.0f / den;
-    float o[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        const int k = CT * tid + c;
-        o[c] = none ? 0.0f : ((nred[0][k] + nred[1][k]) + (nred[2][k] + nred[3][k])) * inv;
-    }
-    mxa::store<CT>(a.out, ((int64_t)p.b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, CT * tid, o);
+    for (int c = 0; c < CT; ++c) x[c] = none ? 0.0f : x[c] * inv;
+    mxa::store<CT>(a.out, ((int64_t)p.b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, CT * tid, x);
 }
 
 struct Plan {
-    int RT, groups, shares;
+    int RT, groups, wanted, shares, most;   // shares the batch should and may have, and one sequence may
+    int waves;   // of a workgroup
     bool one;
 };
 Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
@@ -605,12 +635,23 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
     const int64_t tiles = ((int64_t)M * (Hq / Hkv) + 15) / 16;
     p.groups = (int)((tiles + kMaxRT - 1) / kMaxRT);
     p.RT = (int)((tiles + p.groups - 1) / p.groups);
-    // shares of the whole batch for one round of workgroups (two per CU), none
+    // shares of the whole batch for one round of workgroups, none
     // below the 128 positions of a round of its waves
-    const int64_t most = (int64_t)B * ((max_pos + 4 * kUnit - 1) / (4 * kUnit));
-    const int64_t want = (512 + (int64_t)Hkv * p.groups - 1) / ((int64_t)Hkv * p.groups);
-    p.one = most == B || want * 4 <= B;
-    p.shares = p.one ? B : (int)(want < most ? want : most) + B;
+    const int kRound = p.RT == 1 ? 1024 : 512;   // four and two workgroups a CU
+    int64_t longest = (max_pos + kMinShare * kUnit - 1) / (kMinShare * kUnit);   // shares a sequence may have (share_units)
+    if (longest > kFew) longest = std::max<int64_t>(kFew, (longest + 1) / 2);
+    const int64_t most = B * longest;
+    const int64_t want = (kRound + (int64_t)Hkv * p.groups - 1) / ((int64_t)Hkv * p.groups);
+    // Sequences enough for half the CUs, and short: one workgroup of 16 waves each and no merge.  32 / 4 heads, one
+    // token, full caches, 16 waves / shares and merge, us: B = 64, 1024 positions 13.7 / 19.9, 2048 19.2 / 24.1; B = 32,
+    // 2048 16.5 / 18.5; but B = 8, 2048 15.4 / 11.8, B = 1, 1024 10.8 / 8.1.
+    const int64_t wgs = (int64_t)B * Hkv * p.groups;
+    const bool wide = p.RT == 1 && longest > 1 && max_pos <= 2048 && wgs >= 128 && wgs <= 256;
+    p.waves = wide ? 16 : 4;
+    p.one = wide || longest == 1 || want * 4 <= B || (want == 1 && B == 1);
+    p.wanted = (int)(want < most ? want : most);
+    p.shares = p.one ? B : p.wanted + (B > 1 ? B : 0);
+    p.most = (int)(longest < p.shares ? longest : p.shares);
     return p;
 }
 
@@ -654,12 +695,18 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     a.Hq = Hq;
     a.G = Hq / Hkv;
     a.shares = p.shares;
+    a.wanted = p.wanted;
     a.scale = (float)(1.4426950408889634 / sqrt((double)D));
     const hipStream_t st = mxh::as_stream(stream);
     const dim3 grid(p.shares, Hkv, p.groups);
-#define MXH_K4(DD, RR, QQ)                                                                                  \
-    if (p.one) hipLaunchKernelGGL((attn_kv4_kernel<DD, RR, QQ, true>), grid, dim3(256), 0, st, a);          \
-    else hipLaunchKernelGGL((attn_kv4_kernel<DD, RR, QQ, false>), grid, dim3(256), 0, st, a)
+#define MXH_K4(DD, RR, QQ)                                                                                              \
+    if (p.waves == 16) {                                                                                               \
+        if constexpr (RR == 1) hipLaunchKernelGGL((attn_kv4_kernel<DD, 1, QQ, true, 16>), grid, dim3(1024), 0, st, a); \
+    } else if (p.one) {                                                                                                \
+        hipLaunchKernelGGL((attn_kv4_kernel<DD, RR, QQ, true, 4>), grid, dim3(256), 0, st, a);                         \
+    } else {                                                                                                           \
+        hipLaunchKernelGGL((attn_kv4_kernel<DD, RR, QQ, false, 4>), grid, dim3(256), 0, st, a);                        \
+    }
 #define MXH_K4Q(DD, RR)                  \
     if (q_dtype == MXFP4_DT_BF16) {      \
         MXH_K4(DD, RR, 1);               \
@@ -681,7 +728,10 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
 #undef MXH_K4
     const int rl = mxh::launch_status("attn_kv4 (shares)");
     if (rl != MXFP4_OK || p.one) return rl;
-    if (D == 64) hipLaunchKernelGGL(attn_kv4_merge_kernel<64>, dim3(M * Hq, B), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(attn_kv4_merge_kernel<128>, dim3(M * Hq, B), dim3(256), 0, st, a);
+    // 16 waves where a row has more records than four load at once
+    const bool many = p.shares > kFew * B && p.most > kFew;
+    const dim3 gm(M * Hq, B), bm(many ? 1024 : 256);
+    if (D == 64) hipLaunchKernelGGL((many ? attn_kv4_merge_kernel<64, 16> : attn_kv4_merge_kernel<64, 4>), gm, bm, 0, st, a);
+    else hipLaunchKernelGGL((many ? attn_kv4_merge_kernel<128, 16> : attn_kv4_merge_kernel<128, 4>), gm, bm, 0, st, a);
     return mxh::launch_status("attn_kv4 (merge)");
 }
