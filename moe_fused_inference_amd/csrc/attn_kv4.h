@@ -1,14 +1,26 @@
-// attn_kv4.h -- where attention over the MXFP4 cache leaves a row: fp32, bf16 or
-// fp16, and / or the MXFP4 rows of its bf16 rounding (o_proj's activations).
+// attn_kv4.h -- what the kernels of attention over the MXFP4 cache share: arguments,
+// a batch's shares, a unit's softmax, and where a row goes (fp32, bf16 or fp16, and / or
+// the MXFP4 rows of its bf16 rounding, o_proj's activations).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kv4.h"
 #include "mx_device.h"
 #include "mxfp4_hip.h"
 #include "quant_rows.h"
 
 namespace mxa {
+
+using kv4::Cache;
+
+constexpr int kUnit = 32;              // positions per wave and step
+constexpr float kMost = 2048.0f;       // a lane's terms of a unit sum to at most this
+constexpr float kWide = 262144.0f;     // a reference past it: an exponent's rounding is up to 2^-6 and more
+constexpr float kNone = -3e38f;        // the reference of a row that has seen nothing: exp2(-inf - kNone) = 0
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+constexpr int kFew = 32;               // shares of a sequence that four waves merge at once
+constexpr int kMinShare = 4;           // units, one a wave
 
 struct Out {
     void* o;        // or null
@@ -61,5 +73,266 @@ __device__ __forceinline__ void store(const Out& t, int64_t row, int D, int c0, 
         if (c0 % 32 == 0) t.os[at / 32] = (uint8_t)code;
     }
 }
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ mx::v4f mfma_bf16(uint4 a, uint4 b, mx::v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+}
+
+struct Args {
+    const uint16_t* q;
+    int64_t ldq;                 // elements between tokens of q
+    Cache c;
+    const int32_t* dpos;
+    float* part;
+    Out out;
+    int B, M, Hq, G, shares, wanted;   // shares: how many there may be, over the batch
+    float scale;                 // log2(e) / sqrt(D)
+};
+
+// Units of sequence b.
+__device__ __forceinline__ uint32_t units_of(const Args& a, int b) {
+    const int64_t n = (int64_t)a.dpos[b] + a.M;
+    return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
+}
+// Inclusive prefix sums over the wave (every lane active).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr 1, 2, 4, 8: within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15: row 0's total to row 1, 2's to 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast 31: the first half's to the second
+    return v;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ uint32_t shares_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
+
+// Units of a share for `total` units in the batch: a.wanted of them, in whole rounds of
+// the four waves, two rounds at least from 32 shares a sequence on (fewer records to
+// merge; one token, us with at least 1 / 2 rounds: 4096 positions 8.2 / 9.0, 8000 9.8 /
+// 9.1, 32000 16.4 / 13.5).
+__device__ __forceinline__ uint32_t share_units(uint64_t total, const Args& a) {
+    const uint32_t per = (uint32_t)((total + a.wanted - 1) / a.wanted + 3) & ~3u;
+    return max(per, total > (uint64_t)kFew * kMinShare * a.B ? 2u * kMinShare : (uint32_t)kMinShare);
+}
+
+// What a share holds -- the same whole rounds of the four waves for every sequence, so
+// few units that the batch has at most a.wanted shares, or a few more -- and for share
+// number `at` of the batch its sequence b and its number s there, or for at < 0 the
+// batch's number of sequence b's first share.  Every wave finds them by itself: a lane
+// per sequence, sums over the wave.  All uniform.
+struct Place {
+    int per, b, s, first;
+};
+__device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
+    const int lane = threadIdx.x & 63;
+    auto units = [&](int b0) { return b0 + lane < a.B ? units_of(a, b0 + lane) : 0u; };
+    if (a.B == 1) {
+        const uint32_t nu = units_of(a, 0);
+        p.per = (int)share_units(nu, a);
+        p.first = p.b = 0;
+        p.s = at;
+        return at < 0 || (int64_t)at * p.per < nu;
+    }
+    const uint32_t u0 = units(0);
+    uint64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) total += last_lane(wave_scan(b0 ? units(b0) : u0));
+    uint32_t per = share_units(total, a);
+    for (int i = 0; i < 3; ++i) {      // a sequence's last share is a part of one: longer ones until they are few enough
+        uint32_t n = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) n += last_lane(wave_scan(shares_of(b0 ? units(b0) : u0, per)));
+        if (n <= (uint32_t)a.wanted) break;
+        per = max(per + 4, (uint32_t)((uint64_t)per * n / a.wanted + 3) & ~3u);
+    }
+    p.per = (int)per;
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int ns = (int)shares_of(b0 ? units(b0) : u0, per), upto = (int)wave_scan(ns);
+        int l = p.b - b0;
+        if (at >= 0) {
+            const uint64_t past = __ballot(before + upto > at);
+            l = past ? (int)__builtin_ctzll(past) : 64;
+        }
+        if (l < 64) {
+            p.b = b0 + l;
+            p.first = before + __builtin_amdgcn_readlane(upto - ns, l);
+            p.s = at - p.first;
+            return true;
+        }
+        before += (int)last_lane(upto);
+    }
+    return false;
+}
+
+// N (a multiple of 8) fp32 terms as NP bf16 parts each, whose sum each is (8 bits a
+// part, rounded to nearest, the rest exact): p[k][j] is part j of terms 8 k .. 8 k + 7.
+template <int N, int NP>
+__device__ __forceinline__ void parts(float (&t)[N], uint4 (&p)[N / 8][NP]) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        uint32_t o[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            o[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{t[2 * i], t[2 * i + 1]}), bf16x2_t));
+            if (j + 1 < NP) {
+                t[2 * i] -= __uint_as_float(o[i] << 16);
+                t[2 * i + 1] -= __uint_as_float(o[i] & 0xFFFF0000u);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N / 8; ++k) p[k][j] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    }
+}
+
+// The largest of three, a NaN among them left out (as fmaxf, whose operands the
+// compiler would first pass through an instruction each).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// a * b rounded, minus c: not one fma.
+__device__ __forceinline__ float mul_then_sub(float a, float b, float c) {
+#pragma clang fp contract(off)
+    const float ab = a * b;
+    return ab - c;
+}
+
+// The maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+template <bool MAX>
+__device__ __forceinline__ float over_lq(float v) {
+    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// Eight elements of q as bf16 parts: bf16 itself, or fp16's 11 bits as 8 + 3.
+template <int NQ>
+__device__ __forceinline__ void q_parts(uint4 w, uint4 (&p)[NQ]) {
+    if constexpr (NQ == 1) {
+        p[0] = w;
+    } else {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = mx::f16_to_f32((uint16_t)(x[i / 2] >> (16 * (i & 1))));
+        uint4 o[1][NQ];
+        parts(t, o);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) p[j] = o[0][j];
+    }
+}
+
+// One unit of a row's softmax, in two parts with other work between them.  The lane's N
+// scores s to terms t = exp2(s scale - m) and their sum.  The reference m is not the row's
+// maximum: any gives the same quotient, and no unit looks for one that need not.  `wide`
+// (uniform): a row's reference is past kWide.
+template <int N>
+__device__ __forceinline__ void terms(const float (&s)[N], float scale, float m, bool wide, float (&t)[N], float& sum) {
+    if (!wide) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = fmaf(s[i], scale, -m);
+    } else {   // the rounded product, as in m: the fma's would differ from it by more than a term
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = mul_then_sub(s[i], scale, m);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = __builtin_amdgcn_exp2f(t[i]);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) sum += (t[i] + t[i + 1]) + (t[i + 2] + t[i + 3]);
+}
+// A lane's terms that sum to more than kMost (at its first unit, where m is kNone and they
+// are infinite, or past a much larger score) are made again, on the maximum, and what was
+// summed before is rescaled (rescale(factor)); over(x): the maximum over the row's lanes.
+// p: the terms' parts.  Then l, their sum so far, takes them.
+template <int N, int NP, class Over, class Rescale>
+__device__ __forceinline__ void again(const float (&s)[N], float scale, float& m, float& l, bool& wide, float sum, uint4 (&p)[N / 8][NP],
+                                      Over over, Rescale rescale) {
+    if (__ballot(sum > kMost)) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < N; i += 2) top = max3(top, s[i], s[i + 1 < N ? i + 1 : i]);
+        const float mn = fmaxf(m, over(top) * scale);
+        const float al = __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+        rescale(al);
+        m = mn;
+        wide = __ballot(fabsf(mn) > kWide && mn != kNone) != 0ull;
+        float t[N];
+        terms(s, scale, m, wide, t, sum);
+        parts(t, p);
+    }
+    l += sum;
+}
+
+// A code of a position's word, in the exponent field of a scale for the packed
+// conversions, which read that field alone: its neighbours are around it.
+__device__ __forceinline__ float scale_at(uint32_t word, uint32_t block) {
+    return __uint_as_float(__builtin_amdgcn_alignbit(word, word, 8 * block + 9));
+}
+
+// w * 0 summed: 0, or NaN where one of eight bf16 is an infinity or a NaN.
+__device__ __forceinline__ float not_finite(uint4 w) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z = fmaf(mx::bf16_to_f32((uint16_t)(x[i / 2] >> (16 * (i & 1)))), 0.0f, z);
+    return z;
+}
+
+// The end of row r of kv head g of sequence b, a share from unit u0 on: NW waves' (m, l,
+// columns) to one record, or with ONE the output.  16 neighbouring lanes a row (by
+// threadIdx.x), which all call it, D / 16 columns a lane.
+template <int D, int NW, bool ONE, class M, class L, class O>
+__device__ __forceinline__ void finish(const Args& a, int b, int g, int r, int u0, M m_of, L l_of, O o_of) {
+    constexpr int CT = D / 16;
+    const int c0 = CT * (threadIdx.x & 15);
+    const int64_t pos = (int64_t)a.dpos[b] + r / a.G;
+    if (!ONE && (pos < 0 || pos >= a.c.max_pos || (int64_t)u0 * kUnit > pos)) return;   // no record: the merge reads none
+    float gm = m_of(0);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) gm = fmaxf(gm, m_of(w));
+    float o[CT], den = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) o[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const float wt = __builtin_amdgcn_exp2f(m_of(w) - gm);
+        den = fmaf(wt, l_of(w), den);
+#pragma unroll
+        for (int c = 0; c < CT; c += 4) {
+            const float4 x = o_of(w, c0 + c);
+            o[c] = fmaf(wt, x.x, o[c]);
+            o[c + 1] = fmaf(wt, x.y, o[c + 1]);
+            o[c + 2] = fmaf(wt, x.z, o[c + 2]);
+            o[c + 3] = fmaf(wt, x.w, o[c + 3]);
+        }
+    }
+    if constexpr (ONE) {
+        const bool none = pos < 0 || pos >= a.c.max_pos || den == 0.0f;   // nothing seen: zeros
+        const float inv = none ? 0.0f : 1.0f / den;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c] = none ? 0.0f : o[c] * inv;
+        store<CT>(a.out, ((int64_t)b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, c0, o);
+    } else {
+        float* rec = a.part + (((int64_t)g * a.M * a.G + r) * a.shares + blockIdx.x) * (D + 4);
+#pragma unroll
+        for (int c = 0; c < CT; c += 4) *reinterpret_cast<float4*>(rec + 4 + c0 + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        if (c0 == 0) *reinterpret_cast<float2*>(rec) = make_float2(gm, den);
+    }
+}
+
+// More than 16 query rows of a kv head (attn_kv4_rows.hip), in groups of 32; exact: p in
+// three bf16 parts instead of two.
+int attn_rows(const Args& a, int q_dtype, int groups, int D, bool one, bool exact, hipStream_t st);
 
 }  // namespace mxa

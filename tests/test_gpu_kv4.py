@@ -160,6 +160,10 @@ CASES = [
     (2, 1, 8, 1, 128, 128, 1024, [1023, 2 ** 31 - 1], "bf16", "fp32"),
     (1, 33, 2, 4, 128, 32, 256, [100], "bf16", "fp32"),
     (2, 70, 1, 2, 64, 0, 160, [0, 77], "fp16", "fp32"),
+    (1, 200, 2, 4, 128, 64, 1024, [600], "bf16", "fp32"),                                      # pieces of a prompt
+    (3, 50, 1, 5, 64, 16, 336, [-20, 290, 100], "fp16", "bf16"),
+    (8, 33, 8, 16, 64, 0, 64, [0, 31, -33, 30, 5, -1, 60, 20], "bf16", "fp16"),
+    (1, 130, 1, 1, 128, 0, 144, [0], "fp16", "fp32"),
     (33, 1, 4, 2, 128, 0, 544, [(i * 61) % 545 - 1 for i in range(33)], "bf16", "fp32"),      # one workgroup a head
     (66, 2, 2, 3, 64, 16, 672, [(i * 97) % 670 - 2 * (i % 7 == 0) for i in range(66)], "fp16", "bf16"),
 ]
