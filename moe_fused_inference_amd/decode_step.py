@@ -25,15 +25,19 @@ by attn_decode's codec; they are written the way the matching reference
 step writes them: M = 1 with the decode extension's kv_write codec (the
 graph runner, runtime/model_runner_v3.py:98-101), M > 1 with torch's
 float8_e4m3fn conversion (forward_batch, runtime/model_runner_v2.py:256-257).
+With kv="mxfp4" it holds MXFP4 rows instead (kv4.py), 68 bytes a position and
+head where E4M3 takes 128, written and read by qk_norm_rope_kv4 and attn_kv4.
 """
 import ctypes
 from dataclasses import dataclass, field
 
 import torch
 
-from . import _lib
+from . import _lib, kv4
 from .moe_layer import (FusedRouterLayerCall, PostAttnLayerCall, RoutedLayerCall, StackedExperts, layer_status,
                         workspace as layer_workspace)
+
+_DT_BF16, _DT_F32 = 0, 2   # MXFP4_DT_* of mxfp4_hip.h
 
 
 @dataclass
@@ -156,10 +160,19 @@ class DecodeStep:
     """M tokens of one sequence per step (M = 1: forward_decode; M > 1:
     forward_batch).  ids (M,) int32 and the base position dpos (1,) int32
     stay on the device: each step reads them and leaves the greedy next
-    tokens and dpos + M for the next step."""
+    tokens and dpos + M for the next step.
+
+    kv: "fp8" (E4M3, as the reference) or "mxfp4" (a kv4.KV4 per layer in
+    ``kv4``; max_pos a multiple of 16).  The MXFP4 cache's attention
+    runs in launches of its own: attn_front and attn_next, which put the FP8
+    cache's into the MoE launch, do not apply.  us a layer (32 / 4 heads, hidden
+    2048, 1/8 of the head with it; FP8 / MXFP4): one token, 4000 positions 38.5 /
+    44.1, 32000 57.7 / 48.9; four tokens 62.9 / 66.8, 80.1 / 74.8."""
 
     def __init__(self, model, cfg, M=1, max_pos=4096, device="cuda", fused_router=True, qkv_tail=True,
-                 attn_front=True, attn_next=True):
+                 attn_front=True, attn_next=True, kv="fp8"):
+        if kv not in ("fp8", "mxfp4"):
+            raise RuntimeError(f"kv must be 'fp8' or 'mxfp4', got {kv!r}")
         self.lib = _lib.load()
         self.model, self.cfg, self.M, self.max_pos = model, cfg, int(M), int(max_pos)
         self.kv_codec = 0 if self.M == 1 else 1   # kv_write's codec / torch float8_e4m3fn
@@ -175,7 +188,8 @@ class DecodeStep:
         # with the q|k|v tail, the attention merge and o_proj also run in the
         # MoE launch (mxfp4_decode_layer_post_attn; 32 heads of 128): two
         # launches per layer in all
-        self.attn_front = self.qkv_tail and bool(attn_front) and cfg.n_heads == 32 and cfg.head_dim == 128
+        self.attn_front = (self.qkv_tail and bool(attn_front) and cfg.n_heads == 32 and cfg.head_dim == 128
+                           and kv == "fp8")
         # and with the front, the next layer's attention chunk pass too: one
         # launch per layer (8 query heads per kv head, max_pos * kv heads <= 32768)
         self.attn_next = (self.attn_front and bool(attn_next) and cfg.n_heads == 8 * cfg.n_kv_heads
@@ -211,12 +225,19 @@ class DecodeStep:
         buf("logits", (M, c.vocab), f32)
         nb = self.lib.mxfp4_argmax_workspace_size(M, c.vocab)
         buf("arg_ws", ((nb + 255) // 256 * 256,), u8)   # zero-filled once; each call leaves it so
-        nb = self.lib.mxfp4_attn_decode_workspace_size(M, Hq, self.max_pos)
-        buf("attn_ws", ((nb + 15) // 16 * 16,), u8)
-        buf("attn_ws2", ((nb + 15) // 16 * 16,) if M == 1 else (16,), u8)   # odd layers' chunk records (attn_next)
-        # KV cache of every layer: (L, max_pos, Hkv, D) E4M3 bytes
-        buf("kvk", (c.n_layers, self.max_pos, Hkv, D), u8)
-        buf("kvv", (c.n_layers, self.max_pos, Hkv, D), u8)
+        self.kv4 = None
+        if kv == "mxfp4":
+            nb = self.lib.mxfp4_attn_kv4_workspace_size(1, M, Hq, Hkv, D, self.max_pos)
+            buf("attn_ws", (max(16, (nb + 15) // 16 * 16),), u8)
+            buf("q", (M, Hq, D), bf16)
+            self.kv4 = [kv4.empty_cache(1, self.max_pos, Hkv, D, device) for _ in range(c.n_layers)]
+        else:
+            nb = self.lib.mxfp4_attn_decode_workspace_size(M, Hq, self.max_pos)
+            buf("attn_ws", ((nb + 15) // 16 * 16,), u8)
+            buf("attn_ws2", ((nb + 15) // 16 * 16,) if M == 1 else (16,), u8)   # odd layers' chunk records (attn_next)
+            # KV cache of every layer: (L, max_pos, Hkv, D) E4M3 bytes
+            buf("kvk", (c.n_layers, self.max_pos, Hkv, D), u8)
+            buf("kvv", (c.n_layers, self.max_pos, Hkv, D), u8)
         if M == 1:
             self.layer_ws = layer_workspace(c.top_k, c.moe_inter, H, device)
             self.moe_calls = [RoutedLayerCall(t["y"][0], t["glog"][0], c.top_k, lw.experts, t["moe"][0], None,
@@ -236,10 +257,18 @@ class DecodeStep:
         self.b.dpos.fill_(int(pos))
 
     def fill_cache(self, upto, seed=1):
-        """Synthetic context: random E4M3 bytes for positions [0, upto) of
-        every layer's cache (codes of |v| < 2, no NaN code)."""
-        g = torch.Generator(device=self.b.kvk.device)
+        """Synthetic context: random bytes for positions [0, upto) of every
+        layer's cache (E4M3 codes of |v| < 2, no NaN code; MXFP4 nibbles under
+        scales of 1/4, |v| <= 1.5)."""
+        g = torch.Generator(device=self.b.x.device)
         g.manual_seed(seed)
+        if self.kv4 is not None:
+            for kq, ks, vq, vs in self.kv4:
+                for q, s in ((kq, ks), (vq, vs)):
+                    r = torch.randint(0, 256, q[:, :, :upto].shape, generator=g, device=q.device, dtype=torch.int32)
+                    q[:, :, :upto] = r.to(torch.uint8)
+                    s[:, :, :upto] = 125
+            return
         for kv in (self.b.kvk, self.b.kvv):
             r = torch.randint(0, 256, kv[:, :upto].shape, generator=g, device=kv.device, dtype=torch.int32)
             kv[:, :upto] = ((r & 0x80) | (r & 0x3F)).to(torch.uint8)   # exponent field <= 7: |v| < 2
@@ -284,11 +313,21 @@ class DecodeStep:
         return self.b.attn_ws2 if (self.attn_next and l % 2) else self.b.attn_ws
 
     def _attn_oproj(self, l, lw, qkv, s):
-        """q/k head norm + RoPE, the step's KV rows and attention in one pass,
-        its output straight to MXFP4 of bf16(o) (the raw scores are not kept),
-        then o_proj into b.oproj."""
+        """q/k head norm + RoPE, the step's KV rows and attention (in one pass
+        with the FP8 cache), its output straight to MXFP4 of bf16(o) (the raw
+        scores are not kept), then o_proj into b.oproj."""
         lib, c, b, M = self.lib, self.cfg, self.b, self.M
         H, D, Hq, Hkv = c.hidden, c.head_dim, c.n_heads, c.n_kv_heads
+        if self.kv4 is not None:
+            cache = [t.data_ptr() for t in self.kv4[l]] + [None, 1, self.max_pos, 0, b.dpos.data_ptr()]
+            self._ck(lib.mxfp4_qk_norm_rope_kv4(qkv.data_ptr(), lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), c.rms_eps,
+                                                c.rope_theta, *cache, 1, M, Hq, Hkv, D, b.q.data_ptr(), s),
+                     "qk_norm_rope_kv4")
+            self._ck(lib.mxfp4_attn_kv4(b.q.data_ptr(), _DT_BF16, Hq * D, *cache, None, _DT_F32, b.aq.data_ptr(),
+                                        b.as_.data_ptr(), 1, M, Hq, Hkv, D, b.attn_ws.data_ptr(), b.attn_ws.numel(),
+                                        s), "attn_kv4")
+            self._lin(b.aq, b.as_, lw.o, H, Hq * D, b.oproj, s)
+            return
         kvk, kvv = b.kvk[l], b.kvv[l]
         self._ck(lib.mxfp4_attn_decode_fused(qkv.data_ptr(), lw.q_norm.data_ptr(), lw.k_norm.data_ptr(),
                                              c.rms_eps, c.rope_theta, kvk.data_ptr(), kvv.data_ptr(),

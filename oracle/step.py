@@ -18,10 +18,12 @@ exp), so the comparison is to a tolerance.
 import numpy as np
 
 from . import attn as attn_ref
+from . import kv4 as kv4_ref
 from . import mxfp4 as fmt
 from . import ops
 
 bf16 = fmt.bf16_round
+KV4 = 4                          # kv_codec: MXFP4 rows, the cache of oracle.kv4
 
 
 def rms_norm_ref(x, w, eps, bf16_input=True):
@@ -68,7 +70,8 @@ def layer_ref(lw, cfg, x, base, kvk_l, kvv_l, fused_moe, kv_codec=0, teacher=Non
     """One decoder layer of the step (runtime/model_runner_v2.py:147-208 for
     M = 1, :238-297 for M > 1) on the residual stream x (M, H) bf16 values of
     tokens at positions base..base+M-1.  lw: that layer's weights (as in
-    step_ref), kvk_l / kvv_l: its (max_pos, Hkv, D) caches, updated in place.
+    step_ref), kvk_l / kvv_l: its (max_pos, Hkv, D) caches, updated in place
+    (kv_codec KV4: kvk_l is its MXFP4 cache of oracle.kv4, kvv_l unused).
     Returns the residual stream after the layer (bf16 values).
 
     teacher: optional dict of another implementation's intermediates of this
@@ -97,8 +100,12 @@ def layer_ref(lw, cfg, x, base, kvk_l, kvv_l, fused_moe, kv_codec=0, teacher=Non
     qn = rms_norm_ref(q, lw["q_norm"], eps, bf16_input=False)
     kn = rms_norm_ref(k, lw["k_norm"], eps, bf16_input=False)
     qr, kr = rope_ref(qn, pos, cfg.rope_theta), rope_ref(kn, pos, cfg.rope_theta)
-    attn_ref.kv_write_ref(kr, bf16(v), kvk_l, kvv_l, base, kv_codec)
-    o_att, _ = attn_ref.attn_decode_ref(qr, kvk_l, kvv_l, base)
+    if kv_codec == KV4:
+        kv4_ref.write(kr[None], bf16(v)[None], kvk_l, [base])
+        o_att = kv4_ref.attention(qr[None], kvk_l, [base])[0][0]
+    else:
+        attn_ref.kv_write_ref(kr, bf16(v), kvk_l, kvv_l, base, kv_codec)
+        o_att, _ = attn_ref.attn_decode_ref(qr, kvk_l, kvv_l, base)
     of = bf16(o_att.astype(np.float32)).reshape(M, Hq * D)
     aq, as_ = fmt.quantize_rows(of)
     o = ops.lin_pq_ref(aq, as_, *lw["o"]).astype(np.float32)

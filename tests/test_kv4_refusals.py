@@ -119,3 +119,8 @@ def test_binding_refuses_cpu_tensors_and_bad_allocations():
         a.update(bad)
         with pytest.raises(RuntimeError, match="cache needs"):
             kv4.empty_cache(a["n_pages"], a["page"], a["Hkv"], a["D"], device="cpu")
+
+
+@pytest.mark.parametrize("call", [_write, _read, _attn, _rope])
+def test_more_head_rows_than_32_bits(call):
+    _refused(call(_cache(n_pages=1 << 15, page=1 << 15)), "head rows")      # times four heads: 2^32
