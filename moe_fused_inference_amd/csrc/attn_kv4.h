@@ -21,6 +21,7 @@ constexpr float kNone = -3e38f;        // the reference of a row that has seen n
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 constexpr int kFew = 32;               // shares of a sequence that four waves merge at once
 constexpr int kMinShare = 4;           // units, one a wave
+constexpr uint32_t kPad = 8;          // units that take as long as a workgroup's change to another sequence
 
 struct Out {
     void* o;        // or null
@@ -90,13 +91,13 @@ struct Args {
     const int32_t* dpos;
     float* part;
     Out out;
-    int B, M, Hq, G, shares, wanted;   // shares: how many there may be, over the batch
+    int B, M, Hq, G, shares, records;   // shares of the batch, and records a row may have (its stride)
     float scale;                 // log2(e) / sqrt(D)
 };
 
-// Units of sequence b.
-__device__ __forceinline__ uint32_t units_of(const Args& a, int b) {
-    const int64_t n = (int64_t)a.dpos[b] + a.M;
+// Units of a sequence whose first token is at base.
+__device__ __forceinline__ uint32_t units_of(const Args& a, int base) {
+    const int64_t n = (int64_t)base + a.M;
     return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
 }
 // Inclusive prefix sums over the wave (every lane active).
@@ -110,63 +111,99 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
-__device__ __forceinline__ uint32_t shares_of(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
 
-// Units of a share for `total` units in the batch: a.wanted of them, in whole rounds of
-// the four waves, two rounds at least from 32 shares a sequence on (fewer records to
-// merge; one token, us with at least 1 / 2 rounds: 4096 positions 8.2 / 9.0, 8000 9.8 /
-// 9.1, 32000 16.4 / 13.5).
+// Units of a share for `total` units in the batch: whole rounds of the four waves, as
+// few as a.shares of them need, two rounds at least from 32 shares a sequence on (fewer
+// records to merge; one token, us with at least 1 / 2 rounds: 4096 positions 8.2 / 9.0,
+// 8000 9.8 / 9.1, 32000 16.4 / 13.5).
 __device__ __forceinline__ uint32_t share_units(uint64_t total, const Args& a) {
-    const uint32_t per = (uint32_t)((total + a.wanted - 1) / a.wanted + 3) & ~3u;
+    const uint64_t n = total + a.shares - 1;
+    const uint32_t per = (uint32_t)((n >> 32 ? n / a.shares : (uint32_t)n / (uint32_t)a.shares) + 3) & ~3u;
     return max(per, total > (uint64_t)kFew * kMinShare * a.B ? 2u * kMinShare : (uint32_t)kMinShare);
 }
 
-// What a share holds -- the same whole rounds of the four waves for every sequence, so
-// few units that the batch has at most a.wanted shares, or a few more -- and for share
-// number `at` of the batch its sequence b and its number s there, or for at < 0 the
-// batch's number of sequence b's first share.  Every wave finds them by itself: a lane
+// The batch's units stand in one line, sequence after sequence, each behind kPad places
+// for what a workgroup spends on a sequence besides its units; share i has places i per
+// .. (i + 1) per - 1, so units of one sequence or of several in a row, and all shares are
+// about the same work whatever the lengths.  Every wave finds its place by itself: a lane
 // per sequence, sums over the wave.  All uniform.
 struct Place {
-    int per, b, s, first;
+    uint32_t per;
+    int b, base;        // a sequence, its dpos, and where it starts
+    uint64_t start;
 };
+__device__ __forceinline__ uint32_t pad_of(const Args& a) { return a.B == 1 ? 0u : kPad; }
+// The sequence with place at * p.per (false: that is past the line), or for at < 0
+// sequence p.b.
 __device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
     const int lane = threadIdx.x & 63;
-    auto units = [&](int b0) { return b0 + lane < a.B ? units_of(a, b0 + lane) : 0u; };
+    p.start = 0;
     if (a.B == 1) {
-        const uint32_t nu = units_of(a, 0);
-        p.per = (int)share_units(nu, a);
-        p.first = p.b = 0;
-        p.s = at;
-        return at < 0 || (int64_t)at * p.per < nu;
+        p.b = 0;
+        p.base = __builtin_amdgcn_readfirstlane(a.dpos[0]);
+        const uint32_t n = units_of(a, p.base);
+        p.per = share_units(n, a);
+        return at < 0 || (uint64_t)at * p.per < n;
     }
-    const uint32_t u0 = units(0);
-    uint64_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) total += last_lane(wave_scan(b0 ? units(b0) : u0));
-    uint32_t per = share_units(total, a);
-    for (int i = 0; i < 3; ++i) {      // a sequence's last share is a part of one: longer ones until they are few enough
-        uint32_t n = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) n += last_lane(wave_scan(shares_of(b0 ? units(b0) : u0, per)));
-        if (n <= (uint32_t)a.wanted) break;
-        per = max(per + 4, (uint32_t)((uint64_t)per * n / a.wanted + 3) & ~3u);
+    auto places = [&](int b0, int& base) {
+        base = 0;
+        if (b0 + lane >= a.B) return 0u;
+        base = a.dpos[b0 + lane];
+        const uint32_t n = units_of(a, base);
+        return n ? n + kPad : 0u;
+    };
+    int base;
+    const uint32_t n0 = places(0, base), to0 = wave_scan(n0);
+    uint64_t total = last_lane(to0);
+    for (int b0 = 64; b0 < a.B; b0 += 64) {
+        int t;
+        total += last_lane(wave_scan(places(b0, t)));
     }
-    p.per = (int)per;
-    int before = 0;
+    p.per = share_units(total, a);
+    const uint64_t target = (uint64_t)at * p.per;
+    if (at >= 0 && target >= total) return false;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int ns = (int)shares_of(b0 ? units(b0) : u0, per), upto = (int)wave_scan(ns);
+        const uint32_t n = b0 ? places(b0, base) : n0, to = b0 ? wave_scan(n) : to0;
         int l = p.b - b0;
         if (at >= 0) {
-            const uint64_t past = __ballot(before + upto > at);
+            const uint64_t past = __ballot(p.start + to > target);
             l = past ? (int)__builtin_ctzll(past) : 64;
         }
         if (l < 64) {
             p.b = b0 + l;
-            p.first = before + __builtin_amdgcn_readlane(upto - ns, l);
-            p.s = at - p.first;
+            p.base = __builtin_amdgcn_readlane(base, l);
+            p.start += (uint32_t)__builtin_amdgcn_readlane((int)(to - n), l);
             return true;
         }
-        before += (int)last_lane(upto);
+        p.start += last_lane(to);
     }
     return false;
+}
+// The share with place `at` of the line.
+__device__ __forceinline__ int share_of(uint64_t at, uint32_t per) {
+    return (int)(at >> 32 ? at / per : (uint32_t)at / per);
+}
+// Share blockIdx.x's sequences in turn: segment(b, its dpos, its units u0 .. u1 - 1).
+template <class Segment>
+__device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
+    Place p;
+    if (!find_share(a, blockIdx.x, p)) return;             // uniform
+    const uint64_t from = (uint64_t)blockIdx.x * p.per;
+    const int pad = (int)pad_of(a);
+    for (bool first = true;;) {
+        const int n = (int)units_of(a, p.base);
+        // the share's end and beginning, in units of the sequence (per < 2^28, and a line that is behind `from` ends past it)
+        const int u1 = (int)min((int64_t)n, (int64_t)(from + p.per - p.start) - pad);
+        const int u0 = (int)max((int64_t)0, (int64_t)from - (int64_t)p.start - pad);
+        if (u0 < u1) {
+            if (!first) __syncthreads();                   // LDS is used again
+            first = false;
+            segment(p.b, p.base, u0, u1);
+        }
+        if (n) p.start += n + pad;
+        if (++p.b == a.B || p.start >= from + p.per) return;
+        p.base = __builtin_amdgcn_readfirstlane(a.dpos[p.b]);
+    }
 }
 
 // N (a multiple of 8) fp32 terms as NP bf16 parts each, whose sum each is (8 bits a
@@ -289,14 +326,14 @@ __device__ __forceinline__ float not_finite(uint4 w) {
     return z;
 }
 
-// The end of row r of kv head g of sequence b, a share from unit u0 on: NW waves' (m, l,
+// The end of row r of kv head g of sequence b, a segment from unit u0 on: NW waves' (m, l,
 // columns) to one record, or with ONE the output.  16 neighbouring lanes a row (by
 // threadIdx.x), which all call it, D / 16 columns a lane.
 template <int D, int NW, bool ONE, class M, class L, class O>
-__device__ __forceinline__ void finish(const Args& a, int b, int g, int r, int u0, M m_of, L l_of, O o_of) {
+__device__ __forceinline__ void finish(const Args& a, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
     constexpr int CT = D / 16;
     const int c0 = CT * (threadIdx.x & 15);
-    const int64_t pos = (int64_t)a.dpos[b] + r / a.G;
+    const int64_t pos = (int64_t)base + r / a.G;
     if (!ONE && (pos < 0 || pos >= a.c.max_pos || (int64_t)u0 * kUnit > pos)) return;   // no record: the merge reads none
     float gm = m_of(0);
 #pragma unroll
@@ -324,7 +361,7 @@ __device__ __forceinline__ void finish(const Args& a, int b, int g, int r, int u
         for (int c = 0; c < CT; ++c) o[c] = none ? 0.0f : o[c] * inv;
         store<CT>(a.out, ((int64_t)b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, c0, o);
     } else {
-        float* rec = a.part + (((int64_t)g * a.M * a.G + r) * a.shares + blockIdx.x) * (D + 4);
+        float* rec = a.part + (((int64_t)g * a.M * a.G + r) * a.records + blockIdx.x + b) * (D + 4);
 #pragma unroll
         for (int c = 0; c < CT; c += 4) *reinterpret_cast<float4*>(rec + 4 + c0 + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
         if (c0 == 0) *reinterpret_cast<float2*>(rec) = make_float2(gm, den);

@@ -5,16 +5,17 @@
 //                          rows (tokens x heads of the kv head): a wave takes every
 //                          fourth unit of 32 of the share's positions, with its own
 //                          running softmax; the waves' sums meet in LDS -> one record
-//                          (reference, sum, D column sums) per row and share, or
+//                          (reference, sum, D column sums) per row, share and
+//                          sequence in it, or
 //                          the output where a sequence has one share.
 //   attn_kv4_rows_kernel   the same for more rows (attn_kv4_rows.hip).
 //   attn_kv4_merge_kernel  workgroup (kv head's row, sequence): the row's records
 //                          -> its output.
 //
 // Shares.  dpos lives on the device, so the host fixes only how many shares there
-// may be (about a round of workgroups, plus one a sequence); every workgroup adds
-// up the batch's lengths, and a share is the same number of units for every
-// sequence, so that long and short ones load the chip alike.
+// may be (a round of workgroups); every workgroup adds up the batch's lengths, and
+// a share is the same number of units of all sequences laid end to end, so that
+// long and short ones load the chip alike.
 //
 // Mathematics.  Both products are transposed, S^T = K Q^T and O^T = V^T P^T: an
 // MFMA leaves a lane with four positions of each of two 16-position tiles of one
@@ -125,188 +126,182 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
     auto& qs = lds.qs;
     auto& mo = lds.mo;
     __shared__ float mm[NW][16], ml[NW][16];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l16 = lane & 15, lq = lane >> 4;
     const int g = blockIdx.y, G = a.G, rows = a.M * G;     // at most 16
-    int b = 0, u0 = 0, u1 = INT32_MAX;
-    if constexpr (ONE) {
-        b = blockIdx.x;
-    } else {
-        Place pl;
-        if (!find_share(a, blockIdx.x, pl)) return;        // uniform
-        b = pl.b;
-        u0 = pl.s * pl.per;
-        u1 = u0 + pl.per;
-    }
-    // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
-    const int64_t base = __builtin_amdgcn_readfirstlane(a.dpos[b]);
-    auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
-    const int last = min(clamped(base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
-    const int lim_min = clamped(base);                            // the first token sees up to here
-    u1 = min(u1, (last + kUnit) / kUnit);
-    if (!ONE && u0 >= u1) return;                           // no record: the merge reads none
-    // q, whose parts go to LDS once the first units' loads are on their way
-    const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
-    constexpr int NT = 64 * NW, QN = (R * (D / 8) + NT - 1) / NT;
-    uint4 qw[QN];
+    auto segment = [&](int b, int base, int u0, int u1) {
+        int tid = threadIdx.x;
+        if constexpr (!ONE) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
+        const int lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int l16 = lane & 15, lq = lane >> 4;
+        // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
+        auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
+        const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
+        const int lim_min = clamped(base);                            // the first token sees up to here
+        u1 = min(u1, (last + kUnit) / kUnit);
+        // q, whose parts go to LDS once the first units' loads are on their way
+        const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
+        constexpr int NT = 64 * NW, QN = (R * (D / 8) + NT - 1) / NT;
+        uint4 qw[QN];
 #pragma unroll
-    for (int i = 0; i < QN; ++i) {
-        const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-        qw[i] = make_uint4(0, 0, 0, 0);
-        if (r < rows && (R * (D / 8) % NT == 0 || tid + NT * i < R * (D / 8)))
-            qw[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)(r / G) * a.ldq + (r % G) * D + 8 * ch);
-    }
-    // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
-    uint32_t first[2];
-    auto find_rows = [&](int j0) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int64_t pos = ((int64_t)u0 + wave + NW * (j0 + lane)) * kUnit + 16 * t;
-            first[t] = kNoRow;
-            if (pos < a.c.max_pos) {
-                const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
-                first[t] = row < 0 ? kNoRow : (uint32_t)row;
-            }
+        for (int i = 0; i < QN; ++i) {
+            const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+            qw[i] = make_uint4(0, 0, 0, 0);
+            if (r < rows && (R * (D / 8) % NT == 0 || tid + NT * i < R * (D / 8)))
+                qw[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)(r / G) * a.ldq + (r % G) * D + 8 * ch);
         }
-    };
-    const Lane<D> off(lane);
-    // the wave's j-th unit: its tiles' rows, and which of them exist
-    auto locate = [&](int j, uint32_t (&row)[2]) -> int {
-        const uint32_t r0 = __builtin_amdgcn_readlane(first[0], j & 63), r1 = __builtin_amdgcn_readlane(first[1], j & 63);
-        row[0] = r0 == kNoRow ? 0 : r0;
-        row[1] = r1 == kNoRow ? 0 : r1;
-        return (r0 == kNoRow ? 0 : 1) | (r1 == kNoRow ? 0 : 2);
-    };
-    Raw<D> r;
-    int there = 0;
-    if (u0 + wave < u1) {
-        uint32_t row[2];
-        find_rows(0);
-        there = locate(0, row);
-        load_k(r, a.c, row, off);
-        load_v(r, a.c, row, off);
-    }
-#pragma unroll
-    for (int i = 0; i < QN; ++i) {
-        const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-        uint4 p[NQ];
-        q_parts<NQ>(qw[i], p);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j)
-            if (R * (D / 8) % NT == 0 || r < R) *reinterpret_cast<uint4*>(&qs[j * R + r][8 * ch]) = p[j];
-    }
-    __syncthreads();
-    // 0, or NaN where the row holds an infinity or a NaN (then so is its output)
-    float zero = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&qs[l16][(D / 4) * lq + 8 * kt]));
-    zero = over_lq<false>(zero);
-    // the lane's query is row l16; rows that are none see everything and write nothing
-    const int lim = l16 < rows ? clamped(base + l16 / G) : 1 << 30;
-    float m = kNone, l = 0.0f;
-    bool wide = false;   // uniform: a row's reference is past kWide
-    mx::v4f acc[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c] = mx::v4f{0.f, 0.f, 0.f, 0.f};
-    // Unit u, the wave's j-th.  `more`: the wave's next one is loaded meanwhile (decided in the code, not by a branch:
-    // behind one the compiler waits for the older loads as if these had not been issued, that is for all)
-    auto unit = [&](int u, int j, auto more_) {
-        constexpr bool more = decltype(more_)::value;
-        const int p0 = u * kUnit;
-        uint32_t next[2];
-        int there_next = 0;
-        if constexpr (more) {
-            if (((j + 1) & 63) == 0) find_rows(j + 1);
-            there_next = locate(j + 1, next);
-        }
-        mx::v4f sv[2];
-        sv[0] = sv[1] = mx::v4f{zero, zero, zero, zero};
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            uint4 qf[NQ];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) qf[n] = *reinterpret_cast<const uint4*>(&qs[n * R + l16][(D / 4) * lq + 8 * kt]);
+        // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
+        uint32_t first[2];
+        auto find_rows = [&](int j0) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint4 kd = kv4::eight_bf16(r.k[t][kt], kv4::scale_of(r.ks[t]));
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) sv[t] = mfma_bf16(kd, qf[n], sv[t]);
-            }
-        }
-        if constexpr (more) load_k(r, a.c, next, off);
-        // sv[t][i], s[4 t + i]: position p0 + 16 t + 4 lq + i
-        float s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = sv[i >> 2][i & 3];
-        const bool masked = __builtin_amdgcn_readfirstlane(p0 + kUnit - 1 > lim_min || there != 3);
-        if (masked) {
-            int sees = lim - p0 - 4 * lq;        // the last position that the lane's query sees
-            asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
-        }
-        uint4 p[1][kParts];
-        float t[8], sum;
-        terms(s, a.scale, m, wide, t, sum);
-        parts(t, p);
-        again(s, a.scale, m, l, wide, sum, p, [](float x) { return over_lq<true>(x); },
-              [&](float al) {
-#pragma unroll
-                  for (int c = 0; c < CT; ++c)
-#pragma unroll
-                      for (int i = 0; i < 4; ++i) acc[c][i] *= al;
-              });
-        __builtin_amdgcn_sched_barrier(0);   // 128 registers, four waves a SIMD: no operand of the second product before here,
-        float vs[8];
-        v_scales(r, vs);
-        if (masked) {
-            // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
-            int sees = last - p0 - 4 * lq;
-            asm volatile("" : "+v"(sees));
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) {
-                    r.v[i] = 0;
-                    vs[i] = 1.0f;
+                const int64_t pos = ((int64_t)u0 + wave + NW * (j0 + lane)) * kUnit + 16 * t;
+                first[t] = kNoRow;
+                if (pos < a.c.max_pos) {
+                    const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
+                    first[t] = row < 0 ? kNoRow : (uint32_t)row;
                 }
-        }
-        auto product = [&](auto half) {
-            constexpr int H = decltype(half)::value;
-            uint4 vd[4];
-            decode_v<H>(r.v, vs, vd);
-            if constexpr (H == CT / 4 - 1 && more) load_v(r, a.c, next, off);
-#pragma unroll
-            for (int k = kParts - 1; k >= 0; --k)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[4 * H + c] = mfma_bf16(vd[c], p[0][k], acc[4 * H + c]);
+            }
         };
-        product(std::integral_constant<int, 0>{});
-        __builtin_amdgcn_sched_barrier(0);   // and one half's at a time
-        if constexpr (CT == 8) product(std::integral_constant<int, 1>{});
-        there = there_next;
+        const Lane<D> off(lane);
+        // the wave's j-th unit: its tiles' rows, and which of them exist
+        auto locate = [&](int j, uint32_t (&row)[2]) -> int {
+            const uint32_t r0 = __builtin_amdgcn_readlane(first[0], j & 63), r1 = __builtin_amdgcn_readlane(first[1], j & 63);
+            row[0] = r0 == kNoRow ? 0 : r0;
+            row[1] = r1 == kNoRow ? 0 : r1;
+            return (r0 == kNoRow ? 0 : 1) | (r1 == kNoRow ? 0 : 2);
+        };
+        Raw<D> r;
+        int there = 0;
+        if (u0 + wave < u1) {
+            uint32_t row[2];
+            find_rows(0);
+            there = locate(0, row);
+            load_k(r, a.c, row, off);
+            load_v(r, a.c, row, off);
+        }
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+            uint4 p[NQ];
+            q_parts<NQ>(qw[i], p);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+                if (R * (D / 8) % NT == 0 || r < R) *reinterpret_cast<uint4*>(&qs[j * R + r][8 * ch]) = p[j];
+        }
+        __syncthreads();
+        // 0, or NaN where the row holds an infinity or a NaN (then so is its output)
+        float zero = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&qs[l16][(D / 4) * lq + 8 * kt]));
+        zero = over_lq<false>(zero);
+        // the lane's query is row l16; rows that are none see everything and write nothing
+        const int lim = l16 < rows ? clamped((int64_t)base + l16 / G) : 1 << 30;
+        float m = kNone, l = 0.0f;
+        bool wide = false;   // uniform: a row's reference is past kWide
+        mx::v4f acc[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[c] = mx::v4f{0.f, 0.f, 0.f, 0.f};
+        // Unit u, the wave's j-th.  `more`: the wave's next one is loaded meanwhile (decided in the code, not by a branch:
+        // behind one the compiler waits for the older loads as if these had not been issued, that is for all)
+        auto unit = [&](int u, int j, auto more_) {
+            constexpr bool more = decltype(more_)::value;
+            const int p0 = u * kUnit;
+            uint32_t next[2];
+            int there_next = 0;
+            if constexpr (more) {
+                if (((j + 1) & 63) == 0) find_rows(j + 1);
+                there_next = locate(j + 1, next);
+            }
+            mx::v4f sv[2];
+            sv[0] = sv[1] = mx::v4f{zero, zero, zero, zero};
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                uint4 qf[NQ];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) qf[n] = *reinterpret_cast<const uint4*>(&qs[n * R + l16][(D / 4) * lq + 8 * kt]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint4 kd = kv4::eight_bf16(r.k[t][kt], kv4::scale_of(r.ks[t]));
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) sv[t] = mfma_bf16(kd, qf[n], sv[t]);
+                }
+            }
+            if constexpr (more) load_k(r, a.c, next, off);
+            // sv[t][i], s[4 t + i]: position p0 + 16 t + 4 lq + i
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = sv[i >> 2][i & 3];
+            const bool masked = __builtin_amdgcn_readfirstlane(p0 + kUnit - 1 > lim_min || there != 3);
+            if (masked) {
+                int sees = lim - p0 - 4 * lq;        // the last position that the lane's query sees
+                asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
+            }
+            uint4 p[1][kParts];
+            float t[8], sum;
+            terms(s, a.scale, m, wide, t, sum);
+            parts(t, p);
+            again(s, a.scale, m, l, wide, sum, p, [](float x) { return over_lq<true>(x); },
+                  [&](float al) {
+#pragma unroll
+                      for (int c = 0; c < CT; ++c)
+#pragma unroll
+                          for (int i = 0; i < 4; ++i) acc[c][i] *= al;
+                  });
+            __builtin_amdgcn_sched_barrier(0);   // 128 registers, four waves a SIMD: no operand of the second product before here,
+            float vs[8];
+            v_scales(r, vs);
+            if (masked) {
+                // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
+                int sees = last - p0 - 4 * lq;
+                asm volatile("" : "+v"(sees));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) {
+                        r.v[i] = 0;
+                        vs[i] = 1.0f;
+                    }
+            }
+            auto product = [&](auto half) {
+                constexpr int H = decltype(half)::value;
+                uint4 vd[4];
+                decode_v<H>(r.v, vs, vd);
+                if constexpr (H == CT / 4 - 1 && more) load_v(r, a.c, next, off);
+#pragma unroll
+                for (int k = kParts - 1; k >= 0; --k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[4 * H + c] = mfma_bf16(vd[c], p[0][k], acc[4 * H + c]);
+            };
+            product(std::integral_constant<int, 0>{});
+            __builtin_amdgcn_sched_barrier(0);   // and one half's at a time
+            if constexpr (CT == 8) product(std::integral_constant<int, 1>{});
+            there = there_next;
+        };
+        int u = u0 + wave, j = 0;
+        for (; u + NW < u1; u += NW, ++j) unit(u, j, std::true_type{});
+        if (u < u1) unit(u, j, std::false_type{});
+        // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is
+        // column D/16 (4 lq + i) + c of query l16
+        __syncthreads();
+        const float ls = over_lq<false>(l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < CT; c += 4)
+                *reinterpret_cast<float4*>(&mo[wave][l16][CT * (4 * lq + i) + c]) = make_float4(acc[c][i], acc[c + 1][i], acc[c + 2][i], acc[c + 3][i]);
+        if (lq == 0) {
+            mm[wave][l16] = m;
+            ml[wave][l16] = ls;
+        }
+        __syncthreads();
+        // thread: CT columns of a row (8 of 128, 4 of 64)
+        const int qr = tid >> 4;
+        if (tid < 256 && qr < rows) finish<D, NW, ONE>(a, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
     };
-    int u = u0 + wave, j = 0;
-    for (; u + NW < u1; u += NW, ++j) unit(u, j, std::true_type{});
-    if (u < u1) unit(u, j, std::false_type{});
-    // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is
-    // column D/16 (4 lq + i) + c of query l16
-    __syncthreads();
-    const float ls = over_lq<false>(l);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < CT; c += 4)
-            *reinterpret_cast<float4*>(&mo[wave][l16][CT * (4 * lq + i) + c]) = make_float4(acc[c][i], acc[c + 1][i], acc[c + 2][i], acc[c + 3][i]);
-    if (lq == 0) {
-        mm[wave][l16] = m;
-        ml[wave][l16] = ls;
-    }
-    __syncthreads();
-    // thread: CT columns of a row (8 of 128, 4 of 64)
-    const int qr = tid >> 4;
-    if (tid < 256 && qr < rows) finish<D, NW, ONE>(a, b, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
+    if constexpr (ONE) segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
+    else each_segment(a, segment);
 }
 
 // Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b): the row's
@@ -325,10 +320,13 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     p.b = blockIdx.y;
     find_share(a, -1, p);
     const int g = blockIdx.x / rows, r = blockIdx.x - g * rows;
-    const int64_t pos = (int64_t)a.dpos[p.b] + r / a.G;
+    const int64_t pos = (int64_t)p.base + r / a.G;
+    // its records: those of the shares with its sequence's units 0 .. pos / kUnit
+    p.start += pad_of(a);
+    const int s0 = __builtin_amdgcn_readfirstlane(share_of(p.start, p.per));
     const int ns = __builtin_amdgcn_readfirstlane(
-        pos < 0 || pos >= a.c.max_pos ? 0 : (int)(pos / kUnit) / p.per + 1);   // shares of positions 0 .. pos
-    const float* rec = a.part + ((int64_t)blockIdx.x * a.shares + __builtin_amdgcn_readfirstlane(p.first)) * (D + 4);
+        pos < 0 || pos >= a.c.max_pos ? 0 : share_of(p.start + (uint64_t)(pos / kUnit), p.per) - s0 + 1);
+    const float* rec = a.part + ((int64_t)blockIdx.x * a.records + s0 + p.b) * (D + 4);
     float m = kNone, l = 0.0f;
     cvec o = 0.0f;
     for (int i0 = wave; i0 < ns; i0 += N * NW) {
@@ -385,7 +383,8 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
 
 struct Plan {
     bool many;       // rows for attn_rows
-    int groups, wanted, shares, most;   // shares the batch should and may have, and one sequence may
+    int groups, shares, most;   // shares of the batch (with `one` a sequence each), and one sequence may have
+    int records;     // of a row
     int waves;       // of a workgroup
     bool one;
 };
@@ -394,7 +393,7 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
     const int64_t rows = (int64_t)M * (Hq / Hkv);
     int64_t longest = (max_pos + kMinShare * kUnit - 1) / (kMinShare * kUnit);   // shares a sequence may have (share_units)
     if (longest > kFew) longest = std::max<int64_t>(kFew, (longest + 1) / 2);
-    const int64_t most = B * longest;
+    const int64_t most = B * (longest + (B > 1 ? kPad / kMinShare : 0));   // with a share of whole pads
     p.waves = 4;
     if (rows <= 16) {
         p.groups = 1;
@@ -407,12 +406,17 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
         p.many = true;
         p.groups = (int)((rows + 31) / 32);
     }
-    // shares of the whole batch for one round of workgroups: four or two a CU
-    const int64_t per = (int64_t)Hkv * p.groups;
-    const int64_t want = ((p.many ? 512 : 1024) + per - 1) / per;
-    p.one = p.waves == 16 || longest == 1 || want * 4 <= B || (want == 1 && B == 1);
-    p.wanted = (int)std::min(want, most);
-    p.shares = p.one ? B : p.wanted + (B > 1 ? B : 0);
+    // shares of the whole batch for one round of workgroups, four or two a CU, and none that starts a second round
+    const int64_t want = std::max<int64_t>(1, (p.many ? 512 : 1024) / ((int64_t)Hkv * p.groups));
+    // A workgroup for a sequence, no shares and no merge, where there are many and short ones.  us, shares / one, one
+    // token, sequences of one length and (in brackets) of 0 .. that: 512 workgroups, 2048 positions 43.9 / 31.1 (30.8 /
+    // 26.0), 4096 63.5 / 57.3 (38.2 / 49.2); 2048 workgroups, 8192 positions 446 / 406 (238 / 247).  Nine tokens, 384
+    // workgroups: 2048 positions 54.0 / 38.3 (43.0 / 36.6), 4096 79.5 / 69.0 (56.5 / 65.6).  One piece of a prompt of
+    // 128 tokens, 128 workgroups: 1024 positions 22.7 / 15.8, 8192 49.8 / 84.1.
+    const int64_t wgs = (int64_t)B * Hkv * p.groups;
+    p.one = p.waves == 16 || longest == 1 || want * 4 <= B || (want == 1 && B == 1) || max_pos <= (p.many ? 8 : 4) * wgs;
+    p.shares = p.one ? B : (int)std::min(want, most);
+    p.records = p.shares + B - 1;
     p.most = (int)std::min<int64_t>(longest, p.shares);
     return p;
 }
@@ -431,7 +435,7 @@ int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
 extern "C" size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos) {
     if (B <= 0 || M <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || max_pos <= 0) return 0;
     const Plan p = plan(B, M, Hq, Hkv, max_pos);
-    return p.one ? 0 : (size_t)p.shares * M * Hq * (D + 4) * sizeof(float);
+    return p.one ? 0 : (size_t)p.records * M * Hq * (D + 4) * sizeof(float);
 }
 
 extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,
@@ -468,7 +472,7 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     a.Hq = Hq;
     a.G = Hq / Hkv;
     a.shares = p.shares;
-    a.wanted = p.wanted;
+    a.records = p.records;
     a.scale = (float)(1.4426950408889634 / sqrt((double)D));
     const hipStream_t st = mxh::as_stream(stream);
     if (p.many) {

@@ -69,267 +69,262 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         alignas(16) float mo[kWaves][R][D + 4];
     } lds;
     __shared__ float mm[kWaves][R], ml[kWaves][R];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, lh = lane >> 5;
     const int g = blockIdx.y, r0 = blockIdx.z * R, G = a.G;
     const int rows = a.M * G;
-    int b = 0, u0 = 0, u1 = INT32_MAX;
-    if constexpr (ONE) {
-        b = blockIdx.x;
-    } else {
-        Place pl;
-        if (!find_share(a, blockIdx.x, pl)) return;        // uniform
-        b = pl.b;
-        u0 = pl.s * pl.per;
-        u1 = u0 + pl.per;
-    }
-    // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
-    const int64_t base = __builtin_amdgcn_readfirstlane(a.dpos[b]);
-    auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
-    const int last = min(clamped(base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
-    const int lim_min = __builtin_amdgcn_readfirstlane(clamped(base + r0 / G));        // the group's first token sees up to here
-    const int lim_max = __builtin_amdgcn_readfirstlane(min(clamped(base + (min(r0 + R, rows) - 1) / G), a.c.max_pos - 1));
-    u1 = min(u1, (lim_max + kUnit) / kUnit);
-    if (!ONE && u0 >= u1) return;                           // no record: the merge reads none
-    const int n = u0 + wave < u1 ? (u1 - u0 - wave + kWaves - 1) / kWaves : 0;   // the wave's units: u0 + wave + 4 j
-    // q, whose parts go to LDS once the first units' loads are on their way
-    constexpr int NT = 64 * kWaves, QN = (R * (D / 8) + NT - 1) / NT;
-    uint4 qw[QN];
+    auto segment = [&](int b, int base, int u0, int u1) {
+        int tid = threadIdx.x;
+        if constexpr (!ONE) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
+        const int lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int l32 = lane & 31, lh = lane >> 5;
+        // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
+        auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
+        const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
+        const int lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base + r0 / G));        // the group's first token sees up to here
+        const int lim_max = __builtin_amdgcn_readfirstlane(min(clamped((int64_t)base + (min(r0 + R, rows) - 1) / G), a.c.max_pos - 1));
+        u1 = min(u1, (lim_max + kUnit) / kUnit);
+        if (!ONE && u0 >= u1) return;                           // no row of the group sees the segment: no record
+        const int n = u0 + wave < u1 ? (u1 - u0 - wave + kWaves - 1) / kWaves : 0;   // the wave's units: u0 + wave + 4 j
+        // q, whose parts go to LDS once the first units' loads are on their way
+        constexpr int NT = 64 * kWaves, QN = (R * (D / 8) + NT - 1) / NT;
+        uint4 qw[QN];
 #pragma unroll
-    for (int i = 0; i < QN; ++i) {
-        const int r = r0 + (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-        qw[i] = make_uint4(0, 0, 0, 0);
-        if (r < rows) qw[i] = *reinterpret_cast<const uint4*>(a.q + ((int64_t)b * a.M + r / G) * a.ldq + (int64_t)(g * G + r % G) * D + 8 * ch);
-    }
-    // the first head rows of units j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
-    uint32_t first[2];
-    auto find_rows = [&](int j0) {
+        for (int i = 0; i < QN; ++i) {
+            const int r = r0 + (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+            qw[i] = make_uint4(0, 0, 0, 0);
+            if (r < rows) qw[i] = *reinterpret_cast<const uint4*>(a.q + ((int64_t)b * a.M + r / G) * a.ldq + (int64_t)(g * G + r % G) * D + 8 * ch);
+        }
+        // the first head rows of units j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
+        uint32_t first[2];
+        auto find_rows = [&](int j0) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int64_t pos = ((int64_t)u0 + wave + kWaves * (j0 + lane)) * kUnit + 16 * t;
-            first[t] = kNoRow;
-            if (pos < a.c.max_pos && j0 + lane < n) {
-                const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
-                first[t] = row < 0 ? kNoRow : (uint32_t)row;
+            for (int t = 0; t < 2; ++t) {
+                const int64_t pos = ((int64_t)u0 + wave + kWaves * (j0 + lane)) * kUnit + 16 * t;
+                first[t] = kNoRow;
+                if (pos < a.c.max_pos && j0 + lane < n) {
+                    const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
+                    first[t] = row < 0 ? kNoRow : (uint32_t)row;
+                }
             }
-        }
-    };
-    struct Unit {
-        uint32_t x, y;    // its tiles' first head rows
-        int there, p0;    // which of them exist (none past the last unit), and its first position
-    };
-    auto locate = [&](int j) {
-        if ((j & 63) == 0) find_rows(j);
-        const uint32_t x = __builtin_amdgcn_readlane(first[0], j & 63), y = __builtin_amdgcn_readlane(first[1], j & 63);
-        return Unit{x == kNoRow ? 0 : x, y == kNoRow ? 0 : y, (x == kNoRow ? 0 : 1) | (y == kNoRow ? 0 : 2), (u0 + wave + kWaves * j) * kUnit};
-    };
-    // a unit's bytes, in few and wide loads.  K: row l32, half lh; codes: those of K's (lane < 32) or V's position l32, one
-    // word; V: D/8 bytes of row 16 t + lane / 4
-    v4u rk[D / 64];
-    hvec rv[2];
-    uint32_t rcodes;
-    const uint8_t* const codes_of = lane < 32 ? a.c.ks : a.c.vs;
-    auto load_k = [&](const Unit& u) {
-        const uint64_t at = (uint64_t)(l32 < 16 ? u.x : u.y) + (l32 & 15);
-        const uint8_t* p = a.c.kq + at * (D / 2) + lh * (D / 4);
+        };
+        struct Unit {
+            uint32_t x, y;    // its tiles' first head rows
+            int there, p0;    // which of them exist (none past the last unit), and its first position
+        };
+        auto locate = [&](int j) {
+            if ((j & 63) == 0) find_rows(j);
+            const uint32_t x = __builtin_amdgcn_readlane(first[0], j & 63), y = __builtin_amdgcn_readlane(first[1], j & 63);
+            return Unit{x == kNoRow ? 0 : x, y == kNoRow ? 0 : y, (x == kNoRow ? 0 : 1) | (y == kNoRow ? 0 : 2), (u0 + wave + kWaves * j) * kUnit};
+        };
+        // a unit's bytes, in few and wide loads.  K: row l32, half lh; codes: those of K's (lane < 32) or V's position l32, one
+        // word; V: D/8 bytes of row 16 t + lane / 4
+        v4u rk[D / 64];
+        hvec rv[2];
+        uint32_t rcodes;
+        const uint8_t* const codes_of = lane < 32 ? a.c.ks : a.c.vs;
+        auto load_k = [&](const Unit& u) {
+            const uint64_t at = (uint64_t)(l32 < 16 ? u.x : u.y) + (l32 & 15);
+            const uint8_t* p = a.c.kq + at * (D / 2) + lh * (D / 4);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) rk[i] = *reinterpret_cast<const v4u*>(p + 16 * i);
-        const uint8_t* s = codes_of + at * (D / 32);
-        if constexpr (D == 128) rcodes = *reinterpret_cast<const uint32_t*>(s);
-        else rcodes = *reinterpret_cast<const uint16_t*>(s);
-    };
-    auto load_v = [&](const Unit& u) {
-        rv[0] = *reinterpret_cast<const hvec*>(a.c.vq + (uint64_t)u.x * (D / 2) + lane * (D / 8));
-        rv[1] = *reinterpret_cast<const hvec*>(a.c.vq + (uint64_t)u.y * (D / 2) + lane * (D / 8));
-    };
-    Stage<D>& stage = lds.in.stage[wave];
-    // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
-    auto ragged = [&](const Unit& u) { return __builtin_amdgcn_readfirstlane(u.there != 3 || u.p0 + kUnit - 1 > last); };
-    auto put_codes = [&](int j, const Unit& u) {
-        if (ragged(u)) {
-            int sees = last - u.p0;
-            asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
-            if (!(u.there >> (l32 >> 4) & 1) || l32 > sees) rcodes = 0x7F7F7F7Fu;
-        }
-        stage.codes[j & 1][lane] = rcodes;
-    };
-    auto put_v = [&](int j, const Unit& u) {
-        if (ragged(u)) {
-            int sees = last - u.p0;
-            asm volatile("" : "+v"(sees));
+            for (int i = 0; i < D / 64; ++i) rk[i] = *reinterpret_cast<const v4u*>(p + 16 * i);
+            const uint8_t* s = codes_of + at * (D / 32);
+            if constexpr (D == 128) rcodes = *reinterpret_cast<const uint32_t*>(s);
+            else rcodes = *reinterpret_cast<const uint16_t*>(s);
+        };
+        auto load_v = [&](const Unit& u) {
+            rv[0] = *reinterpret_cast<const hvec*>(a.c.vq + (uint64_t)u.x * (D / 2) + lane * (D / 8));
+            rv[1] = *reinterpret_cast<const hvec*>(a.c.vq + (uint64_t)u.y * (D / 2) + lane * (D / 8));
+        };
+        Stage<D>& stage = lds.in.stage[wave];
+        // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
+        auto ragged = [&](const Unit& u) { return __builtin_amdgcn_readfirstlane(u.there != 3 || u.p0 + kUnit - 1 > last); };
+        auto put_codes = [&](int j, const Unit& u) {
+            if (ragged(u)) {
+                int sees = last - u.p0;
+                asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
+                if (!(u.there >> (l32 >> 4) & 1) || l32 > sees) rcodes = 0x7F7F7F7Fu;
+            }
+            stage.codes[j & 1][lane] = rcodes;
+        };
+        auto put_v = [&](int j, const Unit& u) {
+            if (ragged(u)) {
+                int sees = last - u.p0;
+                asm volatile("" : "+v"(sees));
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (!(u.there >> t & 1) || 16 * t + (lane >> 2) > sees) rv[t] = 0;
+            }
+            const int r = lane >> 2;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                if (!(u.there >> t & 1) || 16 * t + (lane >> 2) > sees) rv[t] = 0;
+                *reinterpret_cast<hvec*>(&stage.v[j & 1][t][(r & 8) + 2 * (r & 3) + ((r >> 2) & 1)][(lane & 3) * (D / 8)]) = rv[t];
+        };
+        Unit ua = locate(0), ub = ua, uc = ua;
+        load_k(ua);
+        load_v(ua);
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
+            uint4 p[NQ];
+            q_parts<NQ>(qw[i], p);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+                if (R * (D / 8) % NT == 0 || r < R) *reinterpret_cast<uint4*>(&lds.in.qs[j * R + r][8 * ch]) = p[j];
         }
-        const int r = lane >> 2;
+        __syncthreads();
+        // the lane's query is row r0 + l32; rows that are none see everything and write nothing.
+        // zero: 0, or NaN where the row holds an infinity or a NaN (then so is its output)
+        const int lim = r0 + l32 < rows ? clamped((int64_t)base + (r0 + l32) / G) : 1 << 30;
+        float zero = 0.0f, m = kNone, l = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-            *reinterpret_cast<hvec*>(&stage.v[j & 1][t][(r & 8) + 2 * (r & 3) + ((r >> 2) & 1)][(lane & 3) * (D / 8)]) = rv[t];
-    };
-    Unit ua = locate(0), ub = ua, uc = ua;
-    load_k(ua);
-    load_v(ua);
-#pragma unroll
-    for (int i = 0; i < QN; ++i) {
-        const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-        uint4 p[NQ];
-        q_parts<NQ>(qw[i], p);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j)
-            if (R * (D / 8) % NT == 0 || r < R) *reinterpret_cast<uint4*>(&lds.in.qs[j * R + r][8 * ch]) = p[j];
-    }
-    __syncthreads();
-    // the lane's query is row r0 + l32; rows that are none see everything and write nothing.
-    // zero: 0, or NaN where the row holds an infinity or a NaN (then so is its output)
-    const int lim = r0 + l32 < rows ? clamped(base + (r0 + l32) / G) : 1 << 30;
-    float zero = 0.0f, m = kNone, l = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&lds.in.qs[l32][(D / 2) * lh + 8 * kt]));
-    zero = over_lh<false>(zero);
-    bool wide = false;
-    mx::v16f acc[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
-
-    // S^T of unit j, whose K is in rk
-    auto scores = [&](int j, const Unit& u, float (&s)[16]) {
-        put_codes(j, u);
-        mx::v16f sv;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sv[i] = zero;
-        const uint32_t w = stage.codes[j & 1][l32];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const uint4 kd = kv4::eight_bf16(rk[kt / 4][kt & 3], scale_at(w, D == 128 ? 2 * lh + (kt >> 2) : lh));
-#pragma unroll
-            for (int k = 0; k < NQ; ++k)
-                sv = mfma32(kd, *reinterpret_cast<const uint4*>(&lds.in.qs[k * R + l32][(D / 2) * lh + 8 * kt]), sv);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = sv[i];
-    };
-    auto masked = [&](const Unit& u, float (&s)[16]) {
-        if (__builtin_amdgcn_readfirstlane(u.p0 + kUnit - 1 > lim_min || u.there != 3)) {
-            int sees = lim - u.p0 - 4 * lh;      // the last position that the lane's query sees
-            asm volatile("" : "+v"(sees));
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!(u.there >> (i >> 3) & 1) || 8 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
-        }
-    };
-    // O^T += V^T P^T of unit j
-    auto products = [&](int j, const uint4 (&p)[2][NP]) {
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {         // eight positions a step
-            uint32_t v[8];
-            float sc[8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint4 w4 = *reinterpret_cast<const uint4*>(&stage.codes[j & 1][32 + 16 * st + 8 * h + 4 * lh]);
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint8_t* x = &stage.v[j & 1][st][8 * h + 2 * i + lh][l32 * (CT / 2)];
-                    if constexpr (D == 128) v[4 * h + i] = *reinterpret_cast<const uint16_t*>(x);
-                    else v[4 * h + i] = *x;
-                    sc[4 * h + i] = scale_at(w[i], D == 128 ? l32 >> 3 : l32 >> 4);
-                }
-            }
-            uint32_t o[CT][4];
-            auto columns = [&](auto pair_) {     // columns 2 P, 2 P + 1 of the lane's
-                constexpr int P = decltype(pair_)::value;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t x = kv4::pair_bf16<P>(v[2 * k], sc[2 * k]), y = kv4::pair_bf16<P>(v[2 * k + 1], sc[2 * k + 1]);
-                    o[2 * P][k] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-                    o[2 * P + 1][k] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-                }
-            };
-            columns(std::integral_constant<int, 0>{});
-            if constexpr (D == 128) columns(std::integral_constant<int, 1>{});
-#pragma unroll
-            for (int k = NP - 1; k >= 0; --k)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) acc[c] = mfma32(make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]), p[st][k], acc[c]);
-        }
-    };
-    auto over = [](float x) { return over_lh<true>(x); };
-    auto rescale = [&](float al) {
+        for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&lds.in.qs[l32][(D / 2) * lh + 8 * kt]));
+        zero = over_lh<false>(zero);
+        bool wide = false;
+        mx::v16f acc[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c][i] *= al;
-    };
-    // A software pipeline, because a wave issues in order: while the matrix unit works on unit j's second product, the
-    // vector unit makes unit j + 1's terms, and unit j + 2's scores come after.
-    float s[16];
-    uint4 pa[2][NP], pb[2][NP];
-    auto step = [&](int j, const uint4 (&p)[2][NP], uint4 (&pn)[2][NP]) {     // unit j + 1 exists: ua is it, ub the one after
-        masked(ua, s);
-        float t[16], sum;
-        terms(s, a.scale, m, wide, t, sum);
-        parts(t, pn);
-        products(j, p);
-        again(s, a.scale, m, l, wide, sum, pn, over, rescale);
-        put_v(j + 1, ua);
-        load_v(ub);
-        if (j + 2 < n) scores(j + 2, ub, s);
-        load_k(uc);
-        ua = ub;
-        ub = uc;
-        uc = locate(j + 4);
-    };
-    if (n > 0) {
-        scores(0, ua, s);
-        ub = locate(1);
-        load_k(ub);
-        put_v(0, ua);
-        load_v(ub);
-        masked(ua, s);
-        float t[16], sum;
-        terms(s, a.scale, m, wide, t, sum);
-        parts(t, pa);
-        again(s, a.scale, m, l, wide, sum, pa, over, rescale);
-        ua = ub;
-        ub = locate(2);
-        if (n > 1) scores(1, ua, s);
-        load_k(ub);
-        uc = locate(3);
-        int j = 0;
-        for (; j + 2 < n; j += 2) {
-            step(j, pa, pb);
-            step(j + 1, pb, pa);
-        }
-        if (j + 1 < n) {
-            step(j, pa, pb);
-            products(j + 1, pb);
-        } else {
-            products(j, pa);
-        }
-    }
-    // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is column
-    // CT (8 (i / 4) + 4 lh + i % 4) + c of query l32
-    __syncthreads();
-    const float ls = over_lh<false>(l);
+            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+
+        // S^T of unit j, whose K is in rk
+        auto scores = [&](int j, const Unit& u, float (&s)[16]) {
+            put_codes(j, u);
+            mx::v16f sv;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float* o = &lds.mo[wave][l32][CT * (8 * (i / 4) + 4 * lh + i % 4)];
-        if constexpr (CT == 4) *reinterpret_cast<float4*>(o) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
-        else *reinterpret_cast<float2*>(o) = make_float2(acc[0][i], acc[1][i]);
-    }
-    if (lh == 0) {
-        mm[wave][l32] = m;
-        ml[wave][l32] = ls;
-    }
-    __syncthreads();
+            for (int i = 0; i < 16; ++i) sv[i] = zero;
+            const uint32_t w = stage.codes[j & 1][l32];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const uint4 kd = kv4::eight_bf16(rk[kt / 4][kt & 3], scale_at(w, D == 128 ? 2 * lh + (kt >> 2) : lh));
+#pragma unroll
+                for (int k = 0; k < NQ; ++k)
+                    sv = mfma32(kd, *reinterpret_cast<const uint4*>(&lds.in.qs[k * R + l32][(D / 2) * lh + 8 * kt]), sv);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = sv[i];
+        };
+        auto masked = [&](const Unit& u, float (&s)[16]) {
+            if (__builtin_amdgcn_readfirstlane(u.p0 + kUnit - 1 > lim_min || u.there != 3)) {
+                int sees = lim - u.p0 - 4 * lh;      // the last position that the lane's query sees
+                asm volatile("" : "+v"(sees));
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(u.there >> (i >> 3) & 1) || 8 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
+            }
+        };
+        // O^T += V^T P^T of unit j
+        auto products = [&](int j, const uint4 (&p)[2][NP]) {
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {         // eight positions a step
+                uint32_t v[8];
+                float sc[8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(&stage.codes[j & 1][32 + 16 * st + 8 * h + 4 * lh]);
+                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint8_t* x = &stage.v[j & 1][st][8 * h + 2 * i + lh][l32 * (CT / 2)];
+                        if constexpr (D == 128) v[4 * h + i] = *reinterpret_cast<const uint16_t*>(x);
+                        else v[4 * h + i] = *x;
+                        sc[4 * h + i] = scale_at(w[i], D == 128 ? l32 >> 3 : l32 >> 4);
+                    }
+                }
+                uint32_t o[CT][4];
+                auto columns = [&](auto pair_) {     // columns 2 P, 2 P + 1 of the lane's
+                    constexpr int P = decltype(pair_)::value;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = kv4::pair_bf16<P>(v[2 * k], sc[2 * k]), y = kv4::pair_bf16<P>(v[2 * k + 1], sc[2 * k + 1]);
+                        o[2 * P][k] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                        o[2 * P + 1][k] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                    }
+                };
+                columns(std::integral_constant<int, 0>{});
+                if constexpr (D == 128) columns(std::integral_constant<int, 1>{});
+#pragma unroll
+                for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] = mfma32(make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]), p[st][k], acc[c]);
+            }
+        };
+        auto over = [](float x) { return over_lh<true>(x); };
+        auto rescale = [&](float al) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c][i] *= al;
+        };
+        // A software pipeline, because a wave issues in order: while the matrix unit works on unit j's second product, the
+        // vector unit makes unit j + 1's terms, and unit j + 2's scores come after.
+        float s[16];
+        uint4 pa[2][NP], pb[2][NP];
+        auto step = [&](int j, const uint4 (&p)[2][NP], uint4 (&pn)[2][NP]) {     // unit j + 1 exists: ua is it, ub the one after
+            masked(ua, s);
+            float t[16], sum;
+            terms(s, a.scale, m, wide, t, sum);
+            parts(t, pn);
+            products(j, p);
+            again(s, a.scale, m, l, wide, sum, pn, over, rescale);
+            put_v(j + 1, ua);
+            load_v(ub);
+            if (j + 2 < n) scores(j + 2, ub, s);
+            load_k(uc);
+            ua = ub;
+            ub = uc;
+            uc = locate(j + 4);
+        };
+        if (n > 0) {
+            scores(0, ua, s);
+            ub = locate(1);
+            load_k(ub);
+            put_v(0, ua);
+            load_v(ub);
+            masked(ua, s);
+            float t[16], sum;
+            terms(s, a.scale, m, wide, t, sum);
+            parts(t, pa);
+            again(s, a.scale, m, l, wide, sum, pa, over, rescale);
+            ua = ub;
+            ub = locate(2);
+            if (n > 1) scores(1, ua, s);
+            load_k(ub);
+            uc = locate(3);
+            int j = 0;
+            for (; j + 2 < n; j += 2) {
+                step(j, pa, pb);
+                step(j + 1, pb, pa);
+            }
+            if (j + 1 < n) {
+                step(j, pa, pb);
+                products(j + 1, pb);
+            } else {
+                products(j, pa);
+            }
+        }
+        // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is column
+        // CT (8 (i / 4) + 4 lh + i % 4) + c of query l32
+        __syncthreads();
+        const float ls = over_lh<false>(l);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float* o = &lds.mo[wave][l32][CT * (8 * (i / 4) + 4 * lh + i % 4)];
+            if constexpr (CT == 4) *reinterpret_cast<float4*>(o) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+            else *reinterpret_cast<float2*>(o) = make_float2(acc[0][i], acc[1][i]);
+        }
+        if (lh == 0) {
+            mm[wave][l32] = m;
+            ml[wave][l32] = ls;
+        }
+        __syncthreads();
 #pragma unroll 1
-    for (int qr = tid >> 4; qr < R; qr += NT / 16)
-        if (r0 + qr < rows)
-            finish<D, kWaves, ONE>(a, b, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
-                                   [&](int w, int c) { return *reinterpret_cast<const float4*>(&lds.mo[w][qr][c]); });
+        for (int qr = tid >> 4; qr < R; qr += NT / 16)
+            if (r0 + qr < rows)
+                finish<D, kWaves, ONE>(a, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
+                                       [&](int w, int c) { return *reinterpret_cast<const float4*>(&lds.mo[w][qr][c]); });
+    };
+    if constexpr (ONE) segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
+    else each_segment(a, segment);
 }
 
 template <int D, int NQ, int NP>

@@ -188,6 +188,29 @@ def test_attention(case):
     assert np.array_equal(np_(oq), wq) and np.array_equal(np_(os_), ws)
 
 
+@pytest.mark.parametrize("B,M,Hkv,G,D,S", [(700, 1, 2, 3, 64, 8192), (250, 5, 1, 8, 128, 8192), (250, 7, 1, 5, 64, 4096), (70, 2, 1, 8, 128, 2048),
+                                          (3, 1, 4, 8, 128, 8192)])
+def test_long_and_short_sequences_together(B, M, Hkv, G, D, S):
+    """One long sequence among many of a few positions, some slots empty: several sequences in a share, and a
+    sequence in several shares."""
+    rng = np.random.default_rng(B)
+    dpos = rng.integers(0, 60, B)
+    dpos[rng.permutation(B)[:B // 8]] = -M
+    dpos[B // 3] = S - M - 100
+    need = (np.maximum(dpos + M, 0) + 15) // 16
+    ids = iter(rng.permutation(int(need.sum()) + 3))
+    pages = np.full((B, S // 16), -1, np.int32)
+    for b in range(B):
+        pages[b, :need[b]] = [next(ids) for _ in range(need[b])]
+    cache = _host_cache(rng, int(need.sum()) + 3, Hkv, 16, D)
+    q = torch.from_numpy(rng.standard_normal((B, M, Hkv * G, D))).bfloat16().to(DEV)
+    dev, dp, tab = _dev(cache), _i32(dpos), _i32(pages)
+    for dt in (torch.float32, torch.float16):
+        o = kv4.attn_decode4(q, dev, dp, tab, dt)
+        _check(o, q, cache, dpos, pages)
+        assert torch.equal(o, kv4.attn_decode4(q, dev, dp, tab, dt))
+
+
 def test_pages_that_are_none():
     """Holes in a table are positions that no token sees; rows with nothing else are zeros."""
     rng = np.random.default_rng(8)
