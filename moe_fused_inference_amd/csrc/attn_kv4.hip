@@ -115,8 +115,9 @@ __device__ __forceinline__ void decode_v(const uint32_t (&v)[8], const float (&s
     for (int c = 0; c < 4; ++c) vd[c] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
 }
 
-template <int D, int NQ, bool ONE, int NW>
+template <int D, int NQ, Work W, int NW>
 __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
+    constexpr bool ONE = W == Work::kSequence;
     constexpr int R = 16, KT = D / 32, CT = D / 16;
     // q, and after the last unit the waves' sums
     __shared__ union Lds {
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
     const int g = blockIdx.y, G = a.G, rows = a.M * G;     // at most 16
     auto segment = [&](int b, int base, int u0, int u1) {
         int tid = threadIdx.x;
-        if constexpr (!ONE) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
+        if constexpr (W == Work::kLine) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
         const int lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int l16 = lane & 15, lq = lane >> 4;
@@ -300,8 +301,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         const int qr = tid >> 4;
         if (tid < 256 && qr < rows) finish<D, NW, ONE>(a, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
     };
-    if constexpr (ONE) segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
-    else each_segment(a, segment);
+    each_segment<W>(a, segment);
 }
 
 // Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b): the row's
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     const int64_t pos = (int64_t)p.base + r / a.G;
     // its records: those of the shares with its sequence's units 0 .. pos / kUnit
     p.start += pad_of(a);
-    const int s0 = __builtin_amdgcn_readfirstlane(share_of(p.start, p.per));
+    const int s0 = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(share_of(p.start, p.per));
     const int ns = __builtin_amdgcn_readfirstlane(
         pos < 0 || pos >= a.c.max_pos ? 0 : share_of(p.start + (uint64_t)(pos / kUnit), p.per) - s0 + 1);
     const float* rec = a.part + ((int64_t)blockIdx.x * a.records + s0 + p.b) * (D + 4);
@@ -481,10 +481,11 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
         return merge(a, p, D, st);
     }
     const dim3 grid(p.shares, Hkv);
-#define MXH_K4(DD, QQ)                                                                                     \
-    if (p.waves == 16) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, true, 16>), grid, dim3(1024), 0, st, a); \
-    else if (p.one) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, true, 4>), grid, dim3(256), 0, st, a);      \
-    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, false, 4>), grid, dim3(256), 0, st, a)
+#define MXH_K4(DD, QQ)                                                                                                \
+    if (p.waves == 16) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 16>), grid, dim3(1024), 0, st, a); \
+    else if (p.one) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 4>), grid, dim3(256), 0, st, a);      \
+    else if (B == 1) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kShare, 4>), grid, dim3(256), 0, st, a);        \
+    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kLine, 4>), grid, dim3(256), 0, st, a)
     if (D == 64) {
         if (q_dtype == MXFP4_DT_BF16) { MXH_K4(64, 1); } else { MXH_K4(64, 2); }
     } else {

@@ -55,8 +55,9 @@ struct Stage {
     alignas(16) uint32_t codes[2][64];        // K's of the unit's 32 positions, then V's
 };
 
-template <int D, int NQ, int NP, bool ONE>
+template <int D, int NQ, int NP, Work W>
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
+    constexpr bool ONE = W == Work::kSequence;
     constexpr int R = 32, KT = D / 16, CT = D / 32;    // rows, steps of S, column tiles (and a lane's columns)
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     typedef uint32_t hvec __attribute__((ext_vector_type(D / 32)));
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
     const int rows = a.M * G;
     auto segment = [&](int b, int base, int u0, int u1) {
         int tid = threadIdx.x;
-        if constexpr (!ONE) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
+        if constexpr (W == Work::kLine) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
         const int lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int l32 = lane & 31, lh = lane >> 5;
@@ -323,15 +324,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 finish<D, kWaves, ONE>(a, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
                                        [&](int w, int c) { return *reinterpret_cast<const float4*>(&lds.mo[w][qr][c]); });
     };
-    if constexpr (ONE) segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
-    else each_segment(a, segment);
+    each_segment<W>(a, segment);
 }
 
 template <int D, int NQ, int NP>
 void launch(const Args& a, int groups, bool one, hipStream_t st) {
     const dim3 grid(a.shares, a.c.Hkv, groups);
-    if (one) hipLaunchKernelGGL((attn_kv4_rows_kernel<D, NQ, NP, true>), grid, dim3(64 * kWaves), 0, st, a);
-    else hipLaunchKernelGGL((attn_kv4_rows_kernel<D, NQ, NP, false>), grid, dim3(64 * kWaves), 0, st, a);
+    const auto kernel = one        ? attn_kv4_rows_kernel<D, NQ, NP, Work::kSequence>
+                        : a.B == 1 ? attn_kv4_rows_kernel<D, NQ, NP, Work::kShare>
+                                   : attn_kv4_rows_kernel<D, NQ, NP, Work::kLine>;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, st, a);
 }
 template <int D>
 void launch(const Args& a, int q_dtype, int groups, bool one, bool exact, hipStream_t st) {

@@ -79,8 +79,9 @@ def attention(q, cache, dpos, pages=None):
         n = min(int(dpos[b]) + M, top)
         if n <= 0:
             continue
-        k, v, there = read(cache, n, [0] * (b + 1), None if pages is None else pages[:b + 1])
-        k, v, there = k[b].astype(np.float64), v[b].astype(np.float64), there[b]
+        one = (cache, pages[b:b + 1]) if pages is not None else ([x[b:b + 1] for x in cache], None)
+        k, v, there = read(one[0], n, [0], one[1])
+        k, v, there = k[0].astype(np.float64), v[0].astype(np.float64), there[0]
         k[~there] = 0
         v[~there] = 0
         for m in range(M):
