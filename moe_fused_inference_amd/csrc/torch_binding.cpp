@@ -17,6 +17,7 @@
 // call).  Compiled by the host compiler (no device code here) and linked
 // against libmxfp4_hip.so.
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdint>
@@ -271,6 +272,11 @@ struct Kv4 {
     int n_pages, page, max_pages, B, Hkv, D;
 };
 
+// torch::empty on t's device, without the dispatcher: about half its time, which a small call's two or three show.
+torch::Tensor empty_on(const torch::Tensor& t, at::IntArrayRef sizes, c10::ScalarType dt) {
+    return at::detail::empty_cuda(sizes, dt, t.device(), c10::nullopt);
+}
+
 int as_int(int64_t v, const char* msg) {
     require(v >= 0 && v <= 0x7FFFFFFF, msg);
     return (int)v;
@@ -347,8 +353,7 @@ std::vector<torch::Tensor> kv4_read(const torch::Tensor& kq, const torch::Tensor
     require(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32, "dtype must be bfloat16, float16 or float32");
     const int n = as_int(n_, "n must not be negative");
     const c10::DeviceGuard guard(kq.device());
-    auto k = torch::empty({c.B, n, c.Hkv, c.D}, kq.options().dtype(dt));
-    auto v = torch::empty({c.B, n, c.Hkv, c.D}, kq.options().dtype(dt));
+    auto k = empty_on(kq, {c.B, n, c.Hkv, c.D}, dt), v = empty_on(kq, {c.B, n, c.Hkv, c.D}, dt);
     if (n != 0 && c.B != 0) {
         check(mxfp4_kv4_read(c.kq, c.ks, c.vq, c.vs, c.pages, c.n_pages, c.page, c.max_pages, c.at, k.data_ptr(), v.data_ptr(),
                              dtype_code(dt), c.B, n, c.Hkv, c.D, stream_of(kq)),
@@ -368,7 +373,7 @@ void kv4_attn_into(const torch::Tensor& q, const Kv4& c, const torch::Tensor& kq
     require(max_pos <= (1ll << 30), "attn_decode4: more than 2^30 positions a sequence");
     const size_t wsb = mxfp4_attn_kv4_workspace_size(c.B, M, Hq, c.Hkv, c.D, (int)max_pos);
     torch::Tensor ws;
-    if (wsb) ws = torch::empty({(int64_t)wsb}, kq.options());
+    if (wsb) ws = empty_on(kq, {(int64_t)wsb}, torch::kUInt8);
     check(mxfp4_attn_kv4(qc.data_ptr(), dtype_code(qc.scalar_type()), token_stride(qc), c.kq, c.ks, c.vq, c.vs, c.pages,
                          c.n_pages, c.page, c.max_pages, c.at, o.defined() ? o.data_ptr() : nullptr,
                          o.defined() ? dtype_code(o.scalar_type()) : 2, oq.defined() ? u8m(oq) : nullptr,
@@ -395,7 +400,7 @@ torch::Tensor kv4_attn(const torch::Tensor& q, const torch::Tensor& kq, const to
     const auto dt = torch::python::detail::py_object_to_dtype(dtype);
     require(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32, "dtype must be bfloat16, float16 or float32");
     const c10::DeviceGuard guard(kq.device());
-    auto o = torch::empty(q.sizes(), q.options().dtype(dt));
+    auto o = empty_on(q, q.sizes(), dt);
     if (o.numel() != 0) kv4_attn_into(q, c, kq, o, torch::Tensor(), torch::Tensor());
     return o;
 }
@@ -406,7 +411,7 @@ std::vector<torch::Tensor> kv4_attn_mx(const torch::Tensor& q, const torch::Tens
     const Kv4 c = kv4_attn_args(q, kq, ks, vq, vs, dpos, pages);
     const c10::DeviceGuard guard(kq.device());
     const int64_t T = q.size(0) * q.size(1), row = q.size(2) * q.size(3);
-    auto oq = torch::empty({T, row / 2}, kq.options()), os = torch::empty({T, row / 32}, kq.options());
+    auto oq = empty_on(kq, {T, row / 2}, torch::kUInt8), os = empty_on(kq, {T, row / 32}, torch::kUInt8);
     if (T != 0) kv4_attn_into(q, c, kq, torch::Tensor(), oq, os);
     return {oq, os};
 }
