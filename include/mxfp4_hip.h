@@ -230,7 +230,8 @@ int mxfp4_kv_write(const void* k, const void* v, uint8_t* kvk, uint8_t* kvv, con
  *              out yet).  NULL: sequence b is page b (n_pages >= B, max_pages
  *              unused)
  * A sequence has positions 0 .. max_pos - 1, max_pos = page (pages NULL) or
- * max_pages * page, at most 2^30.  dpos: device int32 (B), token m of sequence
+ * max_pages * page, at most 2^30; a cache has less than 2^32 - 1 head rows
+ * (n_pages * Hkv * page).  dpos: device int32 (B), token m of sequence
  * b sits at dpos[b] + m; read on the device, so a captured graph follows it.
  * A slot of the batch that is empty has dpos[b] <= -M.
  * Scale code 255 is no scale (the quantizer writes 0 .. 253) and reads as NaN.
@@ -275,7 +276,10 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  *   workspace  16-byte aligned, mxfp4_attn_kv4_workspace_size(B, M, Hq, Hkv, D,
  *              max_pos) bytes (0: may be NULL); nothing persists, but calls that
  *              share one must be stream-ordered
- * Sums and softmax in fp32.  A token outside [0, max_pos), or one that sees no
+ * Sums and softmax in fp32.  The products are bf16 with every operand exact: q in
+ * one part (fp16: two), a probability in three, or in two (16 bits, 2^-17 of it)
+ * where more than 16 rows (M * Hq / Hkv) go to bf16 or fp16 alone.  A token outside
+ * [0, max_pos), or one that sees no
  * position, gets zeros.  What the cache holds past dpos[b] + M - 1 is without
  * effect, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
  * The sums of a token are rounded in an order that depends on the batch's
