@@ -282,6 +282,7 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  * [0, max_pos), or one that sees no
  * position, gets zeros.  What the cache holds past dpos[b] + M - 1 is without
  * effect, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
+ * Keys and values that reach past fp32 (code 253 or 254) are infinite and give NaN.
  * The sums of a token are rounded in an order that depends on the batch's
  * lengths, not on when the workgroups run: the same call gives the same bits.
  */

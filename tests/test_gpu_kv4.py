@@ -226,6 +226,106 @@ def test_pages_that_are_none():
     assert not o[2].any() and not o[3].any() and o[0].any()
 
 
+@pytest.mark.parametrize("M,Hkv,G,D", [(1, 1, 8, 128), (5, 1, 8, 128), (1, 2, 3, 64), (7, 2, 5, 64)])
+def test_holes_in_long_tables(M, Hkv, G, D):
+    rng = np.random.default_rng(M + G)
+    cache = _host_cache(rng, 90, Hkv, 16, D)
+    pages = rng.integers(0, 90, (2, 128)).astype(np.int32)
+    pages[rng.random((2, 128)) < 0.4] = -1
+    pages[1, 40:70] = 90
+    dpos = [2040, 1300]
+    q = torch.from_numpy(rng.standard_normal((2, M, Hkv * G, D))).bfloat16().to(DEV)
+    for dt in (torch.float32, torch.bfloat16):
+        _check(kv4.attn_decode4(q, _dev(cache), _i32(dpos), _i32(pages), dt), q, cache, dpos, pages)
+
+
+@pytest.mark.parametrize("M,Hkv,G,D", [(1, 4, 8, 64), (1, 1, 4, 128), (9, 1, 8, 128), (16, 2, 1, 64), (40, 1, 1, 128)])
+def test_a_long_context(M, Hkv, G, D):
+    """More shares than four waves merge at once."""
+    rng = np.random.default_rng(M + D)
+    S = 16384
+    cache = _host_cache(rng, 1, Hkv, S, D)
+    q = torch.from_numpy(rng.standard_normal((1, M, Hkv * G, D))).bfloat16().to(DEV)
+    for at in (S - M, 9000, 4200, 3, -M):
+        _check(kv4.attn_decode4(q, _dev(cache), _i32([at])), q, cache, [at])
+
+
+def test_one_share_for_two_sequences():
+    """So many kv heads and rows that a workgroup has both sequences, one after the other."""
+    rng = np.random.default_rng(20)
+    Hkv, M, D = 256, 33, 64
+    cache = _host_cache(rng, 8, Hkv, 64, D)
+    pages = np.full((2, 160), -1, np.int32)            # 10240 positions
+    pages[0, :3], pages[1, :4] = (5, 1, 7), (0, 2, 3, 6)
+    q = torch.from_numpy(rng.standard_normal((2, M, Hkv, D))).bfloat16().to(DEV)
+    for dpos in ([150, 200], [-M, 200], [120, -M], [-10, -M]):
+        _check(kv4.attn_decode4(q, _dev(cache), _i32(dpos), _i32(pages)), q, cache, dpos, pages)
+
+
+def test_views_of_q():
+    """Slices of a projection, at strides and addresses that loads of 16 bytes take and that they do not."""
+    rng = np.random.default_rng(21)
+    Hkv, D = 2, 128
+    cache = _host_cache(rng, 3, Hkv, 256, D)
+    dev, dp = _dev(cache), _i32([200, 17, 100])
+    for M, G, dt in ((1, 4, torch.bfloat16), (3, 4, torch.float16), (7, 5, torch.bfloat16)):
+        Hq = Hkv * G
+        for off, extra in ((0, 2 * Hkv * D), (8, 64), (3, 5), (0, 4)):
+            proj = torch.from_numpy(rng.standard_normal((3, M, Hq * D + extra + off))).to(dt).to(DEV)
+            q = proj[..., off:off + Hq * D].unflatten(-1, (Hq, D))
+            for o, w in zip((kv4.attn_decode4(q, dev, dp), *kv4.attn_decode4_mx(q, dev, dp)),
+                            (kv4.attn_decode4(q.contiguous(), dev, dp), *kv4.attn_decode4_mx(q.contiguous(), dev, dp))):
+                assert torch.equal(o, w)
+        q = torch.from_numpy(rng.standard_normal((M, 3, Hq, D))).to(dt).to(DEV).transpose(0, 1)      # tokens before sequences
+        assert torch.equal(kv4.attn_decode4(q, dev, dp), kv4.attn_decode4(q.contiguous(), dev, dp))
+        q = torch.from_numpy(rng.standard_normal((1, 1, Hq, D))).to(dt).to(DEV).expand(3, M, Hq, D)
+        assert torch.equal(kv4.attn_decode4(q, dev, dp), kv4.attn_decode4(q.contiguous(), dev, dp))
+
+
+@pytest.mark.parametrize("M", [2, 9])
+def test_both_outputs_of_one_call(M):
+    """o and oq, os together are what each is alone (o in fp32; bf16 its rounding), and rows behind them stay."""
+    lib, rng = _lib.load(), np.random.default_rng(22)
+    B, Hkv, G, D, S = 2, 1, 4, 128, 1024
+    cache = _dev(_host_cache(rng, B, Hkv, S, D))
+    dp, q = _i32([1000, 411]), torch.from_numpy(rng.standard_normal((B, M, Hkv * G, D))).bfloat16().to(DEV)
+    n = lib.mxfp4_attn_kv4_workspace_size(B, M, Hkv * G, Hkv, D, S)
+    assert n > 0
+    for code, dt in ((0, torch.bfloat16), (1, torch.float16), (2, torch.float32)):
+        ws = torch.full((n + 64,), 99, dtype=torch.uint8, device=DEV)
+        o = torch.full((B * M + 1, Hkv * G, D), 77.0, dtype=dt, device=DEV)
+        oq, os_ = (torch.full((B * M + 1, Hkv * G * w), 55, dtype=torch.uint8, device=DEV) for w in (D // 2, D // 32))
+        _lib.check(lib.mxfp4_attn_kv4(q.data_ptr(), 0, Hkv * G * D, *[t.data_ptr() for t in cache], None, B, S, 0, dp.data_ptr(),
+                                      o.data_ptr(), code, oq.data_ptr(), os_.data_ptr(), B, M, Hkv * G, Hkv, D, ws.data_ptr(), n,
+                                      torch.cuda.current_stream().cuda_stream), "attn_kv4")
+        wq, wsc = kv4.attn_decode4_mx(q, cache, dp)
+        assert torch.equal(oq[:-1], wq) and torch.equal(os_[:-1], wsc)
+        assert torch.equal(o[:-1].view(B, M, Hkv * G, D), kv4.attn_decode4(q, cache, dp).to(dt))
+        assert (o[-1] == 77).all() and (oq[-1] == 55).all() and (os_[-1] == 55).all() and (ws[n:] == 99).all()
+
+
+@pytest.mark.parametrize("B,M,S", [(1, 9, 8192), (3, 6, 4096), (40, 1, 4096), (40, 1, 512)])
+def test_replays_with_other_positions(B, M, S):
+    """Every path captured once and replayed over other lengths, with eager work between, is the eager result."""
+    rng = np.random.default_rng(23 + B)
+    dev = _dev(_host_cache(rng, B, 1, S, 128))
+    q, dp = torch.randn((B, M, 8, 128), device=DEV).bfloat16(), _i32([5] * B)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        kv4.attn_decode4(q, dev, dp)
+        with torch.cuda.graph(graph, stream=side):
+            o = kv4.attn_decode4(q, dev, dp)
+    torch.cuda.current_stream().wait_stream(side)
+    for hi in (S, 40, S // 2, 1):
+        dp.copy_(_i32(rng.integers(-M, hi, B)))
+        q.normal_()
+        graph.replay()
+        assert torch.equal(o, kv4.attn_decode4(q, dev, dp))
+        assert torch.isfinite(o).all()
+
+
 def test_shared_pages():
     """A prefix that two sequences share."""
     rng = np.random.default_rng(9)
