@@ -431,11 +431,16 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
 }
 
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
-    // 16 waves where a row has more records than four load at once
-    const bool many = p.shares > kFew * a.B && p.most > kFew;
-    const dim3 grid(a.M * a.Hq, a.B), block(many ? 1024 : 256);
-    if (D == 64) hipLaunchKernelGGL((many ? attn_kv4_merge_kernel<64, 16> : attn_kv4_merge_kernel<64, 4>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((many ? attn_kv4_merge_kernel<128, 16> : attn_kv4_merge_kernel<128, 4>), grid, block, 0, st, a);
+    // about as many waves as load a row's records at once.  4 / 8 / 16, us: nine tokens over 23001 positions (42 shares)
+    // 23.4 / 23.4 / 25.2; one token over 16000, 16 heads (64 shares) 15.8 / 15.3 / 16.3
+    const int nw = p.shares <= kFew * a.B || p.most <= kFew ? 4 : p.most <= 2 * kFew ? 8 : 16;
+    const dim3 grid(a.M * a.Hq, a.B), block(64 * nw);
+#define MXH_M4(DD)                                                                               \
+    if (nw == 4) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 4>), grid, block, 0, st, a);      \
+    else if (nw == 8) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 8>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 16>), grid, block, 0, st, a)
+    if (D == 64) { MXH_M4(64); } else { MXH_M4(128); }
+#undef MXH_M4
     return mxh::launch_status("attn_kv4 (merge)");
 }
 
