@@ -91,7 +91,8 @@ struct Args {
     int64_t ldq;                 // elements between tokens of q
     Cache c;
     const int32_t* dpos;
-    float* part;
+    int4* places;                // of a sequence, for the merge: its first share, where in that, places a share
+    float* part;                 // records
     Out out;
     int B, M, Hq, G, shares, records;   // shares of the batch, and records a row may have (its stride)
     float scale;                 // log2(e) / sqrt(D)
@@ -134,18 +135,9 @@ struct Place {
     int b, base;        // a sequence, its dpos, and where it starts
     uint64_t start;
 };
-__device__ __forceinline__ uint32_t pad_of(const Args& a) { return a.B == 1 ? 0u : kPad; }
-// The sequence with place at * p.per (B > 1; false: that is past the line), or for at < 0
-// sequence p.b.
-__device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
+// Share blockIdx.x's first sequence; false: it is past the line.
+__device__ __forceinline__ bool find_share(const Args& a, Place& p) {
     const int lane = threadIdx.x & 63;
-    p.start = 0;
-    if (a.B == 1) {
-        p.b = 0;
-        p.base = __builtin_amdgcn_readfirstlane(a.dpos[0]);
-        p.per = share_units(units_of(a, p.base), a);
-        return true;
-    }
     auto places = [&](int b0, int& base) {
         base = 0;
         if (b0 + lane >= a.B) return 0u;
@@ -161,16 +153,27 @@ __device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
         total += last_lane(wave_scan(places(b0, t)));
     }
     p.per = share_units(total, a);
-    const uint64_t target = (uint64_t)at * p.per;
-    if (at >= 0 && target >= total) return false;
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 64) {
+        // The last share, the least full, leaves the places for the merge, which would have to find them again (us with
+        // that / without: 48 sequences of up to 8192 positions 28.9 / 27.9, 200 of 8000 108 / 99)
+        uint64_t start = kPad;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            int t;
+            const uint32_t n = b0 ? places(b0, t) : n0, to = b0 ? wave_scan(n) : to0;
+            const uint64_t at = start + to - n;
+            const uint64_t share = total >> 32 ? at / p.per : (uint32_t)at / p.per;
+            if (b0 + lane < a.B) a.places[b0 + lane] = make_int4((int)share, (int)(at - share * p.per), (int)p.per, 0);
+            start += last_lane(to);
+        }
+    }
+    const uint64_t target = (uint64_t)blockIdx.x * p.per;
+    if (target >= total) return false;
+    p.start = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const uint32_t n = b0 ? places(b0, base) : n0, to = b0 ? wave_scan(n) : to0;
-        int l = p.b - b0;
-        if (at >= 0) {
-            const uint64_t past = __ballot(p.start + to > target);
-            l = past ? (int)__builtin_ctzll(past) : 64;
-        }
-        if (l < 64) {
+        const uint64_t past = __ballot(p.start + to > target);
+        if (past) {
+            const int l = (int)__builtin_ctzll(past);
             p.b = b0 + l;
             p.base = __builtin_amdgcn_readlane(base, l);
             p.start += (uint32_t)__builtin_amdgcn_readlane((int)(to - n), l);
@@ -180,10 +183,7 @@ __device__ __forceinline__ bool find_share(const Args& a, int at, Place& p) {
     }
     return false;
 }
-// The share with place `at` of the line.
-__device__ __forceinline__ int share_of(uint64_t at, uint32_t per) {
-    return (int)(at >> 32 ? at / per : (uint32_t)at / per);
-}
+
 // What a workgroup (blockIdx.x) works on.
 enum class Work {
     kSequence,   // a whole sequence
@@ -201,13 +201,14 @@ __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
         const int base = __builtin_amdgcn_readfirstlane(a.dpos[0]);
         const uint32_t n = units_of(a, base), per = share_units(n, a);
         const uint64_t u0 = (uint64_t)blockIdx.x * per;
+        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.places[0] = make_int4(0, 0, (int)per, 0);
         if (u0 < n) segment(0, base, (int)u0, (int)min((uint64_t)n, u0 + per));
         return;
     }
     Place p;
-    if (!find_share(a, blockIdx.x, p)) return;             // uniform
+    if (!find_share(a, p)) return;             // uniform
     const uint64_t from = (uint64_t)blockIdx.x * p.per;
-    const int pad = (int)pad_of(a);
+    constexpr int pad = kPad;
     for (bool first = true;;) {
         const int n = (int)units_of(a, p.base);
         // the share's end and beginning, in units of the sequence (per < 2^28, and a line that is behind `from` ends past it)

@@ -26,7 +26,7 @@
 // it moves to the maximum only where a lane's terms sum past kMost.
 //
 // What bounds it.  A long batch: memory.  32 sequences of up to 32768 positions (267 MB,
-// four heads of 128, eight query heads each) 59.9 us, of which 5 the merge, 4.9 TB/s in
+// four heads of 128, eight query heads each) 58.8 us, of which 4 the merge, 4.9 TB/s in
 // the shares' kernel; the same loads with nothing done to them 58.4 before the shares
 // were equal, a plain streaming read 6.1 TB/s.  Eight sequences of 65536: 113 us, 5.05
 // TB/s in all.  For that: 128 registers, so four waves a SIMD, each with a unit's loads
@@ -325,17 +325,13 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = a.M * a.G;
-    Place p;
-    p.b = blockIdx.y;
-    find_share(a, -1, p);
-    const int g = blockIdx.x / rows, r = blockIdx.x - g * rows;
-    const int64_t pos = (int64_t)p.base + r / a.G;
+    const int b = blockIdx.y, g = blockIdx.x / rows, r = blockIdx.x - g * rows;
+    const int4 p = a.places[b];
+    const int64_t pos = (int64_t)a.dpos[b] + r / a.G;
     // its records: those of the shares with its sequence's units 0 .. pos / kUnit
-    p.start += pad_of(a);
-    const int s0 = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(share_of(p.start, p.per));
     const int ns = __builtin_amdgcn_readfirstlane(
-        pos < 0 || pos >= a.c.max_pos ? 0 : share_of(p.start + (uint64_t)(pos / kUnit), p.per) - s0 + 1);
-    const float* rec = a.part + ((int64_t)blockIdx.x * a.records + s0 + p.b) * (D + 4);
+        pos < 0 || pos >= a.c.max_pos ? 0 : min((int)(((uint32_t)p.y + (uint32_t)(pos / kUnit)) / (uint32_t)p.z) + 1, a.shares - p.x));
+    const float* rec = a.part + ((int64_t)blockIdx.x * a.records + __builtin_amdgcn_readfirstlane(p.x) + b) * (D + 4);
     float m = kNone, l = 0.0f;
     cvec o = 0.0f;
     for (int i0 = wave; i0 < ns; i0 += N * NW) {
@@ -387,7 +383,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     const float inv = 1.0f / den;
 #pragma unroll
     for (int c = 0; c < CT; ++c) x[c] = none ? 0.0f : x[c] * inv;
-    store<CT>(a.out, ((int64_t)p.b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, CT * tid, x);
+    store<CT>(a.out, ((int64_t)b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, CT * tid, x);
 }
 
 struct Plan {
@@ -449,7 +445,7 @@ int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
 extern "C" size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos) {
     if (B <= 0 || M <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || max_pos <= 0) return 0;
     const Plan p = plan(B, M, Hq, Hkv, max_pos);
-    return p.one ? 0 : (size_t)p.records * M * Hq * (D + 4) * sizeof(float);
+    return p.one ? 0 : (size_t)B * sizeof(int4) + (size_t)p.records * M * Hq * (D + 4) * sizeof(float);
 }
 
 extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,
@@ -479,7 +475,8 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     a.q = static_cast<const uint16_t*>(q);
     a.ldq = ldq;
     a.dpos = dpos;
-    a.part = static_cast<float*>(workspace);
+    a.places = static_cast<int4*>(workspace);
+    a.part = reinterpret_cast<float*>(a.places + B);
     a.out = Out{o, o_dtype, oq, os};
     a.B = B;
     a.M = M;
