@@ -46,13 +46,13 @@ __device__ __forceinline__ float over_lh(float v) {
     return MAX ? fmaxf(x, y) : x + y;
 }
 
-// A wave's V codes and scale words, of two units in turn.  Row 8 h + 4 lh + i of a tile
+// A wave's V nibbles and the scales, of two units in turn.  Row 8 h + 4 lh + i of a tile
 // lies at 8 h + 2 i + lh, so that the two rows that a product's halves read at a time
 // are neighbours.
 template <int D>
 struct Stage {
     alignas(16) uint8_t v[2][2][16][D / 2];
-    alignas(16) uint32_t codes[2][64];        // K's of the unit's 32 positions, then V's
+    alignas(16) float scale[2][64][D / 32];   // K's of the unit's 32 positions, then V's (scale_at: a lane reads a position's as it is used)
 };
 
 template <int D, int NQ, int NP, Work W>
@@ -145,7 +145,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
                 if (!(u.there >> (l32 >> 4) & 1) || l32 > sees) rcodes = 0x7F7F7F7Fu;
             }
-            stage.codes[j & 1][lane] = rcodes;
+            typedef float svec __attribute__((ext_vector_type(D / 32)));
+            svec x;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) x[i] = scale_at(rcodes, i);
+            *reinterpret_cast<svec*>(stage.scale[j & 1][lane]) = x;
         };
         auto put_v = [&](int j, const Unit& u) {
             if (ragged(u)) {
@@ -193,10 +197,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             mx::v16f sv;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sv[i] = zero;
-            const uint32_t w = stage.codes[j & 1][l32];
+            float sc[KT / 4];
+#pragma unroll
+            for (int i = 0; i < KT / 4; ++i) sc[i] = stage.scale[j & 1][l32][KT / 4 * lh + i];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const uint4 kd = kv4::eight_bf16(rk[kt / 4][kt & 3], scale_at(w, D == 128 ? 2 * lh + (kt >> 2) : lh));
+                const uint4 kd = kv4::eight_bf16(rk[kt / 4][kt & 3], sc[kt >> 2]);
 #pragma unroll
                 for (int k = 0; k < NQ; ++k)
                     sv = mfma32(kd, *reinterpret_cast<const uint4*>(&lds.in.qs[k * R + l32][(D / 2) * lh + 8 * kt]), sv);
@@ -221,14 +227,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 float sc[8];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(&stage.codes[j & 1][32 + 16 * st + 8 * h + 4 * lh]);
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint8_t* x = &stage.v[j & 1][st][8 * h + 2 * i + lh][l32 * (CT / 2)];
                         if constexpr (D == 128) v[4 * h + i] = *reinterpret_cast<const uint16_t*>(x);
                         else v[4 * h + i] = *x;
-                        sc[4 * h + i] = scale_at(w[i], D == 128 ? l32 >> 3 : l32 >> 4);
+                        sc[4 * h + i] = stage.scale[j & 1][32 + 16 * st + 8 * h + 4 * lh + i][D == 128 ? l32 >> 3 : l32 >> 4];
                     }
                 }
                 uint32_t o[CT][4];
