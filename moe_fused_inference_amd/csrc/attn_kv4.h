@@ -94,6 +94,7 @@ struct Args {
     int4* places;                // of a sequence, for the merge: its first share, where in that, places a share
     float* part;                 // records
     Out out;
+    int per;                     // units of a share of one sequence, or 0: as share_units finds from its length
     int B, M, Hq, G, shares, records;   // shares of the batch, and records a row may have (its stride)
     float scale;                 // log2(e) / sqrt(D)
 };
@@ -198,11 +199,12 @@ __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
         return;
     }
     if constexpr (W == Work::kShare) {      // (a kernel of its own: nine tokens over 23001 positions 25.1 us, in the loop 25.8)
-        const int base = __builtin_amdgcn_readfirstlane(a.dpos[0]);
-        const uint32_t n = units_of(a, base), per = share_units(n, a);
-        const uint64_t u0 = (uint64_t)blockIdx.x * per;
+        const int base = a.dpos[0];         // (in flight, where nothing here needs it)
+        uint32_t per = a.per;
+        if (per == 0) per = share_units(units_of(a, __builtin_amdgcn_readfirstlane(base)), a);
         if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.places[0] = make_int4(0, 0, (int)per, 0);
-        if (u0 < n) segment(0, base, (int)u0, (int)min((uint64_t)n, u0 + per));
+        const uint32_t u0 = blockIdx.x * per;
+        segment(0, base, (int)u0, (int)(u0 + per));
         return;
     }
     Place p;

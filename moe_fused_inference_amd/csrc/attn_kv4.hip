@@ -143,11 +143,6 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         const int lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int l16 = lane & 15, lq = lane >> 4;
-        // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
-        auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
-        const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
-        const int lim_min = clamped(base);                            // the first token sees up to here
-        u1 = min(u1, (last + kUnit) / kUnit);
         // q, whose parts go to LDS once the first units' loads are on their way
         const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
         constexpr int NT = 64 * NW, QN = (R * (D / 8) + NT - 1) / NT;
@@ -182,12 +177,24 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         };
         Raw<D> r;
         int there = 0;
-        if (u0 + wave < u1) {
+        auto first_loads = [&]() {
             uint32_t row[2];
             find_rows(0);
             there = locate(0, row);
             load_k(r, a.c, row, off);
             load_v(r, a.c, row, off);
+        };
+        if constexpr (W == Work::kShare) first_loads();        // of a share of fixed length before dpos is there: what no token sees is masked
+        base = __builtin_amdgcn_readfirstlane(base);
+        // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
+        auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
+        const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
+        const int lim_min = clamped(base);                            // the first token sees up to here
+        u1 = min(u1, (last + kUnit) / kUnit);
+        if constexpr (W == Work::kShare) {
+            if (u0 >= u1) return;                               // no record: the merge reads none
+        } else {
+            if (u0 + wave < u1) first_loads();
         }
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
@@ -484,6 +491,7 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     a.G = Hq / Hkv;
     a.shares = p.shares;
     a.records = p.records;
+    a.per = B == 1 && (int64_t)p.shares * kMinShare * kUnit >= a.c.max_pos ? kMinShare : 0;
     a.scale = (float)(1.4426950408889634 / sqrt((double)D));
     const hipStream_t st = mxh::as_stream(stream);
     if (p.many) {

@@ -75,6 +75,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
     auto segment = [&](int b, int base, int u0, int u1) {
         int tid = threadIdx.x;
         if constexpr (W == Work::kLine) asm volatile("" : "+v"(tid));   // (a lane's constants are made again for each segment, not held)
+        base = __builtin_amdgcn_readfirstlane(base);
         const int lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int l32 = lane & 31, lh = lane >> 5;
