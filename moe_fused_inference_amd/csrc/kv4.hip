@@ -60,21 +60,24 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const void* __restrict__
 // Eight values of one nibble word as DST, 16 (32) bytes at p.
 template <int DST>
 __device__ __forceinline__ void store8(void* p, int64_t at, uint32_t w, float s) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef float f4 __attribute__((ext_vector_type(4)));
     if constexpr (DST == MXFP4_DT_BF16) {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = kv4::eight_bf16(w, s);
+        const uint4 e = kv4::eight_bf16(w, s);
+        __builtin_nontemporal_store((u4{e.x, e.y, e.z, e.w}), reinterpret_cast<u4*>(static_cast<uint16_t*>(p) + at));
     } else {
-        typedef float f2 __attribute__((ext_vector_type(2)));
         const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
         const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
         if constexpr (DST == MXFP4_DT_F32) {
             float* o = static_cast<float*>(p) + at;
-            *reinterpret_cast<float4*>(o) = make_float4(a[0], a[1], b[0], b[1]);
-            *reinterpret_cast<float4*>(o + 4) = make_float4(d[0], d[1], e[0], e[1]);
+            __builtin_nontemporal_store((f4{a[0], a[1], b[0], b[1]}), reinterpret_cast<f4*>(o));
+            __builtin_nontemporal_store((f4{d[0], d[1], e[0], e[1]}), reinterpret_cast<f4*>(o + 4));
         } else {
             typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-            *reinterpret_cast<h8*>(static_cast<_Float16*>(p) + at) =
-                h8{(_Float16)a[0], (_Float16)a[1], (_Float16)b[0], (_Float16)b[1],
-                   (_Float16)d[0], (_Float16)d[1], (_Float16)e[0], (_Float16)e[1]};
+            __builtin_nontemporal_store((h8{(_Float16)a[0], (_Float16)a[1], (_Float16)b[0], (_Float16)b[1], (_Float16)d[0],
+                                            (_Float16)d[1], (_Float16)e[0], (_Float16)e[1]}),
+                                        reinterpret_cast<h8*>(static_cast<_Float16*>(p) + at));
         }
     }
 }
