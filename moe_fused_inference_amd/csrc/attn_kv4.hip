@@ -26,13 +26,13 @@
 // it moves to the maximum only where a lane's terms sum past kMost.
 //
 // What bounds it.  A long batch: memory.  32 sequences of up to 32768 positions (267 MB,
-// four heads of 128, eight query heads each) 58.8 us, of which 4 the merge, 4.9 TB/s in
-// the shares' kernel; the same loads with nothing done to them 58.4 before the shares
-// were equal, a plain streaming read 6.1 TB/s.  Eight sequences of 65536: 113 us, 5.05
-// TB/s in all.  For that: 128 registers, so four waves a SIMD, each with a unit's loads
+// four heads of 128, eight query heads each) 55.8 us, of which 4 the merge, 5.2 TB/s in
+// the shares' kernel; a plain streaming read 6.1 TB/s.  Eight sequences of 65536: 107 us,
+// 5.35 TB/s in all.  For that: 128 registers, so four waves a SIMD, each with a unit's loads
 // ahead (4.3 KB; 69 KB a CU).  Two ahead by buffer descriptors 74 us, V through LDS 68.
 // A short call: two launches, each one dependent chain of memory latencies (dpos, page,
-// rows; records): 500 positions 5.0 + 3.3 us, 32000 9.0 + 5.0.
+// rows; records): 500 positions 4.4 + 3.2 us, 32000 8.6 + 4.7 (5.0 + 3.3 and 9.0 + 5.0
+// before a share of one sequence loaded its first unit ahead of dpos).
 #include "attn_kv4.h"
 #include "kv4.h"
 #include "mx_device.h"
@@ -46,6 +46,10 @@ namespace {
 using namespace mxa;
 
 constexpr int kParts = 3;              // bf16 parts of a probability
+// A cache of more bytes, half the chip's last one, is not there any more when the next call comes: K by streaming loads.
+// Plain / so, us: 32 sequences of up to 32768 positions (571 MB) 59.0 / 55.9, 48 of 8192 (214 MB) 27.9 / 27.2; but 64
+// of 2000 (71 MB, read again and again) 18.1 / 18.7.  V too: 48 sequences 29.0 (its loads take half lines).
+constexpr int64_t kMuch = 128ll << 20;
 
 // A unit's bytes as a lane loads them.  K: row 16 t + l16, D/8 bytes from D/8 lq on
 // (so its dimensions are D/4 lq .., one block's or half a block's) and their code.
@@ -72,12 +76,13 @@ struct Lane {
     }
 };
 
-// row[t]: tile t's first head row (uniform).
-template <int D>
+// row[t]: tile t's first head row (uniform).  STREAM: K does not stay in the caches, and so leaves them to what does (kMuch).
+template <bool STREAM, int D>
 __device__ __forceinline__ void load_k(Raw<D>& r, const Cache& c, const uint32_t (&row)[2], const Lane<D>& o) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        r.k[t] = *reinterpret_cast<const typename Raw<D>::vec*>(c.kq + (uint64_t)row[t] * (D / 2) + o.k);
+        const auto p = reinterpret_cast<const typename Raw<D>::vec*>(c.kq + (uint64_t)row[t] * (D / 2) + o.k);
+        r.k[t] = STREAM ? __builtin_nontemporal_load(p) : *p;
         r.ks[t] = *(c.ks + (uint64_t)row[t] * (D / 32) + o.ks);
     }
 }
@@ -124,7 +129,7 @@ __device__ __forceinline__ void decode_v(const uint32_t (&v)[8], const float (&s
     for (int c = 0; c < 4; ++c) vd[c] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
 }
 
-template <int D, int NQ, Work W, int NW>
+template <int D, int NQ, Work W, int NW, bool STREAM>
 __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
     constexpr bool ONE = W == Work::kSequence;
     constexpr int R = 16, KT = D / 32, CT = D / 16;
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
             uint32_t row[2];
             find_rows(0);
             there = locate(0, row);
-            load_k(r, a.c, row, off);
+            load_k<STREAM>(r, a.c, row, off);
             load_v(r, a.c, row, off);
         };
         if constexpr (W == Work::kShare) first_loads();        // of a share of fixed length before dpos is there: what no token sees is masked
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                     for (int n = 0; n < NQ; ++n) sv[t] = mfma_bf16(kd, qf[n], sv[t]);
                 }
             }
-            if constexpr (more) load_k(r, a.c, next, off);
+            if constexpr (more) load_k<STREAM>(r, a.c, next, off);
             // sv[t][i], s[4 t + i]: position p0 + 16 t + 4 lq + i
             float s[8];
 #pragma unroll
@@ -500,17 +505,22 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
         return merge(a, p, D, st);
     }
     const dim3 grid(p.shares, Hkv);
-#define MXH_K4(DD, QQ)                                                                                                \
-    if (p.waves == 16) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 16>), grid, dim3(1024), 0, st, a); \
-    else if (p.one) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 4>), grid, dim3(256), 0, st, a);      \
-    else if (B == 1) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kShare, 4>), grid, dim3(256), 0, st, a);        \
-    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kLine, 4>), grid, dim3(256), 0, st, a)
+    const bool much = std::min((int64_t)B * a.c.max_pos, (int64_t)n_pages * page) * Hkv * (D + D / 16) > kMuch;
+#define MXH_W4(DD, QQ, W)                                                                                          \
+    if (much) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, true>), grid, dim3(256), 0, st, a);          \
+    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, false>), grid, dim3(256), 0, st, a)
+#define MXH_K4(DD, QQ)                                                                                                        \
+    if (p.waves == 16) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 16, false>), grid, dim3(1024), 0, st, a); \
+    else if (p.one) { MXH_W4(DD, QQ, kSequence); }                                                                            \
+    else if (B == 1) { MXH_W4(DD, QQ, kShare); }                                                                              \
+    else { MXH_W4(DD, QQ, kLine); }
     if (D == 64) {
         if (q_dtype == MXFP4_DT_BF16) { MXH_K4(64, 1); } else { MXH_K4(64, 2); }
     } else {
         if (q_dtype == MXFP4_DT_BF16) { MXH_K4(128, 1); } else { MXH_K4(128, 2); }
     }
 #undef MXH_K4
+#undef MXH_W4
     const int rl = mxh::launch_status("attn_kv4 (shares)");
     if (rl != MXFP4_OK || p.one) return rl;
     return merge(a, p, D, st);
