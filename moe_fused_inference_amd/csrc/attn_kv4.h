@@ -213,7 +213,7 @@ __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
     constexpr int pad = kPad;
     for (bool first = true;;) {
         const int n = (int)units_of(a, p.base);
-        // the share's end and beginning, in units of the sequence (per < 2^28, and a line that is behind `from` ends past it)
+        // the share's beginning and end in units of the sequence, which ends past `from` (per < 2^28)
         const int u1 = (int)min((int64_t)n, (int64_t)(from + p.per - p.start) - pad);
         const int u0 = (int)max((int64_t)0, (int64_t)from - (int64_t)p.start - pad);
         if (u0 < u1) {

@@ -1,13 +1,13 @@
 // attn_kv4.hip -- attention over the MXFP4 KV cache (kv4.h): M tokens of each of
 // B sequences, token m of sequence b at dpos[b] + m over positions 0 .. dpos[b] + m.
 //
-//   attn_kv4_kernel        workgroup (share of a sequence, kv head g), up to 16 query
+//   attn_kv4_kernel        workgroup (share of the batch, kv head g), up to 16 query
 //                          rows (tokens x heads of the kv head): a wave takes every
 //                          fourth unit of 32 of the share's positions, with its own
 //                          running softmax; the waves' sums meet in LDS -> one record
 //                          (reference, sum, D column sums) per row, share and
-//                          sequence in it, or
-//                          the output where a sequence has one share.
+//                          sequence in it, or the output where a workgroup has a
+//                          whole sequence.
 //   attn_kv4_rows_kernel   the same for more rows (attn_kv4_rows.hip).
 //   attn_kv4_merge_kernel  workgroup (kv head's row, sequence): the row's records
 //                          -> its output.

@@ -166,8 +166,8 @@ class DecodeStep:
     ``kv4``; max_pos a multiple of 16).  The MXFP4 cache's attention
     runs in launches of its own: attn_front and attn_next, which put the FP8
     cache's into the MoE launch, do not apply.  us a layer (32 / 4 heads, hidden
-    2048, 1/8 of the head with it; FP8 / MXFP4): one token, 4000 positions 38.5 /
-    44.1, 32000 57.7 / 48.9; four tokens 62.9 / 66.8, 80.1 / 74.8."""
+    2048, 1/8 of the head with it; FP8 / MXFP4): one token, 4000 positions 38.6 /
+    43.4, 32000 57.7 / 47.2; four tokens 62.8 / 66.1, 80.3 / 74.1."""
 
     def __init__(self, model, cfg, M=1, max_pos=4096, device="cuda", fused_router=True, qkv_tail=True,
                  attn_front=True, attn_next=True, kv="fp8"):
