@@ -284,7 +284,6 @@ int as_int(int64_t v, const char* msg) {
 
 Kv4 kv4_cache(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq, const torch::Tensor& vs,
               const c10::optional<torch::Tensor>& pages, const c10::optional<torch::Tensor>& at, const char* at_msg) {
-    require(kq.is_cuda() && ks.is_cuda() && vq.is_cuda() && vs.is_cuda(), "cache tensors must be cuda");
     require(kq.scalar_type() == torch::kUInt8 && ks.scalar_type() == torch::kUInt8 && vq.scalar_type() == torch::kUInt8 &&
                 vs.scalar_type() == torch::kUInt8,
             "cache tensors must be uint8");
@@ -308,11 +307,14 @@ Kv4 kv4_cache(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Ten
         c.pages = static_cast<const int32_t*>(pages->data_ptr());
         c.B = as_int(pages->size(0), "too many sequences");
         c.max_pages = as_int(pages->size(1), "too many pages");
+        // a table of no columns has no address, which would stand for no table
+        require(c.max_pages > 0, "pages must have a column at least");
     }
     if (at.has_value()) {
         require(at->scalar_type() == torch::kInt32 && at->is_contiguous() && at->device() == dev && at->numel() == c.B, at_msg);
         c.at = static_cast<const int32_t*>(at->data_ptr());
     }
+    require(kq.is_cuda(), "cache tensors must be cuda");
     return c;
 }
 

@@ -540,3 +540,16 @@ def test_refusals_of_tensors():
         kv4.kv4_read(cache, 4, dtype=torch.uint8)
     with pytest.raises(RuntimeError):
         kv4.kv4_read(cache, 4, start=dp[:1])
+
+
+def test_a_table_of_no_columns():
+    """Refused, with the pool as it was: its pages are someone's."""
+    cache, before = (_dev(_host_cache(np.random.default_rng(30), 3, 2, 32, 64)) for _ in range(2))
+    x, q = torch.ones((2, 1, 2, 64), device=DEV), torch.ones((2, 1, 4, 64), device=DEV).bfloat16()
+    tab = _i32([[0, 1], [2, 0]])[:, :0]
+    for t in (tab, tab.contiguous(), torch.empty((2, 0), dtype=torch.int32, device=DEV)):
+        for call in (lambda: kv4.kv4_write(x, x, cache, _i32([0, 0]), t), lambda: kv4.kv4_read(cache, 1, pages=t),
+                     lambda: kv4.attn_decode4(q, cache, _i32([0, 0]), t), lambda: kv4.attn_decode4_mx(q, cache, _i32([0, 0]), t)):
+            with pytest.raises(RuntimeError):
+                call()
+    assert all(torch.equal(a, b) for a, b in zip(cache, before))

@@ -124,3 +124,23 @@ def test_binding_refuses_cpu_tensors_and_bad_allocations():
 @pytest.mark.parametrize("call", [_write, _read, _attn, _rope])
 def test_more_head_rows_than_32_bits(call):
     _refused(call(_cache(n_pages=1 << 15, page=1 << 15)), "head rows")      # times four heads: 2^32
+
+
+def _on_cpu(Hkv=4, D=128, n_pages=2, pages=None):
+    """Every entry of the binding on CPU tensors: (name, call).  What is refused by its shape is refused before
+    the device is looked at."""
+    cache = [torch.zeros((n_pages, Hkv, 32, w), dtype=torch.uint8) for w in (D // 2, D // 32) * 2]
+    d = torch.zeros(n_pages if pages is None else pages.shape[0], dtype=torch.int32)
+    x = torch.zeros((d.numel(), 1, Hkv, D), dtype=torch.bfloat16)
+    q = torch.zeros((d.numel(), 1, 8, D), dtype=torch.bfloat16)
+    return [("write", lambda: kv4.kv4_write(x, x, cache, d, pages)), ("read", lambda: kv4.kv4_read(cache, 4, d, pages)),
+            ("attn", lambda: kv4.attn_decode4(q, cache, d, pages)), ("attn_mx", lambda: kv4.attn_decode4_mx(q, cache, d, pages))]
+
+
+@pytest.mark.parametrize("pages", [torch.zeros((2, 0), dtype=torch.int32), torch.zeros((2, 3), dtype=torch.int32)[:, :0].contiguous(),
+                                   torch.zeros((0, 0), dtype=torch.int32)])
+def test_binding_refuses_a_table_of_no_columns(pages):
+    """It has no address, and no address means that sequence b is page b."""
+    for _, call in _on_cpu(pages=pages):
+        with pytest.raises(RuntimeError, match="a column at least"):
+            call()
