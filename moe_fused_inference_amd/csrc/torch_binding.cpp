@@ -298,6 +298,7 @@ Kv4 kv4_cache(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Ten
     Kv4 c{u8m(kq), u8m(ks), u8m(vq), u8m(vs), nullptr, nullptr, 0, 0, 0, 0, 0, 0};
     c.n_pages = as_int(kq.size(0), "too many pages");
     c.Hkv = as_int(kq.size(1), "too many heads");
+    require(c.Hkv > 0, "a cache needs a kv head at least");     // (query heads are divided by it)
     c.page = as_int(kq.size(2), "page too long");
     c.D = as_int(kq.size(3) * 2, "head_dim too large");
     c.B = c.n_pages;

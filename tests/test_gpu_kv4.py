@@ -553,3 +553,12 @@ def test_a_table_of_no_columns():
             with pytest.raises(RuntimeError):
                 call()
     assert all(torch.equal(a, b) for a, b in zip(cache, before))
+
+
+def test_a_cache_of_no_heads():
+    cache = kv4.KV4(*(torch.empty((2, 0, 32, w), dtype=torch.uint8, device=DEV) for w in (32, 2, 32, 2)))
+    x, q, dp = torch.empty((2, 1, 0, 64), device=DEV), torch.ones((2, 1, 4, 64), device=DEV).bfloat16(), _i32([0, 0])
+    for call in (lambda: kv4.kv4_write(x, x, cache, dp), lambda: kv4.kv4_read(cache, 1), lambda: kv4.attn_decode4(q, cache, dp),
+                 lambda: kv4.attn_decode4_mx(q, cache, dp)):
+        with pytest.raises(RuntimeError, match="a kv head at least"):
+            call()

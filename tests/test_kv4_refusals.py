@@ -144,3 +144,10 @@ def test_binding_refuses_a_table_of_no_columns(pages):
     for _, call in _on_cpu(pages=pages):
         with pytest.raises(RuntimeError, match="a column at least"):
             call()
+
+
+def test_binding_refuses_a_cache_of_no_heads():
+    """The query heads would be divided by none, which ends the process."""
+    for _, call in _on_cpu(Hkv=0):
+        with pytest.raises(RuntimeError, match="a kv head at least"):
+            call()
