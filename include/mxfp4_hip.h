@@ -276,6 +276,7 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  *   workspace  16-byte aligned, mxfp4_attn_kv4_workspace_size(B, M, Hq, Hkv, D,
  *              max_pos) bytes (0: may be NULL); nothing persists, but calls that
  *              share one must be stream-ordered
+ * M and Hq up to 65535, M * Hq / Hkv up to 1048560; the size of a call that is refused is 0.
  * Sums and softmax in fp32.  The products are bf16 with every operand exact: q in
  * one part (fp16: two), a probability in three, or in two (16 bits, 2^-17 of it)
  * where more than 16 rows (M * Hq / Hkv) go to bf16 or fp16 alone.  A token outside

@@ -438,6 +438,16 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
     return p;
 }
 
+// The sizes that the entry takes (plan's integers are good for these).
+constexpr int64_t kMostRows = 65535 * 16;    // of a kv head: M * Hq / Hkv
+bool takes_heads(int M, int Hq, int Hkv) {
+    return M > 0 && M <= 65535 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 65535;
+}
+bool takes(int B, int M, int Hq, int Hkv, int D, int max_pos) {
+    return B > 0 && B <= 65535 && takes_heads(M, Hq, Hkv) && (int64_t)M * (Hq / Hkv) <= kMostRows && (D == 64 || D == 128) &&
+           max_pos > 0 && max_pos <= kv4::kMaxPos;
+}
+
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
     // about as many waves as load a row's records at once.  4 / 8 / 16, us: nine tokens over 23001 positions (42 shares)
     // 23.4 / 23.4 / 25.2; one token over 16000, 16 heads (64 shares) 15.8 / 15.3 / 16.3
@@ -455,7 +465,7 @@ int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
 }  // namespace
 
 extern "C" size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos) {
-    if (B <= 0 || M <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || max_pos <= 0) return 0;
+    if (!takes(B, M, Hq, Hkv, D, max_pos)) return 0;
     const Plan p = plan(B, M, Hq, Hkv, max_pos);
     return p.one ? 0 : (size_t)B * sizeof(int4) + (size_t)p.records * M * Hq * (D + 4) * sizeof(float);
 }
@@ -469,8 +479,9 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     if (rc != MXFP4_OK) return rc;
     MXH_REQUIRE(q && dpos, "attn_kv4: null pointer");
     MXH_REQUIRE(q_dtype == MXFP4_DT_BF16 || q_dtype == MXFP4_DT_F16, "attn_kv4: q dtype %d (bf16 or fp16)", q_dtype);
-    MXH_REQUIRE(M > 0 && M <= 65535 && Hq > 0 && Hq % Hkv == 0 && Hq <= 65535, "attn_kv4: M=%d Hq=%d Hkv=%d", M, Hq, Hkv);
-    MXH_REQUIRE((int64_t)M * (Hq / Hkv) <= 65535 * 16, "attn_kv4: M*Hq/Hkv=%lld (up to %d)", (long long)M * (Hq / Hkv), 65535 * 16);
+    MXH_REQUIRE(takes_heads(M, Hq, Hkv), "attn_kv4: M=%d Hq=%d Hkv=%d", M, Hq, Hkv);
+    MXH_REQUIRE((int64_t)M * (Hq / Hkv) <= kMostRows, "attn_kv4: M*Hq/Hkv=%lld (up to %lld)", (long long)M * (Hq / Hkv),
+                (long long)kMostRows);
     MXH_REQUIRE(ldq >= (int64_t)Hq * D && ldq % 8 == 0 && ((uintptr_t)q & 15) == 0,
                 "attn_kv4: q rows must be 16-byte aligned, at least Hq*D apart");
     MXH_REQUIRE(o || oq, "attn_kv4: no output (o and oq both null)");

@@ -15,6 +15,7 @@
 namespace kv4 {
 
 constexpr int kTile = 16;   // positions of an MFMA tile; pages hold whole tiles
+constexpr int kMaxPos = 1 << 30;   // positions of a sequence
 
 struct Cache {
     uint8_t* kq;
@@ -70,7 +71,7 @@ inline int make_cache(Cache& c, const char* what, const uint8_t* kq, const uint8
     } else {
         MXH_REQUIRE(n_pages >= B, "%s: %d sequences without a page table need as many pages, got %d", what, B, n_pages);
     }
-    MXH_REQUIRE(max_pos <= 1 << 30, "%s: more than 2^30 positions a sequence", what);
+    MXH_REQUIRE(max_pos <= kMaxPos, "%s: more than 2^30 positions a sequence", what);
     MXH_REQUIRE((int64_t)n_pages * page <= ((1ll << 32) - 2) / Hkv, "%s: a cache of 2^32 - 1 head rows or more", what);
     c = Cache{const_cast<uint8_t*>(kq), const_cast<uint8_t*>(ks), const_cast<uint8_t*>(vq), const_cast<uint8_t*>(vs),
               pages, n_pages, page, max_pages, lg, Hkv, (int)max_pos};

@@ -151,3 +151,13 @@ def test_binding_refuses_a_cache_of_no_heads():
     for _, call in _on_cpu(Hkv=0):
         with pytest.raises(RuntimeError, match="a kv head at least"):
             call()
+
+
+def test_workspace_size_of_calls_that_are_refused():
+    """0, whatever the sizes: groups of rows past 32 bits were divided by (2^32 of them are none)."""
+    size, top = _lib.load().mxfp4_attn_kv4_workspace_size, 2 ** 31 - 1
+    assert size(1, 65535, 16, 1, 128, 4096) >= 0 and size(2, 512, 32, 4, 128, 1 << 30) > 0
+    for a in ((1, 1 << 30, 128, 1, 128, 4096), (1, top, 64, 1, 128, 4096), (1, 65536, 1, 1, 128, 4096), (1, 65535, 17, 1, 128, 4096),
+              (1, 1, 65536, 1, 128, 4096), (65536, 1, 8, 8, 128, 4096), (2, 1, 8, 4, 128, top), (2, 1, 8, 4, 96, 4096),
+              (2, 1, 8, 4, 128, -5), (-1, 1, 8, 4, 128, 64), (top, top, top, 1, 128, top)):
+        assert size(*a) == 0, a
