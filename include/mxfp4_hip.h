@@ -240,7 +240,7 @@ int mxfp4_kv_write(const void* k, const void* v, uint8_t* kvk, uint8_t* kvv, con
  * elements each) of src_dtype (MXFP4_DT_*) -> MXFP4 rows, bit-exact to
  * mxfp4_quantize_rows.  Tokens outside the cache, or on no page, write nothing.
  * Two tokens of one call that share a row (a table that names a page twice, where
- * it is written) leave a mixture of both there.
+ * it is written) leave a mixture of both there.  B*M*Hkv*D/8 below 2^32 - 256.
  */
 int mxfp4_kv4_write(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq, uint8_t* ks,
                     uint8_t* vq, uint8_t* vs, const int32_t* pages, int n_pages, int page, int max_pages,
@@ -250,7 +250,7 @@ int mxfp4_kv4_write(const void* k, const void* v, int src_dtype, int64_t ldk, in
  * (start device int32 (B), NULL: 0) as k, v (B, n, Hkv, D) of dst_dtype,
  * 16-byte aligned.  bf16 and fp32 hold every value exactly as far as they reach
  * (past it: infinite); fp16 is rounded to nearest even.  Zeros where a position
- * lies outside the cache or on no page. */
+ * lies outside the cache or on no page.  B*n*Hkv*D/8 below 2^32 - 256. */
 int mxfp4_kv4_read(const uint8_t* kq, const uint8_t* ks, const uint8_t* vq, const uint8_t* vs, const int32_t* pages,
                    int n_pages, int page, int max_pages, const int32_t* start, void* k, void* v, int dst_dtype, int B,
                    int n, int Hkv, int D, void* stream);
@@ -258,7 +258,7 @@ int mxfp4_kv4_read(const uint8_t* kq, const uint8_t* ks, const uint8_t* vq, cons
 /* mxfp4_qk_norm_rope_kv4: mxfp4_qk_norm_rope_kv with this cache: qkv fp32 (B*M,
  * (Hq + 2 Hkv) * D) -> q_out bf16 (B*M, Hq, D), the same bits as there, and k
  * and bf16(v) to the cache, the bits of mxfp4_kv4_write of those bf16 rows.
- * D = 128. */
+ * D = 128; B*M below 2^24, Hq + 2 Hkv up to 262140. */
 int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k_norm_w, float eps, float theta,
                            uint8_t* kq, uint8_t* ks, uint8_t* vq, uint8_t* vs, const int32_t* pages, int n_pages,
                            int page, int max_pages, const int32_t* dpos, int B, int M, int Hq, int Hkv, int D,

@@ -448,10 +448,12 @@ bool takes(int B, int M, int Hq, int Hkv, int D, int max_pos) {
            max_pos > 0 && max_pos <= kv4::kMaxPos;
 }
 
+// Waves of a merge: about as many as load a row's records at once.  4 / 8 / 16, us: nine tokens over 23001 positions (42
+// shares) 23.4 / 23.4 / 25.2; one token over 16000, 16 heads (64 shares) 15.8 / 15.3 / 16.3
+int merge_waves(const Plan& p, int B) { return p.shares <= kFew * B || p.most <= kFew ? 4 : p.most <= 2 * kFew ? 8 : 16; }
+
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
-    // about as many waves as load a row's records at once.  4 / 8 / 16, us: nine tokens over 23001 positions (42 shares)
-    // 23.4 / 23.4 / 25.2; one token over 16000, 16 heads (64 shares) 15.8 / 15.3 / 16.3
-    const int nw = p.shares <= kFew * a.B || p.most <= kFew ? 4 : p.most <= 2 * kFew ? 8 : 16;
+    const int nw = merge_waves(p, a.B);
     const dim3 grid(a.M * a.Hq, a.B), block(64 * nw);
 #define MXH_M4(DD)                                                                               \
     if (nw == 4) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 4>), grid, block, 0, st, a);      \
@@ -491,7 +493,8 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     // p in three bf16 parts (all of fp32) for outputs that show it, in two (2^-17 of a term) for 8 or 11 bits
     const bool exact = (o && o_dtype == MXFP4_DT_F32) || oq;
     const Plan p = plan(B, M, Hq, Hkv, a.c.max_pos);
-    MXH_REQUIRE((int64_t)M * Hq < (1ll << 31), "attn_kv4: M*Hq too large");
+    // (the threads of a launch are counted in 32 bits)
+    MXH_REQUIRE(p.one || (int64_t)M * Hq * merge_waves(p, B) * 64 < (1ll << 32), "attn_kv4: M*Hq=%lld too large", (long long)M * Hq);
     const size_t need = mxfp4_attn_kv4_workspace_size(B, M, Hq, Hkv, D, a.c.max_pos);
     MXH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                 "attn_kv4: workspace must be 16-byte aligned and hold mxfp4_attn_kv4_workspace_size bytes");

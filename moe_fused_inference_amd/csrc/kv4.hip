@@ -158,10 +158,12 @@ __global__ __launch_bounds__(256) void qk_rope_kv4_kernel(const float* __restric
     half_wave_block(mx::bf16_to_f32(rb), q + 32, s + 2);
 }
 
+constexpr int64_t kMostGroups = (1ll << 24) - 1;   // workgroups of 256 threads in one dimension of a launch, whose threads are counted in 32 bits
+
 // T head rows of D values in threads of eight: the grid, or 0 if it is too large.
 unsigned grid_of(int64_t heads, int D) {
     const int64_t g = (heads * (D / 8) + 255) / 256;
-    return heads < (1ll << 31) && g < (1ll << 31) ? (unsigned)g : 0u;
+    return heads < (1ll << 31) && g <= kMostGroups ? (unsigned)g : 0u;
 }
 
 }  // namespace
@@ -231,11 +233,11 @@ extern "C" int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, co
     if (rc != MXFP4_OK) return rc;
     MXH_REQUIRE(qkv && q_norm_w && k_norm_w && dpos && q_out, "qk_norm_rope_kv4: null pointer");
     MXH_REQUIRE(D == kD, "qk_norm_rope_kv4: D=%d (%d)", D, kD);
-    MXH_REQUIRE(M > 0 && Hq > 0 && Hq % Hkv == 0 && (int64_t)B * M < (1ll << 31), "qk_norm_rope_kv4: B=%d M=%d Hq=%d Hkv=%d", B, M,
+    MXH_REQUIRE(M > 0 && Hq > 0 && Hq % Hkv == 0 && (int64_t)B * M <= kMostGroups, "qk_norm_rope_kv4: B=%d M=%d Hq=%d Hkv=%d", B, M,
                 Hq, Hkv);
-    const int nh = Hq + 2 * Hkv;
+    const int64_t nh = (int64_t)Hq + 2 * Hkv;
     MXH_REQUIRE(nh <= 4 * 65535, "qk_norm_rope_kv4: Hq=%d Hkv=%d", Hq, Hkv);
-    hipLaunchKernelGGL(qk_rope_kv4_kernel, dim3(B * M, (nh + 3) / 4), dim3(256), 0, mxh::as_stream(stream), qkv,
+    hipLaunchKernelGGL(qk_rope_kv4_kernel, dim3(B * M, (unsigned)(nh + 3) / 4), dim3(256), 0, mxh::as_stream(stream), qkv,
                        static_cast<const uint16_t*>(q_norm_w), static_cast<const uint16_t*>(k_norm_w), eps, theta, dpos, M, Hq,
                        static_cast<uint16_t*>(q_out), c);
     return mxh::launch_status("qk_norm_rope_kv4");

@@ -161,3 +161,15 @@ def test_workspace_size_of_calls_that_are_refused():
               (1, 1, 65536, 1, 128, 4096), (65536, 1, 8, 8, 128, 4096), (2, 1, 8, 4, 128, top), (2, 1, 8, 4, 96, 4096),
               (2, 1, 8, 4, 128, -5), (-1, 1, 8, 4, 128, 64), (top, top, top, 1, 128, top)):
         assert size(*a) == 0, a
+
+
+def test_launches_of_more_threads_than_32_bits():
+    """Refused by name before a launch: rows of 2^32 threads of eight values, and head counts past 31 bits."""
+    big = _cache(n_pages=64, page=1 << 14, pages=P, max_pages=1 << 10)
+    for D, M in ((128, 1 << 22), (64, 1 << 23)):                   # times 64 sequences: 2^28 (2^29) tokens, 2^32 threads a head
+        _refused(_write(big, D=D, B=64, M=M, Hkv=1), "too large")
+        _refused(_read(big, D=D, B=64, n=M, Hkv=1), "too large")
+    _refused(_rope(big, B=64, M=1 << 18), "M=262144")              # 2^24 workgroups of 256
+    _refused(_rope(Hq=2 ** 31 - 4, Hkv=4), "Hq=2147483644")
+    # rows to merge, a workgroup each (two sequences of 2^24 positions, 2^24 rows of q)
+    _refused(_attn(_cache(n_pages=2, page=1 << 14, pages=P, max_pages=1 << 10), B=2, M=65535, Hq=257, Hkv=257, wsb=1 << 60), "too large")
