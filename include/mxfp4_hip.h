@@ -284,8 +284,9 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  * position, gets zeros.  What the cache holds past dpos[b] + M - 1 is without
  * effect, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
  * Keys and values that reach past fp32 (code 253 or 254) are infinite and give NaN.
- * The sums of a token are rounded in an order that depends on the batch's
- * lengths, not on when the workgroups run: the same call gives the same bits.
+ * The sums of a token are rounded in an order that depends on the call's sizes and
+ * the batch's lengths, not on when the workgroups run nor on what the other rows of q
+ * and the other sequences hold: the same call gives the same bits.
  */
 size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos);
 int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,

@@ -298,9 +298,13 @@ __device__ __forceinline__ void terms(const float (&s)[N], float scale, float m,
     if (!wide) {
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] = fmaf(s[i], scale, -m);
-    } else {   // the rounded product, as in m: the fma's would differ from it by more than a term
+    } else {   // such a row's by the rounded product, as in m: the fma's would differ from it by more than a term
+        const bool mine = fabsf(m) > kWide;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[i] = mul_then_sub(s[i], scale, m);
+        for (int i = 0; i < N; ++i) {
+            const float near = fmaf(s[i], scale, -m), far = mul_then_sub(s[i], scale, m);
+            t[i] = mine ? far : near;
+        }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) t[i] = __builtin_amdgcn_exp2f(t[i]);
@@ -308,10 +312,11 @@ __device__ __forceinline__ void terms(const float (&s)[N], float scale, float m,
 #pragma unroll
     for (int i = 0; i < N; i += 4) sum += (t[i] + t[i + 1]) + (t[i + 2] + t[i + 3]);
 }
-// A lane's terms that sum to more than kMost (at its first unit, where m is kNone and they
-// are infinite, or past a much larger score) are made again, on the maximum, and what was
-// summed before is rescaled (rescale(factor)); over(x): the maximum over the row's lanes.
-// p: the terms' parts.  Then l, their sum so far, takes them.
+// The terms of a row with a lane of more than kMost (at its first unit, where m is kNone
+// and they are infinite, or past a much larger score) are made again, on the maximum, and
+// what was summed before is rescaled (rescale(factor)); over(x): the maximum over the row's
+// lanes.  The wave's other rows get the same terms and a factor of 1: a row's bits are its
+// own.  p: the terms' parts.  Then l, their sum so far, takes them.
 template <int N, int NP, class Over, class Rescale>
 __device__ __forceinline__ void again(const float (&s)[N], float scale, float& m, float& l, bool& wide, float sum, uint4 (&p)[N / 8][NP],
                                       Over over, Rescale rescale) {
@@ -319,7 +324,7 @@ __device__ __forceinline__ void again(const float (&s)[N], float scale, float& m
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < N; i += 2) top = max3(top, s[i], s[i + 1 < N ? i + 1 : i]);
-        const float mn = fmaxf(m, over(top) * scale);
+        const float mn = over(sum) > kMost ? fmaxf(m, over(top) * scale) : m;
         const float al = __builtin_amdgcn_exp2f(m - mn);
         l *= al;
         rescale(al);

@@ -54,20 +54,39 @@ def read(cache, n, start, pages=None):
     return k, v, there
 
 
+def rounding(D, n, big, size, q_parts=1):
+    """How far fp32 sums of the same operands may be from o = sum p v / sum p, as a multiple of sum p |v| / sum p.
+
+    Every fp32 addition and product rounds once, by at most u = 2^-24 of its result, in whatever order the matrix
+    unit and the lanes add; hardware exp2 is off by at most 2 ulp (4 u).  big: the largest sum |q k| / sqrt(D) of
+    a row (0 where the sums are exact), size: its largest |score|, X = log2(e) size.
+    - A score is q_parts D exact products: off by q_parts D u big.  In units of log 2 its exponent is a product by a
+      rounded constant (u X), rounded itself where the row's reference is far (u X), and a difference from the
+      reference (2 u X); then exp2.
+    - Sums meet by factors exp2(reference - reference): the difference rounds by u of it, exp2 and the product by
+      5 u.  A wave's reference moves up by 8 at least each time after the first, so 1 + X / 4 times and 2 X in all; the
+      waves' sums meet in LDS, the records in a wave of the merge (64 batches of eight at most) and its waves once
+      more: each level 2 X in all.
+    So a weight is off by a factor 1 +- e, e = log 2 u (log2(e) q_parts D big + 12 X) + (4 + 5 (1 + X / 4 + 2 + 64)) u.
+    - A numerator adds three parts of each of a wave's n / 4 positions, a denominator the terms of n / 16 in a lane
+      and the lanes; then the waves, and 1024 records at most by eights in waves: 3 n / 4 + 300 and n / 16 + 300
+      additions in a row.
+    """
+    u, x = 2.0 ** -24, np.log2(np.e) * size
+    e = np.log(2) * u * (np.log2(np.e) * q_parts * D * big + 12 * x) + (4 + 5 * (67 + x / 4)) * u
+    return 2 * e + (13 * n / 16 + 600) * u
+
+
 def attention(q, cache, dpos, pages=None):
     """q (B, M, Hq, D) float -> (o, bound), float64 (B, M, Hq, D).
 
-    bound: how far fp32 sums of the same operands may be from o, element by
-    element.  A score is D products summed in fp32 (error <= (D + 2) u sum|q k|,
-    u = 2^-24) and its exponent, in units of log 2, is a product, a difference
-    and a hardware exp2 of error <= 2 ulp (4 u); so every weight is off by a
-    factor 1 +- e, e <= log 2 * (scale * (D + 2) u max sum|q k| + 2 u max|x|) + 4 u.
-    Numerator and denominator sum n such terms (at most n/128 + 32 rounded
-    additions in a row, every V and part of p exact), and both merge twice.  An
-    output sum p v / sum p is then off by at most (2 e + 2 (n/128 + 40) u)
-    sum p |v| / sum p, and a rounding of its own.  A term, or a part of one, below
-    2^-126 of a row whose largest is at least 1 (and at most 2^8) is flushed: up to
-    four such parts a position, each at most 2^-126 max|v|, over a sum of at least 1.
+    bound: a tolerance on fp32 sums of the same operands, element by element.  It is not a proof (rounding is one):
+    it counts a score's D products and few roundings besides, as if the matrix unit rounded a step's sum once and the
+    three parts of a probability were added in one, which in a sum of one part a position would be 3 n / 128 additions
+    for up to 16 rows and 6 n / 128 for more, not n / 128.  Errors of either sign make up for that: on random operands
+    the kernels stay below a hundredth of it.  Scores: (D + 2) u sum|q k| each, u = 2^-24; exponents: 2 u max|x| and
+    exp2's 4 u; sums: n / 128 + 40 additions in a row.  A term, or a part of one, below 2^-126 of a row whose
+    denominator is at least 1 is flushed: up to four such parts a position, each at most 2^-126 max|v|.
     """
     u = 2.0 ** -24
     B, M, Hq, D = q.shape
