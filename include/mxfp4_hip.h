@@ -281,9 +281,12 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  * one part (fp16: two), a probability in three, or in two (16 bits, 2^-17 of it)
  * where more than 16 rows (M * Hq / Hkv) go to bf16 or fp16 alone.  A token outside
  * [0, max_pos), or one that sees no
- * position, gets zeros.  What the cache holds past dpos[b] + M - 1 is without
- * effect, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
- * Keys and values that reach past fp32 (code 253 or 254) are infinite and give NaN.
+ * position, gets zeros.  What the cache holds past a token's position is without
+ * effect on it, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
+ * Keys and values that reach past fp32 (code 253 or 254) are infinite: a token that
+ * sees such a value gets an infinity or NaN in its column, one that sees such a key
+ * what infinite scores give.  Sums run on terms of up to 2^11: they overflow where n
+ * positions' values reach 2^128 / (2^11 n).
  * The sums of a token are rounded in an order that depends on the call's sizes and
  * the batch's lengths, not on when the workgroups run nor on what the other rows of q
  * and the other sequences hold: the same call gives the same bits.

@@ -352,13 +352,43 @@ __device__ __forceinline__ float not_finite(uint4 w) {
     return z;
 }
 
+// Values that are not finite, in a unit with positions that not all of a workgroup's rows
+// see, are taken out of the products (0 times one is NaN), and what sees one is made NaN
+// here, after the last unit: from the first unit that is not `all_see`'s alone, positions up
+// to `to` of the wave's units (u0 + wave + NW j, up to u1 - 1).
+// The lane's query sees up to lim; of V's row it has CT nibbles at each of N columns
+// column(i), and mark(i, c, bits) sets bits of their sum: a NaN's, or none.
+template <int D, int CT, int N, int NW, class Column, class Mark>
+__device__ __forceinline__ void mark_not_finite(const Cache& cache, int b, int g, int wave, int u0, int u1, int all_see, int to, int lim,
+                                                Column column, Mark mark) {
+    for (int pos = max((all_see + 1) / kUnit, u0) * kUnit; pos <= to && pos / kUnit < u1; ++pos) {
+        if ((pos / kUnit - u0) % NW != wave) continue;
+        const int64_t row = kv4::head_row(cache, b, g, pos);
+        if (row < 0 || pos > lim) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int col = column(i);
+            const uint32_t code = cache.vs[row * (D / 32) + col / 32];
+            const uint8_t* p = cache.vq + row * (D / 2) + col / 2;
+            uint32_t w;
+            if constexpr (CT == 8) w = *reinterpret_cast<const uint32_t*>(p);
+            else if constexpr (CT == 4) w = *reinterpret_cast<const uint16_t*>(p);
+            else w = *p;
+            const uint32_t bad = kv4::not_finite(w, code);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) mark(i, c, 0u - (bad >> (4 * c) & 1u) & 0x7FC00000u);
+            __builtin_amdgcn_sched_barrier(0);       // (one at a time: no registers for the others' meanwhile)
+        }
+    }
+}
+
 // The end of row r of kv head g of sequence b, a segment from unit u0 on: NW waves' (m, l,
 // columns) to one record, or with ONE the output.  16 neighbouring lanes a row (by
-// threadIdx.x), which all call it, D / 16 columns a lane.
+// tid), which all call it, D / 16 columns a lane.
 template <int D, int NW, bool ONE, class M, class L, class O>
-__device__ __forceinline__ void finish(const Args& a, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
+__device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
     constexpr int CT = D / 16;
-    const int c0 = CT * (threadIdx.x & 15);
+    const int c0 = CT * (tid & 15);
     const int64_t pos = (int64_t)base + r / a.G;
     if (!ONE && (pos < 0 || pos >= a.c.max_pos || (int64_t)u0 * kUnit > pos)) return;   // no record: the merge reads none
     float gm = m_of(0);

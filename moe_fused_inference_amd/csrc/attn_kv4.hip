@@ -112,6 +112,12 @@ __device__ __forceinline__ void v_scales(const Raw<D>& r, float (&s)[8]) {
         s[i] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, D == 64 && (i & 1) ? turn + 16 : turn));
     }
 }
+// The values of a word under one scale that bf16 does not hold are taken out of it.
+__device__ __forceinline__ void take_out(uint32_t& w, float& scale) {
+    const uint32_t code = __float_as_uint(scale) >> 23 & 255u;
+    w &= ~(15u * kv4::not_finite(w, code));
+    if (code == 255u) scale = 1.0f;
+}
 // MFMA operands of four column tiles: columns D/16 l16 + 4 H + c x the lane's eight positions.
 template <int H>
 __device__ __forceinline__ void decode_v(const uint32_t (&v)[8], const float (&s)[8], uint4 (&vd)[4]) {
@@ -223,6 +229,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         mx::v4f acc[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[c] = mx::v4f{0.f, 0.f, 0.f, 0.f};
+        int dirty = 0;       // uniform: values that are not finite were taken out, among positions that not all rows see
         // Unit u, the wave's j-th.  `more`: the wave's next one is loaded meanwhile (decided in the code, not by a branch:
         // behind one the compiler waits for the older loads as if these had not been issued, that is for all)
         auto unit = [&](int u, int j, auto more_) {
@@ -285,6 +292,16 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                         r.v[i] = 0;
                         vs[i] = 1.0f;
                     }
+                if (lim_min < last) {                // nor may what only some rows see reach the others'
+                    uint32_t large = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) large = max(large, __float_as_uint(vs[i]) & 0x7F800000u);
+                    if (__ballot(large >= kv4::kLargeScale)) {
+                        dirty = 1;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) take_out(r.v[i], vs[i]);
+                    }
+                }
             }
             auto product = [&](auto half) {
                 constexpr int H = decltype(half)::value;
@@ -304,6 +321,14 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         int u = u0 + wave, j = 0;
         for (; u + NW < u1; u += NW, ++j) unit(u, j, std::true_type{});
         if (u < u1) unit(u, j, std::false_type{});
+        if (__builtin_amdgcn_readfirstlane(dirty)) {
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));              // (nothing of a lane is held for this)
+            const int l16 = t & 15, lq = t >> 4 & 3;
+            const int lim = l16 < rows ? clamped((int64_t)base + l16 / G) : 1 << 30;
+            mark_not_finite<D, CT, 4, NW>(a.c, b, g, wave, u0, u1, lim_min, last, lim, [&](int i) { return CT * (4 * lq + i); },
+                                          [&](int i, int c, uint32_t bits) { acc[c][i] = __uint_as_float(__float_as_uint(acc[c][i]) | bits); });
+        }
         // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is
         // column D/16 (4 lq + i) + c of query l16
         __syncthreads();
@@ -320,7 +345,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         __syncthreads();
         // thread: CT columns of a row (8 of 128, 4 of 64)
         const int qr = tid >> 4;
-        if (tid < 256 && qr < rows) finish<D, NW, ONE>(a, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
+        if (tid < 256 && qr < rows) finish<D, NW, ONE>(a, tid, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
     };
     each_segment<W>(a, segment);
 }

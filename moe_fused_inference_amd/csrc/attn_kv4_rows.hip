@@ -153,18 +153,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             for (int i = 0; i < D / 32; ++i) x[i] = scale_at(rcodes, i);
             *reinterpret_cast<svec*>(stage.scale[j & 1][lane]) = x;
         };
+        const int v_row = lane >> 2;                 // the lane's row of V in a tile
+        int dirty = 0;       // uniform: values that are not finite were taken out, among positions that not all rows see
+        const int all_see = min(lim_min, last);      // up to here
         auto put_v = [&](int j, const Unit& u) {
-            if (ragged(u)) {
+            if (__builtin_amdgcn_readfirstlane(u.there != 3 || u.p0 + kUnit - 1 > all_see)) {
                 int sees = last - u.p0;
                 asm volatile("" : "+v"(sees));
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
-                    if (!(u.there >> t & 1) || 16 * t + (lane >> 2) > sees) rv[t] = 0;
+                    if (!(u.there >> t & 1) || 16 * t + v_row > sees) rv[t] = 0;
+                // nor may what only some rows see reach the others'
+                float* scale[2];
+                uint32_t large = 0;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    scale[t] = &stage.scale[j & 1][32 + 16 * t + v_row][D == 128 ? lane & 3 : (lane & 3) >> 1];
+                    large = max(large, __float_as_uint(*scale[t]) & 0x7F800000u);
+                }
+                if (__ballot(large >= kv4::kLargeScale)) {
+                    dirty = 1;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t code = __float_as_uint(*scale[t]) >> 23 & 255u;
+                        if (code == 255u) *scale[t] = 1.0f;
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) rv[t][i] &= ~(15u * kv4::not_finite(rv[t][i], code));
+                    }
+                }
             }
-            const int r = lane >> 2;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                *reinterpret_cast<hvec*>(&stage.v[j & 1][t][(r & 8) + 2 * (r & 3) + ((r >> 2) & 1)][(lane & 3) * (D / 8)]) = rv[t];
+                *reinterpret_cast<hvec*>(&stage.v[j & 1][t][(v_row & 8) + 2 * (v_row & 3) + ((v_row >> 2) & 1)][(lane & 3) * (D / 8)]) = rv[t];
         };
         Unit ua = locate(0), ub = ua, uc = ua;
         load_k(ua);
@@ -309,6 +329,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 products(j, pa);
             }
         }
+        if (__builtin_amdgcn_readfirstlane(dirty))
+            mark_not_finite<D, CT, 16, kWaves>(a.c, b, g, wave, u0, u1, all_see, last, lim,
+                                               [&](int i) { return CT * (8 * (i / 4) + 4 * lh + i % 4); },
+                                               [&](int i, int c, uint32_t bits) { acc[c][i] = __uint_as_float(__float_as_uint(acc[c][i]) | bits); });
         // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is column
         // CT (8 (i / 4) + 4 lh + i % 4) + c of query l32
         __syncthreads();
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
 #pragma unroll 1
         for (int qr = tid >> 4; qr < R; qr += NT / 16)
             if (r0 + qr < rows)
-                finish<D, kWaves, ONE>(a, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
+                finish<D, kWaves, ONE>(a, tid, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
                                        [&](int w, int c) { return *reinterpret_cast<const float4*>(&lds.mo[w][qr][c]); });
     };
     each_segment<W>(a, segment);

@@ -51,6 +51,14 @@ __device__ __forceinline__ uint4 eight_bf16(uint32_t w, float scale) {
     return make_uint4(pair_bf16<0>(w, scale), pair_bf16<1>(w, scale), pair_bf16<2>(w, scale), pair_bf16<3>(w, scale));
 }
 
+// The nibbles of w whose values under scale code `code` bf16 does not hold (infinite, or NaN): a 1 for each.
+// 4 and 6 times 2^126, 2 and more times 2^127, and all of code 255.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w, uint32_t code) {
+    const uint32_t bits = code == 255 ? ~0u : code == 254 ? w >> 2 : code == 253 ? w >> 2 & w >> 1 : 0u;
+    return bits & 0x11111111u;
+}
+constexpr uint32_t kLargeScale = 253u << 23;   // of scale_of's exponent field: values that are not finite may be there
+
 // The cache arguments of an entry point as a Cache; MXFP4_EINVAL with a message if they cannot be one.
 inline int make_cache(Cache& c, const char* what, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq, const uint8_t* vs,
                       const int32_t* pages, int n_pages, int page, int max_pages, int B, int Hkv, int D) {
