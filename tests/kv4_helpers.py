@@ -79,21 +79,25 @@ def attention64(q, cache, dpos, pages=None, exact_scores=False):
         see = there & (torch.arange(n, device=q.device) <= pos[:, None]) & ((pos >= 0) & (pos < top))[:, None]   # (M, n)
         see = see.repeat_interleave(G, 0)
         any_ = see.any(-1, keepdim=True)
-        for g in range(Hkv):
-            k, v = decode64(rows[0][g], rows[1][g]), decode64(rows[2][g], rows[3][g])
+        step = max(1, (1 << 26) // max(M * G * n, n * D))        # kv heads at a time
+        for g in range(0, Hkv, step):
+            h = slice(g, min(g + step, Hkv))
+            k, v = decode64(rows[0][h], rows[1][h]), decode64(rows[2][h], rows[3][h])
             k, v = torch.where(there[:, None], k, 0.0), torch.where(there[:, None], v, 0.0)
-            x = q[b, :, g * G:(g + 1) * G].reshape(M * G, D).double()
-            s = (x @ k.T) / math.sqrt(D)
+            x = q[b].unflatten(1, (Hkv, G))[:, h].transpose(0, 1).flatten(1, 2).double()         # (heads, M * G, D)
+            s = torch.matmul(x, k.transpose(1, 2).contiguous()) / math.sqrt(D)
             size = s.abs().masked_fill(~see, 0).amax(-1, keepdim=True)
-            big = ((x.abs() @ k.abs().T) / math.sqrt(D)).masked_fill(~see, 0).amax(-1, keepdim=True)
+            big = torch.matmul(x.abs(), k.abs().transpose(1, 2).contiguous()) / math.sqrt(D)
+            big = big.masked_fill(~see, 0).amax(-1, keepdim=True)
             s = s.masked_fill(~see, -math.inf)
             p = torch.exp(s - torch.where(any_, s.amax(-1, keepdim=True), 0.0))
             den = torch.where(any_, p.sum(-1, keepdim=True), 1.0)
-            want = p @ v / den
+            want = torch.matmul(p, v) / den
             rel = ref.rounding(D, n, 0.0 if exact_scores else big, size, 2 if q.dtype == torch.float16 else 1)
-            lim = rel * (p @ v.abs()) / den + 2 * 2.0 ** -24 * want.abs() + 4 * n * 2.0 ** -126 * v.abs().max()
-            o[b, :, g * G:(g + 1) * G] = want.view(M, G, D)
-            bound[b, :, g * G:(g + 1) * G] = torch.where(any_, lim, 0.0).view(M, G, D)
+            lim = rel * torch.matmul(p, v.abs()) / den + 2 * 2.0 ** -24 * want.abs() + 4 * n * 2.0 ** -126 * v.abs().max()
+            lim = torch.where(any_, lim, 0.0)
+            for t, to in ((want, o), (lim, bound)):
+                to[b].unflatten(1, (Hkv, G))[:, h] = t.unflatten(1, (M, G)).transpose(0, 1)
     return o, bound
 
 
@@ -114,3 +118,20 @@ def _sizes(q, cache, dpos, pages):
     """sum p |v| / sum p."""
     plus = [cache[0], cache[1], cache[2] & 0x77, cache[3]]
     return attention64(q, plus, dpos, pages)[0]
+
+
+# ------------------------------------------------------------------ the bits of a probability
+P_BITS = 24 * 2.0 ** -24     # see p_rows
+
+
+def p_rows(n, D):
+    """n bf16 values x in (0, 4 sqrt(D) log 2): with a key of -x / q at one position and zeros at the others of a row, that
+    position's probability is p = 2^-t over 1 + others, t = x log2(e) / sqrt(D) < 4, and a value of 1 there alone makes the
+    output p / (p + others).
+
+    How far fp32 may be from it, relatively, u = 2^-24: t's constant and its fma 2.8 u each (u t log 2), exp2 4 u; p's three
+    parts are its 24 bits, their sum one rounding at most; the denominator ten (three in a lane, two over lanes, four waves,
+    one merge), its reciprocal and the product two: under 24 u.  A p of two bf16 parts is off by up to 64 u more.
+    """
+    x = torch.linspace(0.02, 1.0, n, dtype=torch.float64) * 4 * math.sqrt(D) * math.log(2) * 0.99
+    return x.to(torch.bfloat16)

@@ -48,3 +48,26 @@ def test_attention_is_the_softmax_of_the_visible_rows():
     assert (bound[0] > 0).all() and bound.max() < 1e-2 * np.abs(o).max()
     assert not kv4.attention(q, cache, [-2], pages)[0].any()      # an empty slot
     assert not kv4.attention(q, cache, [20], np.array([[-1, 7, -9]], np.int32))[0].any()   # no page at all
+
+
+def test_two_parts_of_a_probability_would_show():
+    """What the bound of the probabilities' bits is good for: p in two bf16 parts passes it, in three it does not."""
+    import torch
+
+    from tests.kv4_helpers import P_BITS, p_rows
+    for D in (64, 128):
+        p = torch.exp2(-p_rows(256, D).double() * np.log2(np.e) / np.sqrt(D)).float()
+        rest, off = p.clone(), []
+        for _ in range(3):
+            rest = rest - rest.bfloat16().float()
+            off.append(float((rest.abs() / p).max()))
+        assert off[1] > P_BITS and off[2] == 0
+
+
+def test_the_proven_bound_is_above_the_tolerance():
+    """rounding() counts more than attention()'s tolerance does, at any size."""
+    u = 2.0 ** -24
+    for D, n, big, size in ((64, 1, 1.0, 1.0), (128, 4096, 30.0, 8.0), (128, 32768, 100.0, 90.0)):
+        e = np.log(2) * (1.4427 * (D + 2) * u * big + 2 * u * 1.4427 * size) + 4 * u
+        assert kv4.rounding(D, n, big, size) > 2 * e + 2 * (n / 128 + 40) * u
+    assert kv4.rounding(128, 4096, 0.0, 8.0) < 3e-4
