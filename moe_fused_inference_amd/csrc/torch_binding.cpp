@@ -309,7 +309,7 @@ Kv4 kv4_cache(const torch::Tensor& kq, const torch::Tensor& ks, const torch::Ten
         c.B = as_int(pages->size(0), "too many sequences");
         c.max_pages = as_int(pages->size(1), "too many pages");
         // a table of no columns has no address, which would stand for no table
-        require(c.max_pages > 0, "pages must have a column at least");
+        require(c.max_pages > 0 || c.B == 0, "pages must have a column at least");
     }
     if (at.has_value()) {
         require(at->scalar_type() == torch::kInt32 && at->is_contiguous() && at->device() == dev && at->numel() == c.B, at_msg);

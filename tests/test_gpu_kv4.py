@@ -562,3 +562,30 @@ def test_a_cache_of_no_heads():
                  lambda: kv4.attn_decode4_mx(q, cache, dp)):
         with pytest.raises(RuntimeError, match="a kv head at least"):
             call()
+
+
+def test_an_empty_batch():
+    cache, dp = kv4.empty_cache(3, 32, 2, 64), torch.empty(0, dtype=torch.int32, device=DEV)
+    x, q = torch.empty((0, 2, 2, 64), device=DEV), torch.empty((0, 2, 4, 64), device=DEV).bfloat16()
+    for cols in (0, 3):
+        t = torch.empty((0, cols), dtype=torch.int32, device=DEV)
+        kv4.kv4_write(x, x, cache, dp, t)
+        assert kv4.kv4_read(cache, 5, dp, t)[0].shape == (0, 5, 2, 64)
+        assert kv4.attn_decode4(q, cache, dp, t).shape == (0, 2, 4, 64) and kv4.attn_decode4_mx(q, cache, dp, t)[1].shape == (0, 8)
+    assert not any(c.any() for c in cache)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,G", [(1, 2), (2, 16)])
+def test_the_smallest_keys_and_values(M, G, D):
+    """Scale code 0: keys and values below bf16's normal numbers, which the products must not take for zeros."""
+    cache = kv4.empty_cache(1, 64, 1, D)
+    cache.kq[0, 0, 0, 0], cache.vq[0, 0, 0] = 0x01, 0x11            # 2^-128 in dimension 0, and everywhere
+    cache.vq[0, 0, 1] = 0x32                                        # 2^-127 and 1.5 * 2^-127
+    q = torch.zeros((1, M, G, D), device=DEV).bfloat16()
+    q[..., 0] = 2.0 ** 127                                          # a score of 1/2 at position 0, 0 at the others
+    q[0, 0, 0, 0] = 2.0 ** 120                                      # 2^-8
+    o = kv4.attn_decode4(q, cache, _i32([1]))
+    host = [np_(c) for c in cache]
+    want, bound = ref.attention(np_(q.float()), host, [1])
+    assert (want != 0).all() and (np.abs(np_(o).astype(np.float64) - want) <= bound + 2.0 ** -148).all()

@@ -137,8 +137,7 @@ def _on_cpu(Hkv=4, D=128, n_pages=2, pages=None):
             ("attn", lambda: kv4.attn_decode4(q, cache, d, pages)), ("attn_mx", lambda: kv4.attn_decode4_mx(q, cache, d, pages))]
 
 
-@pytest.mark.parametrize("pages", [torch.zeros((2, 0), dtype=torch.int32), torch.zeros((2, 3), dtype=torch.int32)[:, :0].contiguous(),
-                                   torch.zeros((0, 0), dtype=torch.int32)])
+@pytest.mark.parametrize("pages", [torch.zeros((2, 0), dtype=torch.int32), torch.zeros((2, 3), dtype=torch.int32)[:, :0].contiguous()])
 def test_binding_refuses_a_table_of_no_columns(pages):
     """It has no address, and no address means that sequence b is page b."""
     for _, call in _on_cpu(pages=pages):
@@ -173,3 +172,11 @@ def test_launches_of_more_threads_than_32_bits():
     _refused(_rope(Hq=2 ** 31 - 4, Hkv=4), "Hq=2147483644")
     # rows to merge, a workgroup each (two sequences of 2^24 positions, 2^24 rows of q)
     _refused(_attn(_cache(n_pages=2, page=1 << 14, pages=P, max_pages=1 << 10), B=2, M=65535, Hq=257, Hkv=257, wsb=1 << 60), "too large")
+
+
+def test_binding_takes_an_empty_batch_whatever_its_table():
+    """No sequence, no work: what is left to refuse is the device."""
+    for shape in ((0, 0), (0, 3)):
+        for _, call in _on_cpu(pages=torch.zeros(shape, dtype=torch.int32)):
+            with pytest.raises(RuntimeError, match="must be cuda"):
+                call()
