@@ -21,8 +21,9 @@ constexpr float kNone = -3e38f;        // the reference of a row that has seen n
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 constexpr int kFew = 32;               // shares of a sequence that four waves merge at once
 constexpr int kMinShare = 4;           // units, one a wave
-// Units that take about as long as a workgroup's change to another sequence.  6 / 9 / 12 / 20, us: 48 sequences of up to
-// 8192 positions (four heads) 30.0 / 28.8 / 30.6 / 30.8; none at all 37.3.
+// Units that take about as long as a workgroup's change to another sequence; whole shares of kMinShare.  4 / 6 / 8 / 9 /
+// 12 / 20, us: 48 sequences of up to 8192 positions (four heads) 30.7 / 29.7 / 28.3 / 27.9 / 29.8 / 29.6, 32 of 32768
+// 58.6 / 56.1 / 56.8 / 56.6 / 56.5 / 56.4, 300 of 8000 139 / 139 / 138 / 138 / 138 / 141; none at all, 48 of 8192 37.3.
 constexpr uint32_t kPad = 8;
 
 struct Out {

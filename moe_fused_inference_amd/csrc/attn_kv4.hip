@@ -26,13 +26,16 @@
 // it moves to the maximum only where a lane's terms sum past kMost.
 //
 // What bounds it.  A long batch: memory.  32 sequences of up to 32768 positions (267 MB,
-// four heads of 128, eight query heads each) 55.8 us, of which 4 the merge, 5.2 TB/s in
+// four heads of 128, eight query heads each) 56.2 us, of which 4.8 the merge, 5.2 TB/s in
 // the shares' kernel; a plain streaming read 6.1 TB/s.  Eight sequences of 65536: 107 us,
 // 5.35 TB/s in all.  For that: 128 registers, so four waves a SIMD, each with a unit's loads
 // ahead (4.3 KB; 69 KB a CU).  Two ahead by buffer descriptors 74 us, V through LDS 68.
 // A short call: two launches, each one dependent chain of memory latencies (dpos, page,
-// rows; records): 500 positions 4.4 + 3.2 us, 32000 8.6 + 4.7 (5.0 + 3.3 and 9.0 + 5.0
+// rows; records): 500 positions 4.5 + 3.2 us, 32000 8.3 + 4.9 (5.0 + 3.3 and 9.0 + 5.0
 // before a share of one sequence loaded its first unit ahead of dpos).
+// Rows are apart: a row's reference moves by its own terms, and values that are not finite
+// are kept from the tokens before them (mark_not_finite).  Both are code off the loop's
+// path; it costs 48 sequences 26.4 -> 26.6 us, 7 x 3 tokens of 5 heads 8.9 -> 9.3.
 #include "attn_kv4.h"
 #include "kv4.h"
 #include "mx_device.h"
@@ -46,9 +49,12 @@ namespace {
 using namespace mxa;
 
 constexpr int kParts = 3;              // bf16 parts of a probability
-// A cache of more bytes, half the chip's last one, is not there any more when the next call comes: K by streaming loads.
-// Plain / so, us: 32 sequences of up to 32768 positions (571 MB) 59.0 / 55.9, 48 of 8192 (214 MB) 27.9 / 27.2; but 64
-// of 2000 (71 MB, read again and again) 18.1 / 18.7.  V too: 48 sequences 29.0 (its loads take half lines).
+// K by streaming loads where there is room for more bytes (the lengths are on the device): half the chip's last cache,
+// past which nothing is there any more when the same cache's next call comes.  Plain / so, us: 32 sequences of up to 32768
+// positions (571 MB) 59.0 / 55.9, 48 of 8192 (214 MB) 27.9 / 27.2.  Below it a cache that is read again at once stays: 48 of
+// 4096 (107 MB) 28.9 / 29.7, 16 of 4096 17.3 / 18.0; where other caches come between, as in a step of many layers (1.5 GB
+// of them in turn), it is the same: 31.8 / 31.7, 18.8 / 18.9, one of 32000 13.3 / 13.0.  V too: 48 of 8192 29.0 (its loads
+// take half lines).
 constexpr int64_t kMuch = 128ll << 20;
 
 // A unit's bytes as a lane loads them.  K: row 16 t + l16, D/8 bytes from D/8 lq on
@@ -455,6 +461,8 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
     // 26.0), 4096 63.5 / 57.3 (38.2 / 49.2); 2048 workgroups, 8192 positions 446 / 406 (238 / 247).  Nine tokens, 384
     // workgroups: 2048 positions 54.0 / 38.3 (43.0 / 36.6), 4096 79.5 / 69.0 (56.5 / 65.6).  One piece of a prompt of
     // 128 tokens, 128 workgroups: 1024 positions 22.7 / 15.8, 8192 49.8 / 84.1.
+    // What it gives away is a batch of one long sequence among short ones, which the host cannot know: one of 8192 positions
+    // among 255 of 64, eight kv heads, 32 / 142 (all of 8192: 406 / 376), one of 32768 among 63, 64 kv heads, 85 / 1048 (3008 / 2899).
     const int64_t wgs = (int64_t)B * Hkv * p.groups;
     p.one = p.waves == 16 || longest == 1 || want * 4 <= B || (want == 1 && B == 1) || max_pos <= (p.many ? 8 : 4) * wgs;
     p.shares = p.one ? B : (int)std::min(want, most);
@@ -515,7 +523,11 @@ extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uin
     MXH_REQUIRE(!oq == !os, "attn_kv4: oq and os go together");
     MXH_REQUIRE(o_dtype >= MXFP4_DT_BF16 && o_dtype <= MXFP4_DT_F32, "attn_kv4: o dtype %d", o_dtype);
     MXH_REQUIRE((((uintptr_t)o) & 15) == 0 && ((uintptr_t)oq & 3) == 0, "attn_kv4: o must be 16-byte, oq 4-byte aligned");
-    // p in three bf16 parts (all of fp32) for outputs that show it, in two (2^-17 of a term) for 8 or 11 bits
+    // p in three bf16 parts, all of fp32's 24 bits, for outputs that show them; for more than 16 rows to bf16 or fp16 alone,
+    // in two: each rounds to nearest, so a term is off by 2^-18 of itself at most, an output by that of sum p |v|, 2^-9 (fp16:
+    // 2^-6) of its own rounding's half step where its terms do not cancel.  The denominator sums fp32 terms.  A piece of 512 tokens over 8192
+    // positions, two / three: 119 / 137 us; 0.23 % / 0.01 % of the bf16 outputs are the neighbour of the nearest (of fp32
+    // torch operators 0.09 %), and the error against 64 bits, which is bf16's own, is 1.66e-3 of the norm for all three.
     const bool exact = (o && o_dtype == MXFP4_DT_F32) || oq;
     const Plan p = plan(B, M, Hq, Hkv, a.c.max_pos);
     // (the threads of a launch are counted in 32 bits)

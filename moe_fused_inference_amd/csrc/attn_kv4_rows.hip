@@ -19,9 +19,9 @@
 //     through the wave's own LDS, with no barrier;
 //   - the software pipeline in `step`: unit j + 1's terms between unit j's products, unit
 //     j + 2's scores after, K loaded two units ahead and V one;
-//   - p in two bf16 parts where 8 or 11 bits go out (fp32 out: three, 134 .. 148).
+//   - p in two bf16 parts where 8 or 11 bits go out (fp32 out: three, 137).
 // And 114 with the scales spread once into LDS, 16 rotations a unit fewer (the same call
-// 114 .. 122 from card to card): 580 TFLOP/s, 680 for 2048 tokens over 32768.
+// 108 .. 119 from card to card): 560 to 620 TFLOP/s, 680 for 2048 tokens over 32768.
 //
 // Operands.  S^T: lane (l32, lh) has row l32 of the unit (a position) and dimensions
 // D/2 lh + 8 kt .. of step kt; the product leaves it positions 8 (i / 4) + 4 lh + i % 4 of
