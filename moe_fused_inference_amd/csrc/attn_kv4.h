@@ -355,30 +355,22 @@ __device__ __forceinline__ float not_finite(uint4 w) {
 
 // Values that are not finite, in a unit with positions that not all of a workgroup's rows
 // see, are taken out of the products (0 times one is NaN), and what sees one is made NaN
-// here, after the last unit: from the first unit that is not `all_see`'s alone, positions up
-// to `to` of the wave's units (u0 + wave + NW j, up to u1 - 1).
-// The lane's query sees up to lim; of V's row it has CT nibbles at each of N columns
-// column(i), and mark(i, c, bits) sets bits of their sum: a NaN's, or none.
-template <int D, int CT, int N, int NW, class Column, class Mark>
-__device__ __forceinline__ void mark_not_finite(const Cache& cache, int b, int g, int wave, int u0, int u1, int all_see, int to, int lim,
-                                                Column column, Mark mark) {
+// here, in a wave's sums once they lie in LDS (mo: row r0 on; by the wave that put them
+// there): from the first unit that is not `all_see`'s alone, positions up to `to` of the
+// wave's units (u0 + wave + NW j, up to u1 - 1).
+template <int D, int NW>
+__device__ __forceinline__ void mark_not_finite(const Args& a, int b, int base, int g, int r0, int rows, int wave, int u0, int u1, int all_see,
+                                                int to, float (*mo)[D + 4]) {
+    asm volatile("" ::: "memory");                   // (behind the wave's own stores, which LDS keeps in order)
     for (int pos = max((all_see + 1) / kUnit, u0) * kUnit; pos <= to && pos / kUnit < u1; ++pos) {
         if ((pos / kUnit - u0) % NW != wave) continue;
-        const int64_t row = kv4::head_row(cache, b, g, pos);
-        if (row < 0 || pos > lim) continue;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int col = column(i);
-            const uint32_t code = cache.vs[row * (D / 32) + col / 32];
-            const uint8_t* p = cache.vq + row * (D / 2) + col / 2;
-            uint32_t w;
-            if constexpr (CT == 8) w = *reinterpret_cast<const uint32_t*>(p);
-            else if constexpr (CT == 4) w = *reinterpret_cast<const uint16_t*>(p);
-            else w = *p;
-            const uint32_t bad = kv4::not_finite(w, code);
-#pragma unroll
-            for (int c = 0; c < CT; ++c) mark(i, c, 0u - (bad >> (4 * c) & 1u) & 0x7FC00000u);
-            __builtin_amdgcn_sched_barrier(0);       // (one at a time: no registers for the others' meanwhile)
+        const int64_t row = kv4::head_row(a.c, b, g, pos);
+        if (row < 0) continue;
+        const int first = (int)max((int64_t)0, ((int64_t)pos - base) * a.G - r0);      // rows from here on see it
+        for (int col = threadIdx.x & 63; col < D; col += 64) {
+            const uint32_t w = a.c.vq[row * (D / 2) + col / 2] >> (4 * (col & 1));
+            if (kv4::not_finite(w, a.c.vs[row * (D / 32) + col / 32]) & 1)
+                for (int r = first; r < rows; ++r) mo[r][col] = __builtin_nanf("");
         }
     }
 }

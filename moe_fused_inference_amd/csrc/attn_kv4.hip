@@ -31,11 +31,11 @@
 // 5.35 TB/s in all.  For that: 128 registers, so four waves a SIMD, each with a unit's loads
 // ahead (4.3 KB; 69 KB a CU).  Two ahead by buffer descriptors 74 us, V through LDS 68.
 // A short call: two launches, each one dependent chain of memory latencies (dpos, page,
-// rows; records): 500 positions 4.5 + 3.2 us, 32000 8.3 + 4.9 (5.0 + 3.3 and 9.0 + 5.0
+// rows; records): 500 positions 4.5 + 3.2 us, 32000 8.1 + 4.9 (5.0 + 3.3 and 9.0 + 5.0
 // before a share of one sequence loaded its first unit ahead of dpos).
 // Rows are apart: a row's reference moves by its own terms, and values that are not finite
 // are kept from the tokens before them (mark_not_finite).  Both are code off the loop's
-// path; it costs 48 sequences 26.4 -> 26.6 us, 7 x 3 tokens of 5 heads 8.9 -> 9.3.
+// path; it costs 48 sequences 26.4 -> 26.5 us, 7 x 3 tokens of 5 heads 8.95 -> 9.1.
 #include "attn_kv4.h"
 #include "kv4.h"
 #include "mx_device.h"
@@ -327,14 +327,6 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         int u = u0 + wave, j = 0;
         for (; u + NW < u1; u += NW, ++j) unit(u, j, std::true_type{});
         if (u < u1) unit(u, j, std::false_type{});
-        if (__builtin_amdgcn_readfirstlane(dirty)) {
-            int t = threadIdx.x;
-            asm volatile("" : "+v"(t));              // (nothing of a lane is held for this)
-            const int l16 = t & 15, lq = t >> 4 & 3;
-            const int lim = l16 < rows ? clamped((int64_t)base + l16 / G) : 1 << 30;
-            mark_not_finite<D, CT, 4, NW>(a.c, b, g, wave, u0, u1, lim_min, last, lim, [&](int i) { return CT * (4 * lq + i); },
-                                          [&](int i, int c, uint32_t bits) { acc[c][i] = __uint_as_float(__float_as_uint(acc[c][i]) | bits); });
-        }
         // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is
         // column D/16 (4 lq + i) + c of query l16
         __syncthreads();
@@ -348,6 +340,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
             mm[wave][l16] = m;
             ml[wave][l16] = ls;
         }
+        if (__builtin_amdgcn_readfirstlane(dirty)) mark_not_finite<D, NW>(a, b, base, g, 0, rows, wave, u0, u1, lim_min, last, mo[wave]);
         __syncthreads();
         // thread: CT columns of a row (8 of 128, 4 of 64)
         const int qr = tid >> 4;

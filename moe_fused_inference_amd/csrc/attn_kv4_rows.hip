@@ -329,10 +329,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 products(j, pa);
             }
         }
-        if (__builtin_amdgcn_readfirstlane(dirty))
-            mark_not_finite<D, CT, 16, kWaves>(a.c, b, g, wave, u0, u1, all_see, last, lim,
-                                               [&](int i) { return CT * (8 * (i / 4) + 4 * lh + i % 4); },
-                                               [&](int i, int c, uint32_t bits) { acc[c][i] = __uint_as_float(__float_as_uint(acc[c][i]) | bits); });
         // the waves' sums in LDS, then one record (or the output) per row: acc[c][i] is column
         // CT (8 (i / 4) + 4 lh + i % 4) + c of query l32
         __syncthreads();
@@ -347,6 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             mm[wave][l32] = m;
             ml[wave][l32] = ls;
         }
+        if (__builtin_amdgcn_readfirstlane(dirty)) mark_not_finite<D, kWaves>(a, b, base, g, r0, min(R, rows - r0), wave, u0, u1, all_see, last, lds.mo[wave]);
         __syncthreads();
 #pragma unroll 1
         for (int qr = tid >> 4; qr < R; qr += NT / 16)
