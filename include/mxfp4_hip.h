@@ -276,12 +276,14 @@ int mxfp4_qk_norm_rope_kv4(const float* qkv, const void* q_norm_w, const void* k
  *   workspace  16-byte aligned, mxfp4_attn_kv4_workspace_size(B, M, Hq, Hkv, D,
  *              max_pos) bytes (0: may be NULL); nothing persists, but calls that
  *              share one must be stream-ordered
- * M and Hq up to 65535, M * Hq / Hkv up to 1048560; the size of a call that is refused is 0.
+ * M and Hq up to 65535, M * Hq / Hkv up to 1048560, M * Hq below 2^22 where the size
+ * is not 0 (some larger ones are taken); the size of a call whose sizes are refused is 0.
  * Sums and softmax in fp32.  The products are bf16 with every operand exact: q in
  * one part (fp16: two), a probability in three, or in two (16 bits, 2^-18 of it)
  * where more than 16 rows (M * Hq / Hkv) go to bf16 or fp16 alone.  A token outside
- * [0, max_pos), or one that sees no position, gets zeros.  What the cache holds past a token's position is without
- * effect on it, NaN included.  A q row with an infinity or a NaN gives a row of NaN.
+ * [0, max_pos), or one that sees no position, gets zeros.  What the cache holds past
+ * a token's position is without effect on it, NaN included.  A q row with an infinity
+ * or a NaN gives a row of NaN.
  * Keys and values that reach past fp32 (code 253 or 254) are infinite: a token that
  * sees such a value gets an infinity or NaN in its column, one that sees such a key
  * what infinite scores give.  Sums run on terms of up to 2^11: they overflow where n

@@ -80,12 +80,11 @@ def rounding(D, n, big, size, q_parts=1):
 def attention(q, cache, dpos, pages=None):
     """q (B, M, Hq, D) float -> (o, bound), float64 (B, M, Hq, D).
 
-    bound: a tolerance on fp32 sums of the same operands, element by element.  It is not a proof (rounding is one):
-    it counts a score's D products and few roundings besides, as if the matrix unit rounded a step's sum once and the
-    three parts of a probability were added in one, which in a sum of one part a position would be 3 n / 128 additions
-    for up to 16 rows and 6 n / 128 for more, not n / 128.  Errors of either sign make up for that: on random operands
-    the kernels stay below a hundredth of it.  Scores: (D + 2) u sum|q k| each, u = 2^-24; exponents: 2 u max|x| and
-    exp2's 4 u; sums: n / 128 + 40 additions in a row.  A term, or a part of one, below 2^-126 of a row whose
+    bound: a tolerance on fp32 sums of the same operands, element by element: scores (D + 2) u sum|q k| each, u = 2^-24,
+    exponents 2 u max|x| and exp2's 4 u, sums n / 128 + 40 additions in a row.  It is not a proof (rounding is one).  A
+    score of fp16 has 2 D products; a wave with a whole sequence adds three parts of its terms, 3 n / 128 matrix steps for
+    up to 16 rows and 6 n / 128 for more, each a sum of products itself.  Errors of either sign make up for that: on
+    random operands the kernels stay below a hundredth of it.  A term, or a part of one, below 2^-126 of a row whose
     denominator is at least 1 is flushed: up to four such parts a position, each at most 2^-126 max|v|.
     """
     u = 2.0 ** -24
