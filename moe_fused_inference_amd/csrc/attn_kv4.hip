@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                         r.v[i] = 0;
                         vs[i] = 1.0f;
                     }
-                if (lim_min < last) {                // nor may what only some rows see reach the others'
+                if (p0 + kUnit - 1 > lim_min && lim_min < last) {   // nor may what only some rows see reach the others'
                     uint32_t large = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) large = max(large, __float_as_uint(vs[i]) & 0x7F800000u);

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                     scale[t] = &stage.scale[j & 1][32 + 16 * t + v_row][D == 128 ? lane & 3 : (lane & 3) >> 1];
                     large = max(large, __float_as_uint(*scale[t]) & 0x7F800000u);
                 }
-                if (__ballot(large >= kv4::kLargeScale)) {
+                if (u.p0 + kUnit - 1 > all_see && __ballot(large >= kv4::kLargeScale)) {
                     dirty = 1;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
