@@ -298,6 +298,28 @@ int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, c
                    void* o, int o_dtype, uint8_t* oq, uint8_t* os, int B, int M, int Hq, int Hkv, int D,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* mxfp4_attn_kv4_masked: mxfp4_attn_kv4 of which a token sees less.
+ *   window, sinks  token at position p sees p - window + 1 .. p and 0 .. sinks - 1
+ *                  of what mxfp4_attn_kv4 gives it.  window 0: no window, and no
+ *                  sinks.  Units of 32 positions that no token of a sequence sees are
+ *                  not read, nor are their pages looked up: they may be none
+ *   tree           device int32 (B, M, ceil(M/32)), 4-byte aligned, or NULL: token m of
+ *                  sequence b sees positions 0 .. dpos[b] - 1 and dpos[b] + i where bit
+ *                  i % 32 of tree[b][m][i / 32] is set (any i, m's own among them; bits
+ *                  from M on are without effect).  mxfp4_tree_masks makes it from a tree's
+ *                  parents.  A token that sees n of the call stands at dpos[b] + n - 1,
+ *                  from which its window counts, and a window hides none of those n:
+ *                  window >= M
+ * The workspace is mxfp4_attn_kv4_masked_workspace_size(..., window, sinks) bytes;
+ * everything else as mxfp4_attn_kv4, which is this with 0, 0, NULL.
+ */
+size_t mxfp4_attn_kv4_masked_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos, int window, int sinks);
+int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,
+                          const uint8_t* vs, const int32_t* pages, int n_pages, int page, int max_pages,
+                          const int32_t* dpos, int window, int sinks, const int32_t* tree, void* o, int o_dtype,
+                          uint8_t* oq, uint8_t* os, int B, int M, int Hq, int Hkv, int D, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------
  * Fused decode MoE layer, one launch per layer, batch 1.
  * Replaces the per-layer sequence prequant -> moe_gateup -> moe_down ->

@@ -98,12 +98,78 @@ struct Args {
     int per;                     // units of a share of one sequence, or 0: as share_units finds from its length
     int B, M, Hq, G, shares, records;   // shares of the batch, and records a row may have (its stride)
     float scale;                 // log2(e) / sqrt(D)
+    // Of the kernels with masks (MASKED) alone
+    int window, sinks;           // a token sees the last `window` positions up to its own (0: all), and the first `sinks`
+    const uint32_t* tree;        // or null: (B, M, words), bit i of a token's words: it sees the call's i-th
+    int words;
 };
 
 // Units of a sequence whose first token is at base.
 __device__ __forceinline__ uint32_t units_of(const Args& a, int base) {
     const int64_t n = (int64_t)base + a.M;
     return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
+}
+
+// Masks.  With a window the units between the sinks and the first position that any
+// token's window reaches are no work: a sequence's units are counted without them (unit
+// v stands for v, or v + gap past the sinks), here, in the shares, and in the merge.
+struct Units {
+    uint32_t n, sinks, gap;
+    __device__ __forceinline__ uint32_t real(uint32_t v) const { return v < sinks ? v : v + gap; }
+    __device__ __forceinline__ uint32_t of_real(uint32_t u) const { return u < sinks ? u : u < sinks + gap ? sinks : u - gap; }
+};
+// A token's window begins at its own position's, which with a tree is its place in its
+// line: base + (what it sees of the call) - 1.  The first and the last begin of tokens
+// t0 .. t1 (with a tree of any; a token that sees none of the call is taken to stand at base - 1).
+__device__ __forceinline__ int clamp_pos(const Args& a, int64_t pos) { return (int)(pos < 0 ? 0 : pos < a.c.max_pos ? pos : a.c.max_pos); }
+__device__ __forceinline__ int first_begin(const Args& a, int base, int t0) {
+    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? 0 : t0 + 1)) : 0;
+}
+__device__ __forceinline__ int last_begin(const Args& a, int base, int t1) {
+    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? a.M : t1 + 1)) : 0;
+}
+template <bool MASKED>
+__device__ __forceinline__ Units units(const Args& a, int base) {
+    Units u{units_of(a, base), 0, 0};
+    if constexpr (MASKED) {
+        if (a.window) {
+            const uint32_t from = min((uint32_t)first_begin(a, base, 0) / kUnit, u.n);
+            u.sinks = min((uint32_t)(a.sinks + kUnit - 1) / kUnit, u.n);
+            u.gap = from > u.sinks ? from - u.sinks : 0;
+            u.n -= u.gap;
+        }
+    }
+    return u;
+}
+// The last position that token t sees, if it is in the cache.
+template <bool MASKED>
+__device__ __forceinline__ int64_t last_seen(const Args& a, int base, int t) {
+    if constexpr (MASKED) {
+        if (a.tree) return min((int64_t)base + a.M, (int64_t)a.c.max_pos) - 1;
+    }
+    return (int64_t)base + t;
+}
+// Words of token t of sequence b, and how many of the call it sees.
+__device__ __forceinline__ const uint32_t* tree_row(const Args& a, int b, int t) { return a.tree + ((int64_t)b * a.M + t) * a.words; }
+__device__ __forceinline__ int tree_count(const Args& a, int b, int t) {
+    const uint32_t* w = tree_row(a, b, t);
+    int n = 0;
+    for (int i = 0; i < a.words; ++i) n += __builtin_popcount(32 * i + 32 <= a.M ? w[i] : w[i] & ((1u << (a.M & 31)) - 1));
+    return n;
+}
+// Which of positions p0 .. p0 + 31 token t sees of those up to the call's last: bit j.
+__device__ __forceinline__ uint32_t tree_bits(const Args& a, int b, int base, int t, int p0) {
+    const int64_t d = (int64_t)p0 - base;          // p0 is the call's d-th
+    if (d <= -32) return ~0u;
+    const uint32_t* w = tree_row(a, b, t);
+    if (d < 0) return (w[0] << (int)-d) | ((1u << (int)-d) - 1);
+    const int64_t i = d >> 5;
+    const uint32_t lo = i < a.words ? w[i] : 0u, hi = i + 1 < a.words ? w[i + 1] : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, (uint32_t)d & 31u);
+}
+// Where token t's window begins.
+__device__ __forceinline__ int begin_of(const Args& a, int b, int base, int t) {
+    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? tree_count(a, b, t) : t + 1)) : 0;
 }
 // Inclusive prefix sums over the wave (every lane active).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
@@ -138,13 +204,14 @@ struct Place {
     uint64_t start;
 };
 // Share blockIdx.x's first sequence; false: it is past the line.
+template <bool MASKED>
 __device__ __forceinline__ bool find_share(const Args& a, Place& p) {
     const int lane = threadIdx.x & 63;
     auto places = [&](int b0, int& base) {
         base = 0;
         if (b0 + lane >= a.B) return 0u;
         base = a.dpos[b0 + lane];
-        const uint32_t n = units_of(a, base);
+        const uint32_t n = units<MASKED>(a, base).n;
         return n ? n + kPad : 0u;
     };
     int base;
@@ -193,7 +260,7 @@ enum class Work {
     kLine,       // a share of the line
 };
 // Its sequences in turn: segment(b, its dpos, its units u0 .. u1 - 1).
-template <Work W, class Segment>
+template <Work W, bool MASKED, class Segment>
 __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
     if constexpr (W == Work::kSequence) {
         segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
@@ -202,18 +269,18 @@ __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
     if constexpr (W == Work::kShare) {      // (a kernel of its own: nine tokens over 23001 positions 25.1 us, in the loop 25.8)
         const int base = a.dpos[0];         // (in flight, where nothing here needs it)
         uint32_t per = a.per;
-        if (per == 0) per = share_units(units_of(a, __builtin_amdgcn_readfirstlane(base)), a);
+        if (per == 0) per = share_units(units<MASKED>(a, __builtin_amdgcn_readfirstlane(base)).n, a);
         if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.places[0] = make_int4(0, 0, (int)per, 0);
         const uint32_t u0 = blockIdx.x * per;
         segment(0, base, (int)u0, (int)(u0 + per));
         return;
     }
     Place p;
-    if (!find_share(a, p)) return;             // uniform
+    if (!find_share<MASKED>(a, p)) return;             // uniform
     const uint64_t from = (uint64_t)blockIdx.x * p.per;
     constexpr int pad = kPad;
     for (bool first = true;;) {
-        const int n = (int)units_of(a, p.base);
+        const int n = (int)units<MASKED>(a, p.base).n;
         // the share's beginning and end in units of the sequence, which ends past `from` (per < 2^28)
         const int u1 = (int)min((int64_t)n, (int64_t)(from + p.per - p.start) - pad);
         const int u0 = (int)max((int64_t)0, (int64_t)from - (int64_t)p.start - pad);
@@ -375,15 +442,46 @@ __device__ __forceinline__ void mark_not_finite(const Args& a, int b, int base, 
     }
 }
 
+// The same with masks: unit_at(k) is the k-th unit of the workgroup, of n; the wave has
+// every NW-th.  some_hide(first position): not all of the workgroup's rows see all of it.
+template <int D, int NW, class UnitAt, class SomeHide>
+__device__ __forceinline__ void mark_not_finite_masked(const Args& a, int b, int base, int g, int r0, int rows, int wave, int n, int last,
+                                                       UnitAt unit_at, SomeHide some_hide, float (*mo)[D + 4]) {
+    asm volatile("" ::: "memory");
+    for (int k = wave; k < n; k += NW) {
+        const int p0 = unit_at(k) * kUnit;
+        if (!some_hide(p0)) continue;
+        for (int pos = p0; pos < p0 + kUnit && pos <= last; ++pos) {
+            const int64_t row = kv4::head_row(a.c, b, g, pos);
+            if (row < 0) continue;
+            for (int col = threadIdx.x & 63; col < D; col += 64) {
+                const uint32_t w = a.c.vq[row * (D / 2) + col / 2] >> (4 * (col & 1));
+                if (!(kv4::not_finite(w, a.c.vs[row * (D / 32) + col / 32]) & 1)) continue;
+                for (int r = 0; r < rows; ++r) {
+                    const int t = (r0 + r) / a.G;
+                    const bool sees = pos <= last_seen<true>(a, base, t) && (pos >= begin_of(a, b, base, t) || pos < a.sinks) &&
+                                      (!a.tree || tree_bits(a, b, base, t, pos) & 1);
+                    if (sees) mo[r][col] = __builtin_nanf("");
+                }
+            }
+        }
+    }
+}
+
 // The end of row r of kv head g of sequence b, a segment from unit u0 on: NW waves' (m, l,
 // columns) to one record, or with ONE the output.  16 neighbouring lanes a row (by
 // tid), which all call it, D / 16 columns a lane.
-template <int D, int NW, bool ONE, class M, class L, class O>
+template <int D, int NW, bool ONE, bool MASKED, class M, class L, class O>
 __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
     constexpr int CT = D / 16;
     const int c0 = CT * (tid & 15);
     const int64_t pos = (int64_t)base + r / a.G;
-    if (!ONE && (pos < 0 || pos >= a.c.max_pos || (int64_t)u0 * kUnit > pos)) return;   // no record: the merge reads none
+    if (!ONE && (pos < 0 || pos >= a.c.max_pos)) return;                      // no record: the merge reads none
+    if constexpr (!ONE && MASKED) {
+        if ((uint32_t)u0 > units<true>(a, base).of_real((uint32_t)last_seen<true>(a, base, r / a.G) / kUnit)) return;
+    } else if (!ONE) {
+        if ((int64_t)u0 * kUnit > pos) return;
+    }
     float gm = m_of(0);
 #pragma unroll
     for (int w = 1; w < NW; ++w) gm = fmaxf(gm, m_of(w));
@@ -417,8 +515,20 @@ __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, 
     }
 }
 
-// More than 16 query rows of a kv head (attn_kv4_rows.hip), in groups of 32; exact: p in
-// three bf16 parts instead of two.
-int attn_rows(const Args& a, int q_dtype, int groups, int D, bool one, bool exact, hipStream_t st);
+// How a call's work is laid out (attn_kv4.hip).
+struct Plan {
+    bool many;       // rows for attn_rows
+    int groups, shares, most;   // shares of the batch (with `one` a sequence each), and one sequence may have
+    int records;     // of a row
+    int waves;       // of a workgroup
+    bool one;
+};
+
+// Up to 16 query rows of a kv head (attn_kv4_few.h); much: K by streaming loads.  And more (attn_kv4_rows.h), in groups of
+// 32; exact: p in three bf16 parts instead of two.  Without masks, and with.
+int attn_few(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
+int attn_few_masked(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
+int attn_rows(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
+int attn_rows_masked(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
 
 }  // namespace mxa

@@ -20,6 +20,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -365,8 +366,32 @@ std::vector<torch::Tensor> kv4_read(const torch::Tensor& kq, const torch::Tensor
     return {k, v};
 }
 
+// What its tokens see of the cache: a window (0: all) with sinks, and the words of a tree or null.
+struct Masks {
+    int window, sinks;
+    const int32_t* tree;
+};
+Masks kv4_masks(const torch::Tensor& q, const c10::optional<int64_t>& window, int64_t sinks, const c10::optional<torch::Tensor>& tree) {
+    Masks m{0, 0, nullptr};
+    if (window.has_value()) {
+        require(*window > 0, "window must be positive");
+        m.window = (int)std::min<int64_t>(*window, 0x7FFFFFFF);
+    }
+    require(sinks >= 0, "sinks must not be negative");
+    require(sinks == 0 || window.has_value(), "sinks need a window");
+    m.sinks = (int)std::min<int64_t>(sinks, 0x7FFFFFFF);
+    if (tree.has_value()) {
+        require(tree->scalar_type() == torch::kInt32 && tree->dim() == 3 && tree->is_contiguous() && tree->device() == q.device() &&
+                    tree->size(0) == q.size(0) && tree->size(1) == q.size(1) && tree->size(2) == (q.size(1) + 31) / 32,
+                "tree must be a contiguous int32 (B,M,ceil(M/32)) tensor on the cache's device");
+        m.tree = static_cast<const int32_t*>(tree->data_ptr());
+        require(m.window == 0 || m.window >= q.size(1), "a tree needs a window of M at least");
+    }
+    return m;
+}
+
 // The attention of q (B,M,Hq,D) over the cache into o and / or oq, os (undefined: not wanted).
-void kv4_attn_into(const torch::Tensor& q, const Kv4& c, const torch::Tensor& kq, const torch::Tensor& o,
+void kv4_attn_into(const torch::Tensor& q, const Kv4& c, const Masks& mk, const torch::Tensor& kq, const torch::Tensor& o,
                    const torch::Tensor& oq, const torch::Tensor& os) {
     const int M = (int)q.size(1), Hq = (int)q.size(2);
     const torch::Tensor qc0 = token_rows(q);
@@ -374,14 +399,14 @@ void kv4_attn_into(const torch::Tensor& q, const Kv4& c, const torch::Tensor& kq
     const torch::Tensor qc = aligned ? qc0 : qc0.clone(at::MemoryFormat::Contiguous);
     const int64_t max_pos = c.pages ? (int64_t)c.max_pages * c.page : c.page;
     require(max_pos <= (1ll << 30), "attn_decode4: more than 2^30 positions a sequence");
-    const size_t wsb = mxfp4_attn_kv4_workspace_size(c.B, M, Hq, c.Hkv, c.D, (int)max_pos);
+    const size_t wsb = mxfp4_attn_kv4_masked_workspace_size(c.B, M, Hq, c.Hkv, c.D, (int)max_pos, mk.window, mk.sinks);
     torch::Tensor ws;
     if (wsb) ws = empty_on(kq, {(int64_t)wsb}, torch::kUInt8);
-    check(mxfp4_attn_kv4(qc.data_ptr(), dtype_code(qc.scalar_type()), token_stride(qc), c.kq, c.ks, c.vq, c.vs, c.pages,
-                         c.n_pages, c.page, c.max_pages, c.at, o.defined() ? o.data_ptr() : nullptr,
-                         o.defined() ? dtype_code(o.scalar_type()) : 2, oq.defined() ? u8m(oq) : nullptr,
-                         os.defined() ? u8m(os) : nullptr, c.B, M, Hq, c.Hkv, c.D, wsb ? ws.data_ptr() : nullptr, wsb,
-                         stream_of(kq)),
+    check(mxfp4_attn_kv4_masked(qc.data_ptr(), dtype_code(qc.scalar_type()), token_stride(qc), c.kq, c.ks, c.vq, c.vs, c.pages,
+                                c.n_pages, c.page, c.max_pages, c.at, mk.window, mk.sinks, mk.tree,
+                                o.defined() ? o.data_ptr() : nullptr, o.defined() ? dtype_code(o.scalar_type()) : 2,
+                                oq.defined() ? u8m(oq) : nullptr, os.defined() ? u8m(os) : nullptr, c.B, M, Hq, c.Hkv, c.D,
+                                wsb ? ws.data_ptr() : nullptr, wsb, stream_of(kq)),
           "attn_decode4");
 }
 
@@ -398,24 +423,28 @@ Kv4 kv4_attn_args(const torch::Tensor& q, const torch::Tensor& kq, const torch::
 
 torch::Tensor kv4_attn(const torch::Tensor& q, const torch::Tensor& kq, const torch::Tensor& ks, const torch::Tensor& vq,
                        const torch::Tensor& vs, const torch::Tensor& dpos, const c10::optional<torch::Tensor>& pages,
-                       const py::object& dtype) {
+                       const py::object& dtype, const c10::optional<int64_t>& window, int64_t sinks,
+                       const c10::optional<torch::Tensor>& tree) {
     const Kv4 c = kv4_attn_args(q, kq, ks, vq, vs, dpos, pages);
+    const Masks mk = kv4_masks(q, window, sinks, tree);
     const auto dt = torch::python::detail::py_object_to_dtype(dtype);
     require(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32, "dtype must be bfloat16, float16 or float32");
     const c10::DeviceGuard guard(kq.device());
     auto o = empty_on(q, q.sizes(), dt);
-    if (o.numel() != 0) kv4_attn_into(q, c, kq, o, torch::Tensor(), torch::Tensor());
+    if (o.numel() != 0) kv4_attn_into(q, c, mk, kq, o, torch::Tensor(), torch::Tensor());
     return o;
 }
 
 std::vector<torch::Tensor> kv4_attn_mx(const torch::Tensor& q, const torch::Tensor& kq, const torch::Tensor& ks,
                                        const torch::Tensor& vq, const torch::Tensor& vs, const torch::Tensor& dpos,
-                                       const c10::optional<torch::Tensor>& pages) {
+                                       const c10::optional<torch::Tensor>& pages, const c10::optional<int64_t>& window,
+                                       int64_t sinks, const c10::optional<torch::Tensor>& tree) {
     const Kv4 c = kv4_attn_args(q, kq, ks, vq, vs, dpos, pages);
+    const Masks mk = kv4_masks(q, window, sinks, tree);
     const c10::DeviceGuard guard(kq.device());
     const int64_t T = q.size(0) * q.size(1), row = q.size(2) * q.size(3);
     auto oq = empty_on(kq, {T, row / 2}, torch::kUInt8), os = empty_on(kq, {T, row / 32}, torch::kUInt8);
-    if (T != 0) kv4_attn_into(q, c, kq, torch::Tensor(), oq, os);
+    if (T != 0) kv4_attn_into(q, c, mk, kq, torch::Tensor(), oq, os);
     return {oq, os};
 }
 
@@ -443,7 +472,8 @@ PYBIND11_MODULE(mxfp4_ext, m) {
     k4.def("read", &kv4_read, py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("n"), py::arg("start"),
            py::arg("pages"), py::arg("dtype"), "positions start[b] .. start[b]+n-1 -> [k, v] (B,n,Hkv,D)");
     k4.def("attn", &kv4_attn, py::arg("q"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("dpos"),
-           py::arg("pages"), py::arg("dtype"), "attention over the MXFP4 cache -> (B,M,Hq,D)");
+           py::arg("pages"), py::arg("dtype"), py::arg("window"), py::arg("sinks"), py::arg("tree"),
+           "attention over the MXFP4 cache -> (B,M,Hq,D)");
     k4.def("attn_mx", &kv4_attn_mx, py::arg("q"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("dpos"),
-           py::arg("pages"), "attn as the MXFP4 rows of its bf16 rounding -> [oq, os]");
+           py::arg("pages"), py::arg("window"), py::arg("sinks"), py::arg("tree"), "attn as the MXFP4 rows of its bf16 rounding -> [oq, os]");
 }

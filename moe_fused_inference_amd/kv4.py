@@ -67,18 +67,24 @@ def kv4_read(cache, n, start=None, pages=None, dtype=torch.bfloat16):
     return k, v
 
 
-def attn_decode4(q, cache, dpos, pages=None, dtype=torch.float32):
+def attn_decode4(q, cache, dpos, pages=None, dtype=torch.float32, window=None, sinks=0, tree=None):
     """softmax(q K^T / sqrt(D)) V of q (B, M, Hq, D) bf16 or fp16, token m of
     sequence b over positions 0 .. dpos[b] + m -> (B, M, Hq, D) of dtype fp32,
     bf16 or fp16.  Zeros for tokens outside the cache and for ones that see no
-    position."""
+    position.
+
+    window: of those positions a token sees the last `window`, its own among them,
+    and the first `sinks`.  Pages whose positions no token sees may be gone.
+    tree: the M tokens are drafts that form a tree, and one sees positions
+    0 .. dpos[b] - 1 and of the drafts those in its mask (``tree_masks``, int32
+    (B, M, ceil(M / 32))); its window, M at least, counts from its place in its line."""
     kq, ks, vq, vs = cache
-    return _ext().attn(q, kq, ks, vq, vs, dpos, pages, dtype)
+    return _ext().attn(q, kq, ks, vq, vs, dpos, pages, dtype, window, sinks, tree)
 
 
-def attn_decode4_mx(q, cache, dpos, pages=None):
+def attn_decode4_mx(q, cache, dpos, pages=None, window=None, sinks=0, tree=None):
     """attn_decode4 as the MXFP4 rows of its bf16 rounding, the activations of an
     o_proj ``lin_pq``: (oq uint8 (B*M, Hq*D/2), os uint8 (B*M, Hq*D/32))."""
     kq, ks, vq, vs = cache
-    oq, os_ = _ext().attn_mx(q, kq, ks, vq, vs, dpos, pages)
+    oq, os_ = _ext().attn_mx(q, kq, ks, vq, vs, dpos, pages, window, sinks, tree)
     return oq, os_
