@@ -320,6 +320,63 @@ int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, const uint8_t
                           uint8_t* oq, uint8_t* os, int B, int M, int Hq, int Hkv, int D, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* mxfp4_kv4_write_slots: mxfp4_kv4_write of T tokens, token t at slots[t] (device
+ * int64), the place page * (rows of a page) + row of the pool; others, -1 among them,
+ * write nothing.  page: any multiple of 16. */
+int mxfp4_kv4_write_slots(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq, uint8_t* ks,
+                          uint8_t* vq, uint8_t* vs, int n_pages, int page, const int64_t* slots, int T, int Hkv, int D,
+                          void* stream);
+
+/* mxfp4_tree_masks: the masks of mxfp4_attn_kv4_masked from a tree's parents.
+ * parents: device int32 (B, M), draft m's an earlier one (0 .. m - 1) or -1, no draft
+ * of the call (it follows the context); with any other it is no draft, nor are its
+ * children.  tree (B, M, ceil(M/32)): itself and its ancestors; depth (B, M): how many
+ * ancestors, so it stands at position dpos[b] + depth; no draft: no bits, and -1.
+ * M up to 4096, B up to 65535. */
+int mxfp4_tree_masks(const int32_t* parents, int32_t* tree, int32_t* depth, int B, int M, void* stream);
+
+/* mxfp4_kv4_keep: the accepted drafts' rows move together.  For k = 0, 1, .. up to
+ * A - 1 or the first negative path[b][k] (device int32 (B, A)), position dpos[b] +
+ * path[b][k] goes to position dpos[b] + k, keys and values of every kv head, in every
+ * one of n_layers caches of one shape (kq, ks, vq, vs: host arrays of their device
+ * pointers); all are read before any is written.  path[b][k] = k stays where it is, and
+ * so does one below k (a path runs forward), one past the cache or on no page, or whose
+ * goal is.  Pages that a table names twice, where they are written, hold a mixture. */
+int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* const* vq, uint8_t* const* vs, int n_layers,
+                   const int32_t* pages, int n_pages, int page, int max_pages, const int32_t* dpos, const int32_t* path,
+                   int B, int A, int Hkv, int D, void* stream);
+
+/* mxfp4_kv4_tables: the page table of a batch from its sequences' lengths, and the
+ * places of their newest tokens, all on the device.
+ *   pages          int32 (B, max_pages), in place: the table of the kv4 entries
+ *   span           int32 (B, 2), 8-byte aligned, in place: sequence b has the pages of
+ *                  [span[b][0], span[b][1]) of its row, and of the sinks those below
+ *                  span[b][1]; zeros for a batch without pages
+ *   free, state    int32 (n_pages), in place: state[0] free pages, the last of which is
+ *                  taken first; state int32 (2), 8-byte aligned: that count, and how many
+ *                  pages this call lacked
+ *   lens           int32 (B): positions that a sequence needs room for; 0 (or less): it
+ *                  has ended and gives all its pages back
+ *   news, starts   int32 (B) or NULL: of these the last news[b] are new tokens; int32
+ *                  (B + 1): how many there are before each sequence's and in all (2^30 at
+ *                  most)
+ *   slots, seq, pos  int64, int32, int32 (T): the tokens, sequence after sequence: their
+ *                  place page * pages[b][p / page] + p % page (-1: none), b and p; from
+ *                  starts[B] on -1.  T = 0: may be NULL
+ *   window, sinks  of the attention (mxfp4_attn_kv4_masked), the same in every call: pages
+ *                  that no window from the first new token on (without new ones: the next)
+ *                  reaches go back too, and once gone they stay gone.  0, 0: none
+ * First the pages that are no longer needed go back, the r-th of R to place count + R -
+ * 1 - r, then those that are needed are taken, both in the table's order; where there
+ * are too few the first get them, and the same lengths ask for the others again.  So a
+ * call and one with the lengths before it leave all as it was.  What grows by new
+ * tokens that are then rejected is taken back by the shorter lengths.
+ * page a power of two from 16 on, B up to 4096, max_pages * page up to 2^30.
+ */
+int mxfp4_kv4_tables(int32_t* pages, int32_t* span, int32_t* free, int32_t* state, const int32_t* lens,
+                     const int32_t* news, int window, int sinks, int B, int max_pages, int n_pages, int page,
+                     int32_t* starts, int64_t* slots, int32_t* seq, int32_t* pos, int T, void* stream);
+
 /* ---------------------------------------------------------------------
  * Fused decode MoE layer, one launch per layer, batch 1.
  * Replaces the per-layer sequence prequant -> moe_gateup -> moe_down ->

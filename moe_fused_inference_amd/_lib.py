@@ -90,6 +90,12 @@ SIGNATURES = {
     "mxfp4_attn_kv4_masked_workspace_size": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
     "mxfp4_attn_kv4_masked": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_p, _c_i, _c_i, _c_p,
                                      _c_p, _c_i, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_sz, _c_p]),
+    "mxfp4_kv4_write_slots": (_c_i, [_c_p, _c_p, _c_i, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i,
+                                     _c_p]),
+    "mxfp4_tree_masks": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i, _c_p]),
+    "mxfp4_kv4_keep": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_p]),
+    "mxfp4_kv4_tables": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p,
+                                _c_i, _c_p]),
     "mxfp4_moe_group": (_c_i, [_c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p]),
     "mxfp4_route_topk": (_c_i, [_c_p, _c_i64, _c_i, _c_i, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p]),
     "mxfp4_route_tables": (_c_i, [_c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i,

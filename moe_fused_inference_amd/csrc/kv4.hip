@@ -2,7 +2,8 @@
 //
 //   kv4_write_kernel    k, v rows (bf16, fp16 or fp32) -> MXFP4 at positions
 //                       dpos[b] + m: per 32-block the library's quantizer
-//                       (quant_rows.h), eight values a lane, a block a quad.
+//                       (quant_rows.h), eight values a lane, a block a quad; or at
+//                       the places of a list (slots), a token each.
 //   qk_rope_kv4_kernel  the decode step's form: q / k head RMSNorm and RoPE of
 //                       the fp32 projections (head_rope.h), q out as bf16, k
 //                       and bf16(v) to the cache.
@@ -30,22 +31,33 @@ __device__ __forceinline__ int64_t row_of(const Cache& c, const int32_t* at, int
     return kv4::head_row(c, b, g, (int)pos);
 }
 
+// The row of head g at a place of the pool, page * (rows of a page) + row, or -1.
+__device__ __forceinline__ int64_t row_of_slot(const Cache& c, int64_t slot, int g) {
+    if (slot < 0 || slot >= (int64_t)c.n_pages * c.page) return -1;       // (what is left has 32 bits)
+    const uint32_t pid = (uint32_t)slot / (uint32_t)c.page;
+    return ((int64_t)pid * c.Hkv + g) * c.page + ((uint32_t)slot - pid * (uint32_t)c.page);
+}
+
 // Thread: eight consecutive values of a head row of k and of v; LU = log2(D / 8).
-template <int SRC, int LU>
+// SLOTS: the tokens' places, and M = 1; else dpos.
+template <int SRC, int LU, bool SLOTS>
 __global__ __launch_bounds__(256) void kv4_write_kernel(const void* __restrict__ k, const void* __restrict__ v,
                                                         int64_t ldk, int64_t ldv, int vec, Cache c,
-                                                        const int32_t* __restrict__ dpos, int M, int64_t heads) {
+                                                        const int32_t* __restrict__ dpos, const int64_t* __restrict__ slots, int M,
+                                                        int64_t heads) {
     constexpr int D = 8 << LU;
     const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t th = idx >> LU;             // token * Hkv + head
     if (th >= heads) return;                  // whole quads: heads << LU is a multiple of 8
     const int u = (int)idx & ((1 << LU) - 1);
     const int tok = (int)((uint32_t)th / (uint32_t)c.Hkv), g = (int)th - tok * c.Hkv;
-    const int b = (int)((uint32_t)tok / (uint32_t)M), m = tok - b * M;
+    const int b = SLOTS ? 0 : (int)((uint32_t)tok / (uint32_t)M), m = tok - b * M;
     float kv[8], vv[8];
     mxq::load8<SRC>(k, (int64_t)tok * ldk + g * D, 8 * u, D, vec & 1, kv);
     mxq::load8<SRC>(v, (int64_t)tok * ldv + g * D, 8 * u, D, vec & 2, vv);
-    const int64_t row = row_of(c, dpos, b, m, g);
+    int64_t row;
+    if constexpr (SLOTS) row = row_of_slot(c, slots[tok], g);
+    else row = row_of(c, dpos, b, m, g);
     uint32_t kc, vc;
     const uint32_t kp = mxq::quantize8<SRC, 0>(kv, kc), vp = mxq::quantize8<SRC, 0>(vv, vc);
     if (row < 0) return;
@@ -168,6 +180,37 @@ unsigned grid_of(int64_t heads, int D) {
 
 }  // namespace
 
+namespace {
+
+// kv4_write's checks of k and v, and its launch: B * M tokens.
+template <bool SLOTS>
+int write_rows(const char* what, const Cache& c, const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv,
+               const int32_t* dpos, const int64_t* slots, int64_t tokens, int M, int D, hipStream_t st) {
+    MXH_REQUIRE(src_dtype >= MXFP4_DT_BF16 && src_dtype <= MXFP4_DT_F32, "%s: bad dtype %d", what, src_dtype);
+    MXH_REQUIRE(ldk >= (int64_t)c.Hkv * D && ldv >= (int64_t)c.Hkv * D, "%s: token stride below Hkv*D=%lld", what,
+                (long long)c.Hkv * D);
+    const int64_t heads = tokens * c.Hkv;
+    const unsigned grid = grid_of(heads, D);
+    MXH_REQUIRE(grid > 0, "%s: %lld head rows: too large", what, (long long)heads);
+    const int esz = src_dtype == MXFP4_DT_F32 ? 4 : 2;
+    auto wide = [&](const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld * esz % 16 == 0; };
+    const int vec = (wide(k, ldk) ? 1 : 0) | (wide(v, ldv) ? 2 : 0);
+#define MXH_KV4W(SRC)                                                                                                            \
+    if (D == 64)                                                                                                                 \
+        hipLaunchKernelGGL((kv4_write_kernel<SRC, 3, SLOTS>), dim3(grid), dim3(256), 0, st, k, v, ldk, ldv, vec, c, dpos, slots, M, heads); \
+    else                                                                                                                         \
+        hipLaunchKernelGGL((kv4_write_kernel<SRC, 4, SLOTS>), dim3(grid), dim3(256), 0, st, k, v, ldk, ldv, vec, c, dpos, slots, M, heads)
+    switch (src_dtype) {
+        case MXFP4_DT_BF16: MXH_KV4W(MXFP4_DT_BF16); break;
+        case MXFP4_DT_F16: MXH_KV4W(MXFP4_DT_F16); break;
+        default: MXH_KV4W(MXFP4_DT_F32); break;
+    }
+#undef MXH_KV4W
+    return mxh::launch_status(what);
+}
+
+}  // namespace
+
 extern "C" int mxfp4_kv4_write(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq, uint8_t* ks,
                                uint8_t* vq, uint8_t* vs, const int32_t* pages, int n_pages, int page, int max_pages,
                                const int32_t* dpos, int B, int M, int Hkv, int D, void* stream) {
@@ -175,27 +218,19 @@ extern "C" int mxfp4_kv4_write(const void* k, const void* v, int src_dtype, int6
     const int rc = kv4::make_cache(c, "kv4_write", kq, ks, vq, vs, pages, n_pages, page, max_pages, B, Hkv, D);
     if (rc != MXFP4_OK) return rc;
     MXH_REQUIRE(k && v && dpos, "kv4_write: null pointer");
-    MXH_REQUIRE(src_dtype >= MXFP4_DT_BF16 && src_dtype <= MXFP4_DT_F32, "kv4_write: bad dtype %d", src_dtype);
     MXH_REQUIRE(M > 0, "kv4_write: M=%d", M);
-    MXH_REQUIRE(ldk >= (int64_t)Hkv * D && ldv >= (int64_t)Hkv * D, "kv4_write: token stride below Hkv*D=%lld",
-                (long long)Hkv * D);
-    const int64_t heads = (int64_t)B * M * Hkv;
-    const unsigned grid = grid_of(heads, D);
-    MXH_REQUIRE(grid > 0, "kv4_write: B*M*Hkv=%lld too large", (long long)heads);
-    const int esz = src_dtype == MXFP4_DT_F32 ? 4 : 2;
-    auto wide = [&](const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld * esz % 16 == 0; };
-    const int vec = (wide(k, ldk) ? 1 : 0) | (wide(v, ldv) ? 2 : 0);
-    const hipStream_t st = mxh::as_stream(stream);
-#define MXH_KV4W(SRC)                                                                                                       \
-    if (D == 64) hipLaunchKernelGGL((kv4_write_kernel<SRC, 3>), dim3(grid), dim3(256), 0, st, k, v, ldk, ldv, vec, c, dpos, M, heads); \
-    else hipLaunchKernelGGL((kv4_write_kernel<SRC, 4>), dim3(grid), dim3(256), 0, st, k, v, ldk, ldv, vec, c, dpos, M, heads)
-    switch (src_dtype) {
-        case MXFP4_DT_BF16: MXH_KV4W(MXFP4_DT_BF16); break;
-        case MXFP4_DT_F16: MXH_KV4W(MXFP4_DT_F16); break;
-        default: MXH_KV4W(MXFP4_DT_F32); break;
-    }
-#undef MXH_KV4W
-    return mxh::launch_status("kv4_write");
+    return write_rows<false>("kv4_write", c, k, v, src_dtype, ldk, ldv, dpos, nullptr, (int64_t)B * M, M, D, mxh::as_stream(stream));
+}
+
+extern "C" int mxfp4_kv4_write_slots(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq,
+                                     uint8_t* ks, uint8_t* vq, uint8_t* vs, int n_pages, int page, const int64_t* slots, int T,
+                                     int Hkv, int D, void* stream) {
+    Cache c;
+    const int rc = kv4::make_cache(c, "kv4_write_slots", kq, ks, vq, vs, nullptr, n_pages, page, 0, 1, Hkv, D);
+    if (rc != MXFP4_OK) return rc;
+    MXH_REQUIRE(k && v && slots, "kv4_write_slots: null pointer");
+    MXH_REQUIRE(T > 0, "kv4_write_slots: T=%d", T);
+    return write_rows<true>("kv4_write_slots", c, k, v, src_dtype, ldk, ldv, nullptr, slots, T, 1, D, mxh::as_stream(stream));
 }
 
 extern "C" int mxfp4_kv4_read(const uint8_t* kq, const uint8_t* ks, const uint8_t* vq, const uint8_t* vs, const int32_t* pages,

@@ -7,7 +7,7 @@
 //              prequant, lin_pq, moe_gateup, moe_down, moe_combine,
 //              moe_gateup_tab, moe_down_tab, attn_decode, kv_write
 // and a third of this library's own:
-//   kv4     -- the MXFP4 KV cache: write, read, attn, attn_mx (kv4.py)
+//   kv4     -- the MXFP4 KV cache: write, read, attn, attn_mx, write_slots, tree_masks, keep, tables (kv4.py)
 // Names, argument order and meaning, output shapes and dtypes, and the
 // argument-check messages are the reference's.  Each op is a thin shim:
 // checks, torch allocations on the input's device (caching allocator), then
@@ -448,6 +448,114 @@ std::vector<torch::Tensor> kv4_attn_mx(const torch::Tensor& q, const torch::Tens
     return {oq, os};
 }
 
+// k, v (T,Hkv,D) -> the pool's rows at slots (T) int64.
+void kv4_write_slots(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& kq, const torch::Tensor& ks,
+                     const torch::Tensor& vq, const torch::Tensor& vs, const torch::Tensor& slots) {
+    const Kv4 c = kv4_cache(kq, ks, vq, vs, c10::nullopt, c10::nullopt, "");
+    require(k.device() == kq.device() && v.device() == kq.device(), "k/v must be on the cache's device");
+    require((is_float16s(k) || k.scalar_type() == torch::kFloat32) && v.scalar_type() == k.scalar_type(),
+            "k/v must be bfloat16, float16 or float32, both of one type");
+    require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == c.Hkv && k.size(2) == c.D, "k/v must be (T,Hkv,D)");
+    require(slots.scalar_type() == torch::kInt64 && slots.is_contiguous() && slots.device() == kq.device() && slots.dim() == 1 &&
+                slots.numel() == k.size(0),
+            "slots must be a contiguous int64 (T,) tensor on the cache's device");
+    const int T = as_int(k.size(0), "too many tokens");
+    if (T == 0) return;
+    const c10::DeviceGuard guard(kq.device());
+    const torch::Tensor kc = token_rows(k.unsqueeze(0)), vc = token_rows(v.unsqueeze(0));
+    check(mxfp4_kv4_write_slots(kc.data_ptr(), vc.data_ptr(), dtype_code(kc.scalar_type()), token_stride(kc), token_stride(vc), c.kq,
+                                c.ks, c.vq, c.vs, c.n_pages, c.page, static_cast<const int64_t*>(slots.data_ptr()), T, c.Hkv, c.D,
+                                stream_of(kq)),
+          "kv4_write_slots");
+}
+
+bool is_i32(const torch::Tensor& t, int64_t dim) { return t.scalar_type() == torch::kInt32 && t.dim() == dim && t.is_contiguous(); }
+int32_t* i32m(const torch::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// parents (B,M) -> [tree (B,M,ceil(M/32)), depth (B,M)].
+std::vector<torch::Tensor> kv4_tree_masks(const torch::Tensor& parents) {
+    require(is_i32(parents, 2), "parents must be a contiguous int32 (B,M) tensor");
+    require(parents.is_cuda(), "parents must be cuda");
+    const int B = as_int(parents.size(0), "too many sequences"), M = as_int(parents.size(1), "too many drafts");
+    const c10::DeviceGuard guard(parents.device());
+    auto tree = empty_on(parents, {B, M, (M + 31) / 32}, torch::kInt32), depth = empty_on(parents, {B, M}, torch::kInt32);
+    if (B != 0 && M != 0) check(mxfp4_tree_masks(i32m(parents), i32m(tree), i32m(depth), B, M, stream_of(parents)), "tree_masks");
+    return {tree, depth};
+}
+
+// The rows dpos[b] + path[b,k] of every layer's cache -> dpos[b] + k.  caches: a list of (kq, ks, vq, vs).
+void kv4_keep(const std::vector<std::vector<torch::Tensor>>& caches, const torch::Tensor& dpos, const torch::Tensor& path,
+              const c10::optional<torch::Tensor>& pages) {
+    require(!caches.empty(), "kv4_keep needs a cache at least");
+    std::vector<uint8_t*> p[4];
+    Kv4 c{};
+    for (size_t l = 0; l < caches.size(); ++l) {
+        const auto& t = caches[l];
+        require(t.size() == 4, "a cache is four tensors");
+        const Kv4 x = kv4_cache(t[0], t[1], t[2], t[3], pages, dpos, "dpos must be a contiguous int32 (B,) tensor on the cache's device");
+        require(t[0].sizes() == caches[0][0].sizes() && t[0].device() == caches[0][0].device(), "caches must be of one shape and device");
+        if (l == 0) c = x;
+        p[0].push_back(x.kq);
+        p[1].push_back(x.ks);
+        p[2].push_back(x.vq);
+        p[3].push_back(x.vs);
+    }
+    const torch::Tensor& kq = caches[0][0];
+    require(is_i32(path, 2) && path.device() == kq.device() && path.size(0) == c.B,
+            "path must be a contiguous int32 (B,A) tensor on the cache's device");
+    const int A = as_int(path.size(1), "too many drafts");
+    if (A == 0 || c.B == 0) return;
+    const c10::DeviceGuard guard(kq.device());
+    check(mxfp4_kv4_keep(p[0].data(), p[1].data(), p[2].data(), p[3].data(), as_int((int64_t)caches.size(), "too many caches"), c.pages,
+                         c.n_pages, c.page, c.max_pages, c.at, i32m(path), c.B, A, c.Hkv, c.D, stream_of(kq)),
+          "kv4_keep");
+}
+
+// The table of a batch follows its lengths, in place; with `news` -> [slots, seq, pos (T), starts (B+1)].
+std::vector<torch::Tensor> kv4_tables(const torch::Tensor& pages, const torch::Tensor& span, const torch::Tensor& free,
+                                      const torch::Tensor& state, int64_t page_, const c10::optional<int64_t>& window, int64_t sinks,
+                                      const torch::Tensor& lens, const c10::optional<torch::Tensor>& news, int64_t T_) {
+    const auto dev = pages.device();
+    require(is_i32(pages, 2) && pages.size(1) > 0, "pages must be a contiguous int32 (B,max_pages) tensor");
+    const int B = as_int(pages.size(0), "too many sequences"), max_pages = as_int(pages.size(1), "too many pages");
+    require(is_i32(span, 2) && span.size(0) == B && span.size(1) == 2 && span.device() == dev, "span must be a contiguous int32 (B,2) tensor on the table's device");
+    require(is_i32(free, 1) && free.device() == dev, "free must be a contiguous int32 (n_pages,) tensor on the table's device");
+    require(is_i32(state, 1) && state.numel() == 2 && state.device() == dev, "state must be a contiguous int32 (2,) tensor on the table's device");
+    require(is_i32(lens, 1) && lens.numel() == B && lens.device() == dev, "lens must be a contiguous int32 (B,) tensor on the table's device");
+    if (news.has_value())
+        require(is_i32(*news, 1) && news->numel() == B && news->device() == dev, "new must be a contiguous int32 (B,) tensor on the table's device");
+    const int page = as_int(page_, "page too long"), T = as_int(T_, "T must not be negative");
+    require(T == 0 || news.has_value(), "T tokens need new");
+    if (window.has_value()) require(*window > 0, "window must be positive");
+    require(sinks >= 0 && (sinks == 0 || window.has_value()), "sinks need a window");
+    require(pages.is_cuda(), "tables must be cuda");
+    const c10::DeviceGuard guard(dev);
+    torch::Tensor slots, seq, pos, starts;
+    if (news.has_value()) {
+        slots = empty_on(pages, {T}, torch::kInt64);
+        seq = empty_on(pages, {T}, torch::kInt32);
+        pos = empty_on(pages, {T}, torch::kInt32);
+        starts = empty_on(pages, {(int64_t)B + 1}, torch::kInt32);
+    }
+    if (B == 0) {
+        if (news.has_value()) {
+            for (const auto& t : {slots, seq, pos}) t.fill_(-1);
+            starts.zero_();
+            return {slots, seq, pos, starts};
+        }
+        return {};
+    }
+    const bool some = news.has_value();
+    check(mxfp4_kv4_tables(i32m(pages), i32m(span), i32m(free), i32m(state), i32m(lens), some ? i32m(*news) : nullptr,
+                           window.has_value() ? (int)std::min<int64_t>(*window, 0x7FFFFFFF) : 0, (int)std::min<int64_t>(sinks, 0x7FFFFFFF),
+                           B, max_pages, as_int(free.numel(), "too many pages"), page, some ? i32m(starts) : nullptr,
+                           T ? static_cast<int64_t*>(slots.data_ptr()) : nullptr, T ? i32m(seq) : nullptr, T ? i32m(pos) : nullptr, T,
+                           stream_of(pages)),
+          "kv4_tables");
+    if (!some) return {};
+    return {slots, seq, pos, starts};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(mxfp4_ext, m) {
@@ -476,4 +584,8 @@ PYBIND11_MODULE(mxfp4_ext, m) {
            "attention over the MXFP4 cache -> (B,M,Hq,D)");
     k4.def("attn_mx", &kv4_attn_mx, py::arg("q"), py::arg("kq"), py::arg("ks"), py::arg("vq"), py::arg("vs"), py::arg("dpos"),
            py::arg("pages"), py::arg("window"), py::arg("sinks"), py::arg("tree"), "attn as the MXFP4 rows of its bf16 rounding -> [oq, os]");
+    k4.def("write_slots", &kv4_write_slots, "k, v (T,Hkv,D) -> MXFP4 rows at slots");
+    k4.def("tree_masks", &kv4_tree_masks, "parents (B,M) -> [tree, depth]");
+    k4.def("keep", &kv4_keep, "the accepted drafts' rows move together");
+    k4.def("tables", &kv4_tables, "a batch's page table follows its lengths -> [slots, seq, pos, starts], or nothing");
 }

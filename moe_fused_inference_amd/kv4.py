@@ -17,7 +17,7 @@ Every call checks its arguments (RuntimeError), allocates outputs and workspace
 with torch's caching allocator and queues its work on torch's current stream of
 the cache's device.
 """
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -45,6 +45,45 @@ def empty_cache(n_pages, page, Hkv, D=128, device="cuda"):
     return KV4(t(D // 2), t(D // 32), t(D // 2), t(D // 32))
 
 
+class PageTables(NamedTuple):
+    """A batch's page table over a pool, and what is left of the pool (:func:`page_tables`).  ``pages`` is what the
+    calls here take as theirs; the others are ``kv4_tables``' own.  ``state``: free pages, and how many the last
+    call lacked."""
+    pages: torch.Tensor      # int32 (B, max_pages)
+    span: torch.Tensor       # int32 (B, 2)
+    free: torch.Tensor       # int32 (n_pages)
+    state: torch.Tensor      # int32 (2)
+    page: int
+    window: Optional[int] = None
+    sinks: int = 0
+
+
+class Slots(NamedTuple):
+    """Where a call's new tokens go, sequence after sequence: the pool's rows for ``kv4_write_slots`` (-1: none),
+    each token's sequence and position (-1 past the last), and how many there are before each sequence's and in all."""
+    slots: torch.Tensor      # int64 (T)
+    seq: torch.Tensor        # int32 (T)
+    pos: torch.Tensor        # int32 (T)
+    starts: torch.Tensor     # int32 (B + 1)
+
+
+def page_tables(B, max_pages, n_pages, page, window=None, sinks=0, device="cuda"):
+    """The table of B sequences without pages, of max_pages each at most, over a pool of n_pages pages of `page`
+    positions (a power of two from 16 on), all free.  window, sinks: those of its attention, if it has them;
+    pages that no window reaches any more are then given back."""
+    if B <= 0 or max_pages <= 0 or n_pages <= 0 or page < 16 or page & (page - 1):
+        raise RuntimeError(f"a table needs sequences, pages, and a page of a power of two from 16 on, got B={B} max_pages={max_pages} "
+                           f"n_pages={n_pages} page={page}")
+    if (window is not None and window <= 0) or sinks < 0 or (sinks and window is None):
+        raise RuntimeError(f"a window is positive, and sinks need one, got window={window} sinks={sinks}")
+
+    def t(x):
+        return x.to(device=device, dtype=torch.int32).contiguous()
+
+    return PageTables(t(torch.full((B, max_pages), -1)), t(torch.zeros(B, 2)), t(torch.arange(n_pages - 1, -1, -1)),
+                      t(torch.tensor([n_pages, 0])), page, window, sinks)
+
+
 def _ext():
     return fp4_ext.load_compiled().kv4
 
@@ -56,6 +95,42 @@ def kv4_write(k, v, cache, dpos, pages=None):
     (slices of a projection) are read as they are."""
     kq, ks, vq, vs = cache
     _ext().write(k, v, kq, ks, vq, vs, dpos, pages)
+
+
+def kv4_tables(tables, lens, new=None, T=0):
+    """The page table follows the lengths (int32 (B,) on the device), in place: every sequence has the pages of its
+    first lens[b] positions after the call (those that its window still reaches), taken from the pool; what it had
+    beyond goes back, all of it where lens[b] <= 0, the end of a sequence.  Where the pool lacks pages, the first
+    sequences get them, ``state[1]`` says how many lack, and the same call asks for them again.  A call and one with
+    the lengths before it (drafts that are rejected) leave everything as it was.
+
+    new (int32 (B,)): the last new[b] positions are new tokens; -> their Slots, T places."""
+    got = _ext().tables(tables.pages, tables.span, tables.free, tables.state, tables.page, tables.window, tables.sinks, lens, new, T)
+    return Slots(*got) if got else None
+
+
+def kv4_write_slots(k, v, cache, slots):
+    """kv4_write of tokens one after another: k, v (T, Hkv, D) -> the pool's rows slots (int64 (T,), those of
+    ``kv4_tables``); tokens whose slot is none write nothing."""
+    kq, ks, vq, vs = cache
+    _ext().write_slots(k, v, kq, ks, vq, vs, slots)
+
+
+def tree_masks(parents):
+    """parents (int32 (B, M)) of trees of drafts, each an earlier draft or -1 for none (anything else: no draft, nor
+    are its children) -> (tree, depth): what ``attn_decode4`` takes, itself and its ancestors as bits, and the number
+    of ancestors (-1: no draft), so that draft m's position, for its rotation, is dpos[b] + depth[b, m]."""
+    tree, depth = _ext().tree_masks(parents)
+    return tree, depth
+
+
+def kv4_keep(caches, dpos, path, pages=None):
+    """What stays of a verified tree moves together: the rows at positions dpos[b] + path[b, k] go to dpos[b] + k, in
+    a cache or each of a list of them (a model's layers, one launch for 64).  path (int32 (B, A)): drafts in the
+    order of their line, so path[b, k] >= k (others stay where they are), -1 from its end on."""
+    if isinstance(caches[0], torch.Tensor):
+        caches = [caches]
+    _ext().keep([list(c) for c in caches], dpos, path, pages)
 
 
 def kv4_read(cache, n, start=None, pages=None, dtype=torch.bfloat16):
