@@ -18,6 +18,8 @@
 #include "attn_kv4.h"
 #include "mx_host.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int kMostSequences = 4096;
@@ -53,16 +55,23 @@ struct Move {
     __device__ __forceinline__ int take() const { return take0() + max(0, hi2 - max(w2, hi)); }
     __device__ __forceinline__ int take_at(int a) const { return a < take0() ? s1 + a : max(w2, hi) + a - take0(); }
 };
-__device__ __forceinline__ Move move_of(const Tables& t, int b) {
-    Move m;
+// What a sequence's moves come from: its range, length and new tokens.
+struct Lengths {
+    int lo, hi, len, news;
+};
+__device__ __forceinline__ Lengths lengths_of(const Tables& t, int b) {
     const int2 s = t.span[b];
-    m.hi = min(max(s.y, 0), t.max_pages);
-    m.lo = min(max(s.x, 0), m.hi);
+    return Lengths{s.x, s.y, t.lens[b], t.news ? t.news[b] : 0};
+}
+__device__ __forceinline__ Move move_of(const Tables& t, const Lengths& x) {
+    Move m;
+    m.hi = min(max(x.hi, 0), t.max_pages);
+    m.lo = min(max(x.lo, 0), m.hi);
     const int64_t room = (int64_t)t.max_pages << t.lg;
-    const int64_t len = min((int64_t)max(t.lens[b], 0), room);
+    const int64_t len = min((int64_t)max(x.len, 0), room);
     m.hi2 = (int)((len + (1 << t.lg) - 1) >> t.lg);
     int64_t first = 0;                                  // the first page that a window of the call's first token, or the next, reaches
-    if (t.window) first = max((int64_t)0, len - max(t.news ? t.news[b] : 0, 0) - t.window + 1) >> t.lg;
+    if (t.window) first = max((int64_t)0, len - max(x.news, 0) - t.window + 1) >> t.lg;
     m.lo2 = (int)min(max((int64_t)m.lo, first), (int64_t)m.hi2);
     m.s1 = min(t.sink_pages, m.hi);
     m.s2 = min(t.sink_pages, m.hi2);
@@ -71,13 +80,19 @@ __device__ __forceinline__ Move move_of(const Tables& t, int b) {
     return m;
 }
 
-// Sums over the sequences before each, of a batch, by NT threads.
-template <int NT>
+// Sums over the sequences before each, of a batch of CAP at most, by NT threads.  KEEP: their lengths too, so that nothing
+// is loaded again.
+template <int NT, int CAP, bool KEEP>
 struct Sums {
     static constexpr int kWaves = NT / 64;
-    int back[kMostSequences], take[kMostSequences], token[kMostSequences];
+    int back[CAP], take[CAP], token[CAP];
     uint32_t wave[3][kWaves];
     int total[3];
+    Lengths lengths[KEEP ? CAP : 1];
+    __device__ __forceinline__ Lengths of(const Tables& t, int b) const {
+        if constexpr (KEEP) return lengths[b];
+        return lengths_of(t, b);
+    }
 };
 __device__ __forceinline__ uint32_t capped_scan(uint32_t v) {      // wave_scan whose sums end at kMostTokens
     auto add = [](uint32_t a, uint32_t b) { return min(a + b, (uint32_t)kMostTokens); };
@@ -89,18 +104,20 @@ __device__ __forceinline__ uint32_t capped_scan(uint32_t v) {      // wave_scan 
     v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
     return v;
 }
-template <int NT>
-__device__ __forceinline__ void sum_up(const Tables& t, Sums<NT>& s) {
+template <int NT, int CAP, bool KEEP>
+__device__ __forceinline__ void sum_up(const Tables& t, Sums<NT, CAP, KEEP>& s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t before[3] = {0, 0, 0};
     for (int b0 = 0; b0 < t.B; b0 += NT) {
         const int b = b0 + threadIdx.x;
         uint32_t n[3] = {0, 0, 0}, to[3];
         if (b < t.B) {
-            const Move m = move_of(t, b);
+            const Lengths x = lengths_of(t, b);
+            const Move m = move_of(t, x);
+            if constexpr (KEEP) s.lengths[b] = x;
             n[0] = m.back();
             n[1] = m.take();
-            n[2] = t.news ? min(max(t.news[b], 0), kMostTokens) : 0;
+            n[2] = min(max(x.news, 0), kMostTokens);
         }
         to[0] = mxa::wave_scan(n[0]);
         to[1] = mxa::wave_scan(n[1]);
@@ -111,7 +128,7 @@ __device__ __forceinline__ void sum_up(const Tables& t, Sums<NT>& s) {
         uint32_t at[3], sum[3];
         for (int i = 0; i < 3; ++i) {
             at[i] = sum[i] = before[i];
-            for (int w = 0; w < Sums<NT>::kWaves; ++w) {
+            for (int w = 0; w < Sums<NT, CAP, KEEP>::kWaves; ++w) {
                 const uint32_t x = s.wave[i][w];
                 if (w < wave) at[i] += x;
                 sum[i] += x;
@@ -122,14 +139,14 @@ __device__ __forceinline__ void sum_up(const Tables& t, Sums<NT>& s) {
             }
             before[i] = sum[i];
         }
+        // (the sum before it: a capped one is not the sum with it less its own)
+        const uint32_t prev = __shfl_up(to[2], 1);
         if (b < t.B) {
             s.back[b] = (int)(at[0] + to[0] - n[0]);
             s.take[b] = (int)(at[1] + to[1] - n[1]);
-            // (the sum before it: a capped one is not the sum with it less its own)
-            const uint32_t prev = __shfl_up(to[2], 1);
             s.token[b] = (int)min(at[2] + (lane ? prev : 0u), (uint32_t)kMostTokens);
         }
-        __syncthreads();
+        if (b0 + NT < t.B) __syncthreads();
     }
     if (threadIdx.x == 0)
         for (int i = 0; i < 3; ++i) s.total[i] = (int)before[i];
@@ -147,32 +164,32 @@ __device__ __forceinline__ int find(const int* sums, int n, int i) {
     return lo;
 }
 
-// The pages of sequence b, by n threads of which this is the i-th.  count: free pages before the call; R, A: the call's.
-template <int NT>
-__device__ __forceinline__ void move_pages(const Tables& t, const Sums<NT>& s, int b, int i, int n, int count) {
-    const Move m = move_of(t, b);
+// The pages that move, by n threads of which this is the i-th.  count: free pages before the call.
+template <class S>
+__device__ __forceinline__ void move_pages(const Tables& t, const S& s, int i, int n, int count) {
     const int R = s.total[0], A = s.total[1];
-    int32_t* const row = t.pages + (int64_t)b * t.max_pages;
-    for (int k = i; k < m.back(); k += n) {
-        const int r = s.back[b] + k, at = m.back_at(k);
-        const int32_t id = row[at];
-        row[at] = -1;
+    auto taken = [&](int a, int32_t id) {
+        const int b = find(s.take, t.B, a);
+        t.pages[(int64_t)b * t.max_pages + move_of(t, s.of(t, b)).take_at(a - s.take[b])] = id;
+    };
+    for (uint32_t r = i; r < (uint32_t)R; r += n) {
+        const int b = find(s.back, t.B, (int)r);
+        int32_t* const at = t.pages + (int64_t)b * t.max_pages + move_of(t, s.of(t, b)).back_at((int)r - s.back[b]);
+        const int32_t id = *at;
+        *at = -1;
         const int64_t place = (int64_t)count + R - 1 - r;
         if (place < t.n_pages) t.free[place] = id;
-        if (r < A) {                                    // taken at once
-            const int to = find(s.take, t.B, r);
-            t.pages[(int64_t)to * t.max_pages + move_of(t, to).take_at(r - s.take[to])] = id;
-        }
+        if (r < (uint32_t)A) taken((int)r, id);                        // at once
     }
-    for (int k = i; k < m.take(); k += n) {
-        const int64_t place = (int64_t)count + R - 1 - (s.take[b] + k);
-        if (place >= 0 && place < count) row[m.take_at(k)] = t.free[place];
+    for (uint32_t a = R + i; a < (uint32_t)A; a += n) {
+        const int64_t place = (int64_t)count + R - 1 - a;
+        if (place >= 0) taken((int)a, t.free[place]);
     }
 }
 // Sequence b's new range: what it took, where pages lack.
-template <int NT>
-__device__ __forceinline__ int2 new_span(const Tables& t, const Sums<NT>& s, int b, int count) {
-    const Move m = move_of(t, b);
+template <class S>
+__device__ __forceinline__ int2 new_span(const Tables& t, const S& s, int b, int count) {
+    const Move m = move_of(t, s.of(t, b));
     const int n = m.take(), got = (int)min((int64_t)n, max((int64_t)0, (int64_t)count + s.total[0] - s.take[b]));
     int hi = m.hi2;
     if (got < n) hi = got < m.take0() ? m.s1 + got : max(m.w2, m.hi) + got - m.take0();
@@ -185,21 +202,14 @@ __device__ __forceinline__ int2 new_state(const Tables& t, int count, int R, int
     return make_int2((int)min(there - min((int64_t)A, there), (int64_t)t.n_pages), (int)(A - min((int64_t)A, there)));
 }
 
-// The tokens of sequence b, the first of which is token `start`, by n threads of which this is the i-th.
-__device__ __forceinline__ void place_tokens(const Tables& t, int b, int start, int i, int n) {
-    const int count = min(max(t.news[b], 0), t.T - start);
-    const int64_t first = (int64_t)t.lens[b] - t.news[b], room = (int64_t)t.max_pages << t.lg;
-    for (int j = i; j < count; j += n) {
-        const int64_t p = first + j;
-        int64_t slot = -1;
-        if (p >= 0 && p < room) {
-            const int32_t id = t.pages[(int64_t)b * t.max_pages + (p >> t.lg)];
-            if ((uint32_t)id < (uint32_t)t.n_pages) slot = ((int64_t)id << t.lg) + (p & ((1 << t.lg) - 1));
-        }
-        t.slots[start + j] = slot;
-        t.seq[start + j] = b;
-        t.pos[start + j] = (int32_t)p;
-    }
+// Token `at`, of sequence b, at position p.
+__device__ __forceinline__ int32_t page_of(const Tables& t, int b, int64_t p) {
+    return p >= 0 && p < (int64_t)t.max_pages << t.lg ? t.pages[(int64_t)b * t.max_pages + (p >> t.lg)] : -1;
+}
+__device__ __forceinline__ void place_token(const Tables& t, int at, int b, int64_t p, int32_t id) {
+    t.slots[at] = (uint32_t)id < (uint32_t)t.n_pages ? ((int64_t)id << t.lg) + (p & ((1 << t.lg) - 1)) : -1;
+    t.seq[at] = b;
+    t.pos[at] = (int32_t)p;
 }
 __device__ __forceinline__ void no_token(const Tables& t, int at) {
     t.slots[at] = -1;
@@ -207,52 +217,69 @@ __device__ __forceinline__ void no_token(const Tables& t, int at) {
     t.pos[at] = -1;
 }
 
-template <int NT, bool ALONE>
+template <int NT, int CAP, bool ALONE>
 __global__ __launch_bounds__(NT) void kv4_pages_kernel(Tables t) {
-    __shared__ Sums<NT> s;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ Sums<NT, CAP, ALONE> s;
     const int count = free_count(t);
     sum_up(t, s);
-    if constexpr (ALONE) {
-        for (int b = wave; b < t.B; b += NT / 64) move_pages(t, s, b, lane, 64, count);
-    } else {
-        for (int b = blockIdx.x; b < t.B; b += gridDim.x) move_pages(t, s, b, threadIdx.x, NT, count);
-    }
+    move_pages(t, s, (int)(blockIdx.x * NT + threadIdx.x), (int)(gridDim.x * NT), count);
     if (t.starts && blockIdx.x == 0)
         for (int b = threadIdx.x; b <= t.B; b += NT) t.starts[b] = b < t.B ? s.token[b] : s.total[2];
     if constexpr (ALONE) {
-        __syncthreads();                                 // every range has been read, and the table is written
-        for (int b = threadIdx.x; b < t.B; b += NT) t.span[b] = new_span(t, s, b, count);      // (each reads its own alone)
+        for (int b = threadIdx.x; b < t.B; b += NT) t.span[b] = new_span(t, s, b, count);
+        __syncthreads();                                 // the table is written, and the count has been read
         if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1]);
-        if (!t.starts) return;
-        for (int b = wave; b < t.B; b += NT / 64)
-            if (s.token[b] < t.T) place_tokens(t, b, s.token[b], lane, 64);
-        for (int i = s.total[2] + threadIdx.x; i < t.T; i += NT) no_token(t, i);
+        for (int at = threadIdx.x; at < t.T; at += NT) {
+            if (at >= s.total[2]) {
+                no_token(t, at);
+                continue;
+            }
+            const int b = find(s.token, t.B, at);
+            const Lengths x = s.of(t, b);
+            const int64_t p = (int64_t)x.len - x.news + at - s.token[b];
+            place_token(t, at, b, p, page_of(t, b, p));
+        }
     }
 }
 
-// Workgroup (x, y): tokens of sequence x, part y of them; past the sequences, those that there are none of.  The last x
-// alone: the ranges and the count.
-template <int NT>
+// Workgroup (x, y): tokens of sequence x, part y of them, a thread kTokens at a time, and a share of the places past the
+// last token.  The last x alone, past the sequences: the ranges and the count.
+constexpr int kTokens = 4;
+template <int NT, int CAP>
 __global__ __launch_bounds__(NT) void kv4_slots_kernel(Tables t) {
     const int b = blockIdx.x, i = blockIdx.y * NT + threadIdx.x, n = gridDim.y * NT;
-    if (b < t.B) {
-        if (t.starts && t.starts[b] < t.T) place_tokens(t, b, t.starts[b], i, n);
+    if (t.starts) {                              // (every workgroup some, as the tokens may be few)
+        const int64_t all = (int64_t)gridDim.x * n;
+        for (int64_t at = (int64_t)t.starts[t.B] + (int64_t)b * n + i; at < t.T; at += all) no_token(t, (int)at);
+    }
+    if (b + 1 < (int)gridDim.x) {
+        if (t.starts[b] >= t.T) return;
+        const int start = t.starts[b], news = t.news[b], end = min(max(news, 0), t.T - start);
+        const int64_t first = (int64_t)t.lens[b] - news;
+        for (int j0 = i; j0 < end; j0 += kTokens * n) {
+            int32_t id[kTokens];
+#pragma unroll
+            for (int k = 0; k < kTokens; ++k) id[k] = page_of(t, b, first + min(j0 + (int64_t)k * n, (int64_t)end - 1));
+#pragma unroll
+            for (int k = 0; k < kTokens; ++k) {
+                const int64_t j = j0 + (int64_t)k * n;
+                if (j < end) place_token(t, start + (int)j, b, first + j, id[k]);
+            }
+        }
         return;
     }
-    if (t.starts)
-        for (int64_t at = (int64_t)t.starts[t.B] + i; at < t.T; at += n) no_token(t, (int)at);
     if (blockIdx.y) return;
-    __shared__ Sums<NT> s;
+    __shared__ Sums<NT, CAP, false> s;
     const int count = free_count(t);
     sum_up(t, s);
-    for (int q = threadIdx.x; q < t.B; q += NT) t.span[q] = new_span(t, s, q, count);
+    for (int q = threadIdx.x; q < t.B; q += NT) t.span[q] = new_span(t, s, q, count);      // (each reads its own alone)
     if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1]);
 }
 
-// Entries of the table up to which one workgroup does everything.
+// Entries of the table, and sequences, up to which one workgroup does everything.
 constexpr int64_t kFewEntries = 32768;
-constexpr int kFewTokens = 8192;
+constexpr int kFewTokens = 8192, kFewSequences = 1024;
+constexpr int kThreads = 512;
 
 }  // namespace
 
@@ -277,14 +304,17 @@ extern "C" int mxfp4_kv4_tables(int32_t* pages, int32_t* span, int32_t* free, in
     const Tables t{pages, reinterpret_cast<int2*>(span), free, state, lens, news, starts, slots, seq, pos, B, max_pages, n_pages, lg,
                    window, sink_pages < max_pages ? sink_pages : max_pages, T};
     const hipStream_t st = mxh::as_stream(stream);
-    if ((int64_t)B * max_pages <= kFewEntries && T <= kFewTokens) {
-        hipLaunchKernelGGL((kv4_pages_kernel<1024, true>), dim3(1), dim3(1024), 0, st, t);
+    if (B <= kFewSequences && (int64_t)B * max_pages <= kFewEntries && T <= kFewTokens) {
+        hipLaunchKernelGGL((kv4_pages_kernel<1024, kFewSequences, true>), dim3(1), dim3(1024), 0, st, t);
         return mxh::launch_status("kv4_tables");
     }
-    hipLaunchKernelGGL((kv4_pages_kernel<256, false>), dim3(B < 256 ? B : 256), dim3(256), 0, st, t);
+    const int64_t entries = ((int64_t)B * max_pages + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL((kv4_pages_kernel<kThreads, kMostSequences, false>), dim3((unsigned)std::min<int64_t>(entries, 256)), dim3(kThreads),
+                       0, st, t);
     const int rc = mxh::launch_status("kv4_tables");
     if (rc != MXFP4_OK) return rc;
-    const int64_t parts = ((int64_t)T / B + 1023) / 1024;
-    hipLaunchKernelGGL(kv4_slots_kernel<256>, dim3(B + 1, (unsigned)(parts < 1 ? 1 : parts > 64 ? 64 : parts)), dim3(256), 0, st, t);
+    const int64_t parts = ((int64_t)T / B + kTokens * kThreads - 1) / (kTokens * kThreads);
+    hipLaunchKernelGGL((kv4_slots_kernel<kThreads, kMostSequences>), dim3(T ? B + 1 : 1, (unsigned)(parts < 1 ? 1 : parts > 64 ? 64 : parts)),
+                       dim3(kThreads), 0, st, t);
     return mxh::launch_status("kv4_tables (slots)");
 }
