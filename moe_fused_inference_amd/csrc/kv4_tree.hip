@@ -17,12 +17,14 @@ namespace {
 constexpr int kMostDrafts = 4096;
 constexpr int kThreads = 256;
 
-// Workgroup (sequence, kThreads drafts from c0 on), which makes the bits of the drafts before them too.
+// Workgroup (sequence, 64 drafts from c0 on), which makes the bits of the drafts before them too; then four threads a
+// draft, each every fourth 64 bits of its row, so that what they store lies together.  64 trees of 500, us: 6.0 with a
+// thread a draft and 256 drafts a workgroup.  WIDE: a row is whole words of 64 bits.
+template <bool WIDE>
 __global__ __launch_bounds__(kThreads) void tree_masks_kernel(const int32_t* __restrict__ parents, uint32_t* __restrict__ tree,
                                                               int32_t* __restrict__ depth, int M) {
     extern __shared__ uint64_t lds[];
-    const int b = blockIdx.x, c0 = blockIdx.y * kThreads, words = (M + 31) / 32;
-    const int top = min(M, c0 + kThreads), blocks = (top + 63) / 64;
+    const int b = blockIdx.x, c0 = blockIdx.y * 64, words = (M + 31) / 32, blocks = blockIdx.y + 1;
     uint64_t* const bits = lds;                                  // of each draft, within its 64
     int* const out = reinterpret_cast<int*>(lds + 64 * blocks);  // where its line goes on: an earlier 64's draft, -1 nowhere, -2 it is none
     const int lane = threadIdx.x & 63;
@@ -44,7 +46,7 @@ __global__ __launch_bounds__(kThreads) void tree_masks_kernel(const int32_t* __r
         out[m] = to;
     }
     __syncthreads();
-    const int m = c0 + threadIdx.x;
+    const int m = c0 + (threadIdx.x >> 2), part = threadIdx.x & 3;
     if (m >= M) return;
     int n = 0, at = m;
     while (at >= 0) {
@@ -52,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void tree_masks_kernel(const int32_t* __r
         at = out[at];
     }
     const bool none = at == -2;
-    depth[(int64_t)b * M + m] = none ? -1 : n - 1;
+    if (part == 0) depth[(int64_t)b * M + m] = none ? -1 : n - 1;
     uint32_t* const row = tree + ((int64_t)b * M + m) * words;
     at = none ? -1 : m;
     for (int k = (words - 1) / 2; k >= 0; --k) {
@@ -61,8 +63,13 @@ __global__ __launch_bounds__(kThreads) void tree_masks_kernel(const int32_t* __r
             a = bits[at];
             at = out[at];
         }
-        row[2 * k] = (uint32_t)a;
-        if (2 * k + 1 < words) row[2 * k + 1] = (uint32_t)(a >> 32);
+        if ((k & 3) != part) continue;
+        if constexpr (WIDE) {
+            *reinterpret_cast<uint64_t*>(row + 2 * k) = a;
+        } else {
+            row[2 * k] = (uint32_t)a;
+            if (2 * k + 1 < words) row[2 * k + 1] = (uint32_t)(a >> 32);
+        }
     }
 }
 
@@ -71,17 +78,20 @@ struct Layers {
     uint8_t* t[kLayers][4];      // kq, ks, vq, vs
 };
 
-// Workgroup (sequence and kv head, layer): a thread 16 bytes of a row's nibbles, or its codes, of keys or of values, of as
-// many drafts as there are threads for.  What is moved is read before any of it is written; a later round reads only rows
-// from its own drafts on (path[b][k] >= k), and writes none before.
-template <int D>
-__global__ __launch_bounds__(kThreads) void kv4_keep_kernel(Layers layers, kv4::Cache c, const int32_t* __restrict__ dpos,
-                                                            const int32_t* __restrict__ path, int A) {
-    constexpr int Q = D / 32, kItems = 2 * Q + 2, R = kThreads / kItems;
+constexpr int kAtOnce = 4;       // of a workgroup
+
+// Workgroup (sequence and kv head, kAtOnce layers) of T threads: a thread 16 bytes of a row's nibbles, or its codes, of
+// keys or of values, in every layer, of as many drafts as there are threads for.  What is moved is read before any of it is
+// written; a later round reads only rows from its own drafts on (path[b][k] >= k), and writes none before.  32 paths of up to
+// 9, 48 layers, us: 10.2 with a layer a workgroup of 256 threads, most of which had nothing to move.
+template <int D, int T>
+__global__ __launch_bounds__(T) void kv4_keep_kernel(Layers layers, int n_layers, kv4::Cache c, const int32_t* __restrict__ dpos,
+                                                     const int32_t* __restrict__ path, int A) {
+    constexpr int Q = D / 32, kItems = 2 * Q + 2, R = T / kItems, U = kAtOnce;
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     const int b = blockIdx.x / c.Hkv, g = blockIdx.x - b * c.Hkv, lane = threadIdx.x & 63;
+    const int l0 = blockIdx.y * U, nl = min(U, n_layers - l0);
     const int32_t* const line = path + (int64_t)b * A;
-    uint8_t* const* const t = layers.t[blockIdx.y];
     const int64_t base = dpos[b];
     const int k = threadIdx.x / kItems, item = threadIdx.x - k * kItems;
     int n = A;                                                    // its drafts, up to the first that is none
@@ -92,6 +102,12 @@ __global__ __launch_bounds__(kThreads) void kv4_keep_kernel(Layers layers, kv4::
             break;
         }
     }
+    const bool codes = item >= 2 * Q;
+    auto tensor = [&](int u) {                                    // (uniform loads, and a choice)
+        uint8_t* const* const t = layers.t[l0 + u];
+        return item < Q ? t[0] : item < 2 * Q ? t[2] : item == 2 * Q ? t[1] : t[3];
+    };
+    const uint32_t stride = codes ? D / 32 : D / 2, off = codes ? 0 : 16 * (item < Q ? item : item - Q);
     for (int k0 = 0; k0 < n; k0 += R) {
         const int i = k0 + k;
         int64_t from = -1, to = -1;
@@ -103,22 +119,35 @@ __global__ __launch_bounds__(kThreads) void kv4_keep_kernel(Layers layers, kv4::
             }
         }
         const bool moves = from >= 0 && to >= 0;
-        v4u w = 0;
-        uint8_t* const q = t[item < Q ? 0 : 2] + 16 * (item < Q ? item : item - Q);     // of a nibble item
-        uint8_t* const s = t[item == 2 * Q ? 1 : 3];                                    // of a code item
-        if (moves) {
-            if (item < 2 * Q) w = *reinterpret_cast<const v4u*>(q + from * (D / 2));
-            else if constexpr (D == 128) w[0] = *reinterpret_cast<const uint32_t*>(s + from * 4);
-            else w[0] = *reinterpret_cast<const uint16_t*>(s + from * 2);
+        v4u w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            w[u] = 0;
+            if (!moves || u >= nl) continue;
+            const uint8_t* const p = tensor(u) + from * stride + off;
+            if (!codes) w[u] = *reinterpret_cast<const v4u*>(p);
+            else if constexpr (D == 128) w[u][0] = *reinterpret_cast<const uint32_t*>(p);
+            else w[u][0] = *reinterpret_cast<const uint16_t*>(p);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the rows are here, not on their way, when another wave writes
         __syncthreads();
-        if (moves) {
-            if (item < 2 * Q) *reinterpret_cast<v4u*>(q + to * (D / 2)) = w;
-            else if constexpr (D == 128) *reinterpret_cast<uint32_t*>(s + to * 4) = w[0];
-            else *reinterpret_cast<uint16_t*>(s + to * 2) = (uint16_t)w[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!moves || u >= nl) continue;
+            uint8_t* const p = tensor(u) + to * stride + off;
+            if (!codes) *reinterpret_cast<v4u*>(p) = w[u];
+            else if constexpr (D == 128) *reinterpret_cast<uint32_t*>(p) = w[u][0];
+            else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[u][0];
         }
     }
+}
+template <int D>
+void launch_keep(const Layers& t, int n, const kv4::Cache& c, const int32_t* dpos, const int32_t* path, int B, int A, hipStream_t st) {
+    const dim3 grid(B * c.Hkv, (n + kAtOnce - 1) / kAtOnce);
+    const int items = 2 * (D / 32) + 2;      // threads a draft
+    if (A * (int64_t)items <= 64) hipLaunchKernelGGL((kv4_keep_kernel<D, 64>), grid, dim3(64), 0, st, t, n, c, dpos, path, A);
+    else if (A * (int64_t)items <= 128) hipLaunchKernelGGL((kv4_keep_kernel<D, 128>), grid, dim3(128), 0, st, t, n, c, dpos, path, A);
+    else hipLaunchKernelGGL((kv4_keep_kernel<D, 256>), grid, dim3(256), 0, st, t, n, c, dpos, path, A);
 }
 
 }  // namespace
@@ -126,10 +155,11 @@ __global__ __launch_bounds__(kThreads) void kv4_keep_kernel(Layers layers, kv4::
 extern "C" int mxfp4_tree_masks(const int32_t* parents, int32_t* tree, int32_t* depth, int B, int M, void* stream) {
     MXH_REQUIRE(parents && tree && depth, "tree_masks: null pointer");
     MXH_REQUIRE(B > 0 && B <= 65535 && M > 0 && M <= kMostDrafts, "tree_masks: B=%d M=%d (up to %d drafts)", B, M, kMostDrafts);
-    const int chunks = (M + kThreads - 1) / kThreads;
-    const size_t lds = (size_t)((M + 63) / 64 * 64) * (sizeof(uint64_t) + sizeof(int));
-    hipLaunchKernelGGL(tree_masks_kernel, dim3(B, chunks), dim3(kThreads), lds, mxh::as_stream(stream), parents,
-                       reinterpret_cast<uint32_t*>(tree), depth, M);
+    const int chunks = (M + 63) / 64;
+    const size_t lds = (size_t)(chunks * 64) * (sizeof(uint64_t) + sizeof(int));
+    const bool wide = (M + 31) / 32 % 2 == 0 && ((uintptr_t)tree & 7) == 0;
+    hipLaunchKernelGGL(wide ? tree_masks_kernel<true> : tree_masks_kernel<false>, dim3(B, chunks), dim3(kThreads), lds,
+                       mxh::as_stream(stream), parents, reinterpret_cast<uint32_t*>(tree), depth, M);
     return mxh::launch_status("tree_masks");
 }
 
@@ -154,9 +184,8 @@ extern "C" int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* c
             t.t[l][2] = vq[l0 + l];
             t.t[l][3] = vs[l0 + l];
         }
-        const dim3 grid(B * Hkv, n);
-        if (D == 64) hipLaunchKernelGGL(kv4_keep_kernel<64>, grid, dim3(kThreads), 0, mxh::as_stream(stream), t, c, dpos, path, A);
-        else hipLaunchKernelGGL(kv4_keep_kernel<128>, grid, dim3(kThreads), 0, mxh::as_stream(stream), t, c, dpos, path, A);
+        if (D == 64) launch_keep<64>(t, n, c, dpos, path, B, A, mxh::as_stream(stream));
+        else launch_keep<128>(t, n, c, dpos, path, B, A, mxh::as_stream(stream));
         const int rc = mxh::launch_status("kv4_keep");
         if (rc != MXFP4_OK) return rc;
     }

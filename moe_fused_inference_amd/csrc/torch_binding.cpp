@@ -483,30 +483,48 @@ std::vector<torch::Tensor> kv4_tree_masks(const torch::Tensor& parents) {
     return {tree, depth};
 }
 
-// The rows dpos[b] + path[b,k] of every layer's cache -> dpos[b] + k.  caches: a list of (kq, ks, vq, vs).
-void kv4_keep(const std::vector<std::vector<torch::Tensor>>& caches, const torch::Tensor& dpos, const torch::Tensor& path,
-              const c10::optional<torch::Tensor>& pages) {
-    require(!caches.empty(), "kv4_keep needs a cache at least");
+// The rows dpos[b] + path[b,k] of every layer's cache -> dpos[b] + k.  caches: a sequence of (kq, ks, vq, vs), read as it
+// is (48 layers: 192 tensors; as vectors of tensors they took 9 us of the call's 17).
+void kv4_keep(const py::handle& caches, const torch::Tensor& dpos, const torch::Tensor& path, const c10::optional<torch::Tensor>& pages) {
+    const auto fast = [](PyObject* o, const char* msg) {
+        PyObject* const f = PySequence_Fast(o, msg);
+        if (!f) throw py::error_already_set();
+        return py::reinterpret_steal<py::object>(f);
+    };
+    const py::object list = fast(caches.ptr(), "caches must be a sequence");
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+    require(n > 0, "kv4_keep needs a cache at least");
     std::vector<uint8_t*> p[4];
+    for (auto& x : p) x.reserve(n);
     Kv4 c{};
-    for (size_t l = 0; l < caches.size(); ++l) {
-        const auto& t = caches[l];
-        require(t.size() == 4, "a cache is four tensors");
-        const Kv4 x = kv4_cache(t[0], t[1], t[2], t[3], pages, dpos, "dpos must be a contiguous int32 (B,) tensor on the cache's device");
-        require(t[0].sizes() == caches[0][0].sizes() && t[0].device() == caches[0][0].device(), "caches must be of one shape and device");
-        if (l == 0) c = x;
-        p[0].push_back(x.kq);
-        p[1].push_back(x.ks);
-        p[2].push_back(x.vq);
-        p[3].push_back(x.vs);
+    torch::Tensor first[4];
+    for (Py_ssize_t l = 0; l < n; ++l) {
+        const py::object cache = fast(PySequence_Fast_GET_ITEM(list.ptr(), l), "a cache is four tensors");
+        require(PySequence_Fast_GET_SIZE(cache.ptr()) == 4, "a cache is four tensors");
+        const at::Tensor* t[4];
+        for (int i = 0; i < 4; ++i) {
+            PyObject* const o = PySequence_Fast_GET_ITEM(cache.ptr(), i);
+            require(THPVariable_Check(o), "a cache is four tensors");
+            t[i] = &THPVariable_Unpack(o);
+        }
+        if (l == 0) {
+            c = kv4_cache(*t[0], *t[1], *t[2], *t[3], pages, dpos, "dpos must be a contiguous int32 (B,) tensor on the cache's device");
+            for (int i = 0; i < 4; ++i) first[i] = *t[i];
+        } else {
+            for (int i = 0; i < 4; ++i)
+                require(t[i]->scalar_type() == torch::kUInt8 && t[i]->sizes() == first[i].sizes() && t[i]->is_contiguous() &&
+                            t[i]->device() == first[0].device(),
+                        "caches must be contiguous, of one shape and device");
+        }
+        for (int i = 0; i < 4; ++i) p[i].push_back(u8m(*t[i]));
     }
-    const torch::Tensor& kq = caches[0][0];
+    const torch::Tensor& kq = first[0];
     require(is_i32(path, 2) && path.device() == kq.device() && path.size(0) == c.B,
             "path must be a contiguous int32 (B,A) tensor on the cache's device");
     const int A = as_int(path.size(1), "too many drafts");
     if (A == 0 || c.B == 0) return;
     const c10::DeviceGuard guard(kq.device());
-    check(mxfp4_kv4_keep(p[0].data(), p[1].data(), p[2].data(), p[3].data(), as_int((int64_t)caches.size(), "too many caches"), c.pages,
+    check(mxfp4_kv4_keep(p[0].data(), p[1].data(), p[2].data(), p[3].data(), as_int((int64_t)n, "too many caches"), c.pages,
                          c.n_pages, c.page, c.max_pages, c.at, i32m(path), c.B, A, c.Hkv, c.D, stream_of(kq)),
           "kv4_keep");
 }

@@ -130,7 +130,7 @@ def kv4_keep(caches, dpos, path, pages=None):
     order of their line, so path[b, k] >= k (others stay where they are), -1 from its end on."""
     if isinstance(caches[0], torch.Tensor):
         caches = [caches]
-    _ext().keep([list(c) for c in caches], dpos, path, pages)
+    _ext().keep(caches, dpos, path, pages)
 
 
 def kv4_read(cache, n, start=None, pages=None, dtype=torch.bfloat16):
