@@ -18,7 +18,6 @@ constexpr int kUnit = 32;              // positions per wave and step
 constexpr float kMost = 2048.0f;       // a lane's terms of a unit sum to at most this
 constexpr float kWide = 262144.0f;     // a reference past it: an exponent's rounding is up to 2^-6 and more
 constexpr float kNone = -3e38f;        // the reference of a row that has seen nothing: exp2(-inf - kNone) = 0
-constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 constexpr int kFew = 32;               // shares of a sequence that four waves merge at once
 constexpr int kMinShare = 4;           // units, one a wave
 // Units that take about as long as a workgroup's change to another sequence; whole shares of kMinShare.  4 / 6 / 8 / 9 /
@@ -87,6 +86,18 @@ __device__ __forceinline__ mx::v4f mfma_bf16(uint4 a, uint4 b, mx::v4f c) {
                                                    0, 0, 0);
 }
 
+// n / d for n below 2^32 by the high half of a product, which is it or one less (a division is about 25 instructions, and a
+// short call's prologue is a chain of them).
+struct Divisor {
+    uint32_t d, m;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) : d(d), m(0xFFFFFFFFu / d) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t q = __umulhi(n, m);
+        return q + (n - q * d >= d ? 1u : 0u);
+    }
+};
+
 struct Args {
     const uint16_t* q;
     int64_t ldq;                 // elements between tokens of q
@@ -97,6 +108,8 @@ struct Args {
     Out out;
     int per;                     // units of a share of one sequence, or 0: as share_units finds from its length
     int B, M, Hq, G, shares, records;   // shares of the batch, and records a row may have (its stride)
+    Divisor by_G, by_rows, by_shares;   // by_rows: M * G
+    __device__ __forceinline__ int token(int r) const { return (int)by_G((uint32_t)r); }    // of row r of a kv head
     float scale;                 // log2(e) / sqrt(D)
     // Of the kernels with masks (MASKED) alone
     int window, sinks;           // a token sees the last `window` positions up to its own (0: all), and the first `sinks`
@@ -189,7 +202,7 @@ __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__b
 // 8000 9.8 / 9.1, 32000 16.4 / 13.5).
 __device__ __forceinline__ uint32_t share_units(uint64_t total, const Args& a) {
     const uint64_t n = total + a.shares - 1;
-    const uint32_t per = (uint32_t)((n >> 32 ? n / a.shares : (uint32_t)n / (uint32_t)a.shares) + 3) & ~3u;
+    const uint32_t per = (uint32_t)((n >> 32 ? n / a.shares : a.by_shares((uint32_t)n)) + 3) & ~3u;
     return max(per, total > (uint64_t)kFew * kMinShare * a.B ? 2u * kMinShare : (uint32_t)kMinShare);
 }
 
@@ -405,6 +418,21 @@ __device__ __forceinline__ void again(const float (&s)[N], float scale, float& m
     l += sum;
 }
 
+// The same of a row's first unit: on its maximum at once.
+template <int N, int NP, class Over>
+__device__ __forceinline__ void first_terms(float (&s)[N], float scale, float& m, float& l, bool& wide, uint4 (&p)[N / 8][NP], Over over) {
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < N; i += 2) top = max3(top, s[i], s[i + 1 < N ? i + 1 : i]);
+    top = over(top);
+    if (top > -INFINITY) m = top * scale;                // else it sees nothing, or is NaN
+    wide = __ballot(fabsf(m) > kWide && m != kNone) != 0ull;
+    float t[N], sum;
+    terms(s, scale, m, wide, t, sum);
+    parts(t, p);
+    l = sum;
+}
+
 // A code of a position's word, in the exponent field of a scale for the packed
 // conversions, which read that field alone: its neighbours are around it.
 __device__ __forceinline__ float scale_at(uint32_t word, uint32_t block) {
@@ -475,10 +503,11 @@ template <int D, int NW, bool ONE, bool MASKED, class M, class L, class O>
 __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
     constexpr int CT = D / 16;
     const int c0 = CT * (tid & 15);
-    const int64_t pos = (int64_t)base + r / a.G;
+    const int t = a.token(r);
+    const int64_t pos = (int64_t)base + t;
     if (!ONE && (pos < 0 || pos >= a.c.max_pos)) return;                      // no record: the merge reads none
     if constexpr (!ONE && MASKED) {
-        if ((uint32_t)u0 > units<true>(a, base).of_real((uint32_t)last_seen<true>(a, base, r / a.G) / kUnit)) return;
+        if ((uint32_t)u0 > units<true>(a, base).of_real((uint32_t)last_seen<true>(a, base, t) / kUnit)) return;
     } else if (!ONE) {
         if ((int64_t)u0 * kUnit > pos) return;
     }
@@ -506,7 +535,7 @@ __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, 
         const float inv = none ? 0.0f : 1.0f / den;
 #pragma unroll
         for (int c = 0; c < CT; ++c) o[c] = none ? 0.0f : o[c] * inv;
-        store<CT>(a.out, ((int64_t)b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, c0, o);
+        store<CT>(a.out, ((int64_t)b * a.M + t) * a.Hq + g * a.G + r - t * a.G, D, c0, o);
     } else {
         float* rec = a.part + (((int64_t)g * a.M * a.G + r) * a.records + blockIdx.x + b) * (D + 4);
 #pragma unroll

@@ -50,6 +50,22 @@ namespace {
 // take half lines).
 constexpr int64_t kMuch = 128ll << 20;
 
+// Row r of kv head g, of sequence b: its records.
+struct Records {
+    int g, token, head, n;
+    const float* at;
+};
+template <int D, bool MASKED>
+__device__ __forceinline__ Records records_of(const Args& a, int4 p, int base, int b, int row) {
+    const int rows = a.M * a.G, g = (int)a.by_rows(row), r = row - g * rows, t = a.token(r);
+    const int64_t pos = (int64_t)base + t;
+    // those of the shares with its sequence's units up to the last that it sees
+    uint32_t top = (uint32_t)(pos / kUnit);
+    if constexpr (MASKED) top = units<true>(a, base).of_real((uint32_t)(last_seen<true>(a, base, t) / kUnit));
+    const int n = pos < 0 || pos >= a.c.max_pos ? 0 : min((int)(((uint32_t)p.y + top) / (uint32_t)p.z) + 1, a.shares - p.x);
+    return Records{g, t, r - t * a.G, n, a.part + ((int64_t)row * a.records + p.x + b) * (D + 4)};
+}
+
 // Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b): the row's
 // records dealt to NW waves, eight loaded at a time (one memory latency for up to
 // 8 NW), each with a running reference; a lane holds D / 64 columns.
@@ -61,17 +77,10 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     __shared__ __align__(16) float mo[NW][D];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rows = a.M * a.G;
-    const int b = blockIdx.y, g = blockIdx.x / rows, r = blockIdx.x - g * rows;
-    const int4 p = a.places[b];
-    const int base = a.dpos[b];
-    const int64_t pos = (int64_t)base + r / a.G;
-    // its records: those of the shares with its sequence's units up to the last that it sees
-    uint32_t top = (uint32_t)(pos / kUnit);
-    if constexpr (MASKED) top = units<true>(a, base).of_real((uint32_t)(last_seen<true>(a, base, r / a.G) / kUnit));
-    const int ns = __builtin_amdgcn_readfirstlane(
-        pos < 0 || pos >= a.c.max_pos ? 0 : min((int)(((uint32_t)p.y + top) / (uint32_t)p.z) + 1, a.shares - p.x));
-    const float* rec = a.part + ((int64_t)blockIdx.x * a.records + __builtin_amdgcn_readfirstlane(p.x) + b) * (D + 4);
+    const int b = blockIdx.y;
+    const Records rs = records_of<D, MASKED>(a, a.places[b], a.dpos[b], b, blockIdx.x);
+    const int ns = __builtin_amdgcn_readfirstlane(rs.n);
+    const float* rec = rs.at;
     float m = kNone, l = 0.0f;
     cvec o = 0.0f;
     for (int i0 = wave; i0 < ns; i0 += N * NW) {
@@ -123,26 +132,99 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     const float inv = 1.0f / den;
 #pragma unroll
     for (int c = 0; c < CT; ++c) x[c] = none ? 0.0f : x[c] * inv;
-    store<CT>(a.out, ((int64_t)b * a.M + r / a.G) * a.Hq + g * a.G + r % a.G, D, CT * tid, x);
+    store<CT>(a.out, ((int64_t)b * a.M + rs.token) * a.Hq + rs.g * a.G + rs.head, D, CT * tid, x);
 }
 
-Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
+// The same, to the same bits, where there are many rows of up to kFew records: 16 lanes a row, a lane D / 16 columns, with
+// the four waves' sums of the kernel above as four in registers.
+template <int D, bool MASKED>
+__global__ __launch_bounds__(256) void attn_kv4_merge_rows_kernel(Args a) {
+    constexpr int CT = D / 16, N = 4;
+    const int tid = threadIdx.x, t = tid & 15, b = blockIdx.y;
+    const int row = blockIdx.x * 16 + (tid >> 4), total = a.M * a.Hq;
+    const Records rs = records_of<D, MASKED>(a, a.places[b], a.dpos[b], b, min(row, total - 1));
+    // the states of records t and t + 16, and the reference of those of t's class modulo 4
+    float2 st[2];
+    float ref = kNone;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        st[i] = make_float2(kNone, 0.0f);
+        if (t + 16 * i < rs.n) st[i] = *reinterpret_cast<const float2*>(rs.at + (int64_t)(t + 16 * i) * (D + 4));
+        ref = fmaxf(ref, st[i].x);
+    }
+    ref = fmaxf(ref, mx::dpp<0x124>(ref));               // row_ror 4, 8
+    ref = fmaxf(ref, mx::dpp<0x128>(ref));
+    float w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = __builtin_amdgcn_exp2f(st[i].x - ref);
+    float l[N], o[N][CT];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        l[k] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[k][c] = 0.0f;
+    }
+    for (int i0 = 0; __any(i0 < rs.n); i0 += N) {
+        float4 v[N][CT / 4];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int c = 0; c < CT / 4; ++c)
+                v[k][c] = *reinterpret_cast<const float4*>(rs.at + (int64_t)min(i0 + k, max(rs.n - 1, 0)) * (D + 4) + 4 + CT * t + 4 * c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int from = (i0 & 15) + k;
+            const float wt = __shfl(i0 < 16 ? w[0] : w[1], from, 16), ly = __shfl(i0 < 16 ? st[0].y : st[1].y, from, 16);
+            if (i0 + k < rs.n) {
+                l[k] = fmaf(wt, ly, l[k]);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) o[k][c] = fmaf(wt, reinterpret_cast<const float*>(&v[k][c / 4])[c % 4], o[k][c]);
+            }
+        }
+    }
+    float m[N], gm, den = 0.0f, x[CT];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        m[k] = __shfl(ref, k, 16);
+        gm = k ? fmaxf(gm, m[k]) : m[k];
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) x[c] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float wt = __builtin_amdgcn_exp2f(m[k] - gm);
+        den = fmaf(wt, l[k], den);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) x[c] = fmaf(wt, o[k][c], x[c]);
+    }
+    const bool none = den == 0.0f;    // no position, or none on a page: zeros
+    const float inv = 1.0f / den;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) x[c] = none ? 0.0f : x[c] * inv;
+    if (row < total) store<CT>(a.out, ((int64_t)b * a.M + rs.token) * a.Hq + rs.g * a.G + rs.head, D, CT * t, x);
+}
+
+// room: positions of a sequence that its tokens may see together (room_of); fewer than there are: a window's.
+Plan plan(int B, int M, int Hq, int Hkv, int max_pos, int room) {
     Plan p{};
+    const bool window = room < max_pos;
+    max_pos = room;
     const int64_t rows = (int64_t)M * (Hq / Hkv);
     int64_t longest = (max_pos + kMinShare * kUnit - 1) / (kMinShare * kUnit);   // shares a sequence may have (share_units)
     if (longest > kFew) longest = std::max<int64_t>(kFew, (longest + 1) / 2);
     const int64_t most = B * (longest + (B > 1 ? kPad / kMinShare : 0));   // with a share of whole pads
     p.waves = 4;
-    if (rows <= 16) {
-        p.groups = 1;
+    if (rows <= 16) p.groups = 1;
+    else {
+        p.many = true;
+        p.groups = (int)((rows + 31) / 32);
+    }
+    const int64_t wgs = (int64_t)B * Hkv * p.groups;
+    if (!p.many && !window) {
         // Sequences enough for half the CUs, and short: one workgroup of 16 waves each and no merge.  32 / 4 heads, one
         // token, full caches, 16 waves / shares and merge, us: B = 64, 1024 positions 13.7 / 19.9, 2048 19.2 / 24.1; B = 32,
         // 2048 16.5 / 18.5; but B = 8, 2048 15.4 / 11.8, B = 1, 1024 10.8 / 8.1.
-        const int64_t wgs = (int64_t)B * Hkv;
         if (longest > 1 && max_pos <= 2048 && wgs >= 128 && wgs <= 256) p.waves = 16;
-    } else {
-        p.many = true;
-        p.groups = (int)((rows + 31) / 32);
     }
     // shares of the whole batch for one round of workgroups, four or two a CU, and none that starts a second round
     const int64_t want = std::max<int64_t>(1, (p.many ? 512 : 1024) / ((int64_t)Hkv * p.groups));
@@ -153,8 +235,26 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos) {
     // 128 tokens, 128 workgroups: 1024 positions 22.7 / 15.8, 8192 49.8 / 84.1.
     // What it gives away is a batch of one long sequence among short ones, which the host cannot know: one of 8192 positions
     // among 255 of 64, eight kv heads, 32 / 142 (all of 8192: 406 / 376), one of 32768 among 63, 64 kv heads, 85 / 1048 (3008 / 2899).
-    const int64_t wgs = (int64_t)B * Hkv * p.groups;
     p.one = p.waves == 16 || longest == 1 || want * 4 <= B || (want == 1 && B == 1) || max_pos <= (p.many ? 8 : 4) * wgs;
+    if (window) {
+        // A window bounds what a long sequence among short ones takes, and most sequences fill it, so a workgroup has a
+        // whole one further up: up to 16 rows of 16 waves, where each has a CU to itself.  us, shares / one (4, 16 waves), one
+        // token, 8 query heads a kv head: 4 workgroups, 256 positions 8.5 / 7.7, 7.7, 512 8.6 / 9.5, 9.3; 32, 512 10.4 / 9.7,
+        // 9.4, 1024 11.7 / 13.3, 12.2; 64, 2048 18.4 / 20.5, 17.5, 3000 18.6 / 26.0, 21.5; 128, 4096 28.5 / 37.2, 27.7, 8192
+        // 41.5 / 70.0, 45.9; 256, 512 20.2 / 10.5, 11.1, 2048 29.3 / 21.8, 19.2, 8192 65.8 / 75.4, 59.0; 512, 2048 45.8 /
+        // 30.8, 39.9, 8192 120 / 109, 114; 800, 1024 47.1 / 29.3, 48.9, 4096 103 / 91, 113.
+        // More rows, shares / one: 4 workgroups, 128 positions 10.9 / 9.9, 256 10.9 / 11.7; 32, 256 12.4 / 11.8, 512 13.2 /
+        // 14.7; 128, 1024 21.1 / 20.9 (one sequence), 22.9 / 20.5 (eight), 2048 25.6 / 30.7, 30.4 / 31.1; 256, 2048 33.1 / 31.2,
+        // 39.9 / 31.6, 4096 48.0 / 50.1, 56.1 / 50.6; 400, 4096 78.3 / 69.0; 512, 8192 131 / 125, 145 / 127 (32 sequences).
+        const bool own = wgs <= 256;
+        constexpr int few = 3 * kMinShare * kUnit;
+        if (p.many) {
+            p.one = p.one || max_pos <= 2 * kMinShare * kUnit || max_pos <= (wgs < 384 ? 15 : 24) * wgs;
+        } else {
+            p.one = p.one || max_pos <= few || max_pos <= (own ? 34 : 16) * wgs;
+            if (p.one && own && max_pos > few) p.waves = 16;
+        }
+    }
     p.shares = p.one ? B : (int)std::min(want, most);
     p.records = p.shares + B - 1;
     p.most = (int)std::min<int64_t>(longest, p.shares);
@@ -177,6 +277,14 @@ int merge_waves(const Plan& p, int B) { return p.shares <= kFew * B || p.most <=
 
 template <bool MASKED>
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
+    // 16 lanes a row where there are many.  us, a workgroup / 16 lanes: 288 rows 12.9 / 18.5, 832 18.0 / 20.0, 1536 22.6 /
+    // 23.2, 2048 23.6 / 22.8, 3328 28.3 / 26.4, 4096 47.9 / 44.1 (one sequence), 23.1 / 20.6 (eight).
+    if (p.most <= kFew && (int64_t)a.B * a.M * a.Hq >= 2048) {
+        const dim3 grid((a.M * a.Hq + 15) / 16, a.B);
+        if (D == 64) hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<64, MASKED>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<128, MASKED>), grid, dim3(256), 0, st, a);
+        return mxh::launch_status("attn_kv4 (merge of rows)");
+    }
     const int nw = merge_waves(p, a.B);
     const dim3 grid(a.M * a.Hq, a.B), block(64 * nw);
 #define MXH_M4(DD)                                                                                       \
@@ -212,7 +320,7 @@ extern "C" size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, i
 
 extern "C" size_t mxfp4_attn_kv4_masked_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos, int window, int sinks) {
     if (!takes(B, M, Hq, Hkv, D, max_pos) || window < 0 || sinks < 0) return 0;
-    return workspace_of(plan(B, M, Hq, Hkv, room_of(M, max_pos, window, sinks)), B, M, Hq, D);
+    return workspace_of(plan(B, M, Hq, Hkv, max_pos, room_of(M, max_pos, window, sinks)), B, M, Hq, D);
 }
 
 extern "C" int mxfp4_attn_kv4(const void* q, int q_dtype, int64_t ldq, const uint8_t* kq, const uint8_t* ks, const uint8_t* vq,
@@ -257,7 +365,7 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     if (window == 0) sinks = 0;
     const bool masked = window != 0 || tree;
     const int room = room_of(M, a.c.max_pos, window, sinks);
-    const Plan p = plan(B, M, Hq, Hkv, room);
+    const Plan p = plan(B, M, Hq, Hkv, a.c.max_pos, room);
     // (the threads of a launch are counted in 32 bits)
     MXH_REQUIRE(p.one || (int64_t)M * Hq * merge_waves(p, B) * 64 < (1ll << 32), "attn_kv4: M*Hq=%lld too large", (long long)M * Hq);
     const size_t need = workspace_of(p, B, M, Hq, D);
@@ -274,6 +382,9 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     a.Hq = Hq;
     a.G = Hq / Hkv;
     a.shares = p.shares;
+    a.by_G = Divisor(a.G);
+    a.by_rows = Divisor(M * a.G);
+    a.by_shares = Divisor(p.shares);
     a.records = p.records;
     a.per = B == 1 && (int64_t)p.shares * kMinShare * kUnit >= room ? kMinShare : 0;
     a.window = window;

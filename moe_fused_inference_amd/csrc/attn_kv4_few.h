@@ -124,12 +124,10 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         uint4 qw[QN];
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
-            const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-            qw[i] = make_uint4(0, 0, 0, 0);
-            if (r < rows && (R * (D / 8) % NT == 0 || tid + NT * i < R * (D / 8)))
-                qw[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)(r / G) * a.ldq + (r % G) * D + 8 * ch);
+            const int r = min((tid + NT * i) / (D / 8), rows - 1), ch = (tid + NT * i) % (D / 8), t = a.token(r);    // (rows past the last are the last)
+            qw[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)t * a.ldq + (r - t * G) * D + 8 * ch);
         }
-        // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
+        // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kv4::kNoRow: there is no such tile)
         uint32_t first[2];
         Units un{};      // (MASKED)
         auto find_rows = [&](int j0) {
@@ -138,20 +136,17 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                 int64_t u = (int64_t)u0 + wave + NW * (j0 + lane);
                 if constexpr (MASKED) u += u < un.sinks ? 0 : un.gap;
                 const int64_t pos = u * kUnit + 16 * t;
-                first[t] = kNoRow;
-                if (pos < a.c.max_pos) {
-                    const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
-                    first[t] = row < 0 ? kNoRow : (uint32_t)row;
-                }
+                first[t] = kv4::kNoRow;
+                if (pos < a.c.max_pos) first[t] = kv4::head_row32(a.c, b, g, (int)pos);
             }
         };
         const Lane<D> off(lane);
         // the wave's j-th unit: its tiles' rows, and which of them exist
         auto locate = [&](int j, uint32_t (&row)[2]) -> int {
             const uint32_t r0 = __builtin_amdgcn_readlane(first[0], j & 63), r1 = __builtin_amdgcn_readlane(first[1], j & 63);
-            row[0] = r0 == kNoRow ? 0 : r0;
-            row[1] = r1 == kNoRow ? 0 : r1;
-            return (r0 == kNoRow ? 0 : 1) | (r1 == kNoRow ? 0 : 2);
+            row[0] = r0 == kv4::kNoRow ? 0 : r0;
+            row[1] = r1 == kv4::kNoRow ? 0 : r1;
+            return (r0 == kv4::kNoRow ? 0 : 1) | (r1 == kv4::kNoRow ? 0 : 2);
         };
         Raw<D> r;
         int there = 0;
@@ -202,9 +197,9 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&qs[l16][(D / 4) * lq + 8 * kt]));
         zero = over_lq<false>(zero);
         // the lane's query is row l16; rows that are none see everything and write nothing
-        const int lim = l16 < rows ? clamped(last_seen<MASKED>(a, base, l16 / G)) : 1 << 30;
+        const int lim = l16 < rows ? clamped(last_seen<MASKED>(a, base, a.token(l16))) : 1 << 30;
         int begin = 0;
-        if constexpr (MASKED) begin = l16 < rows ? begin_of(a, b, base, l16 / G) : 0;
+        if constexpr (MASKED) begin = l16 < rows ? begin_of(a, b, base, a.token(l16)) : 0;
         float m = kNone, l = 0.0f;
         bool wide = false;   // uniform: a row's reference is past kWide
         mx::v4f acc[CT];
@@ -250,7 +245,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                     if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
                 if constexpr (MASKED) {
                     const int from = begin - p0 - 4 * lq, sinks = a.sinks - p0 - 4 * lq;
-                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min(l16 / G, a.M - 1), p0) >> (4 * lq) : ~0u;
+                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min(a.token(l16), a.M - 1), p0) >> (4 * lq) : ~0u;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int at = 16 * (i >> 2) + (i & 3);

@@ -84,15 +84,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
         auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
         const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
-        int lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base + r0 / G));        // the group's first token sees up to here
-        const int t1 = (min(r0 + R, rows) - 1) / G;                                           // its last token
+        int lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base + a.token(r0)));        // the group's first token sees up to here
+        const int t1 = a.token(min(r0 + R, rows) - 1);                                           // its last token
         const int lim_max = __builtin_amdgcn_readfirstlane(min(clamped(last_seen<MASKED>(a, base, t1)), a.c.max_pos - 1));
         // (MASKED) where the group's first and last window begin; its units: `head` of the sinks, then others
         int begin_min = 0, begin_max = 0, head = 0, tail = 0;
         if constexpr (MASKED) {
             if (a.tree) lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base - 1));
             const Units un = units<true>(a, base);
-            begin_min = __builtin_amdgcn_readfirstlane(first_begin(a, base, r0 / G));
+            begin_min = __builtin_amdgcn_readfirstlane(first_begin(a, base, a.token(r0)));
             begin_max = __builtin_amdgcn_readfirstlane(last_begin(a, base, t1));
             u1 = min(u1, lim_max < 0 ? 0 : min((int)un.n, (int)un.of_real(lim_max / kUnit) + 1));
             if (!ONE && u0 >= u1) return;                       // no row of the group sees the segment: no record
@@ -107,16 +107,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         auto real = [&](int k) { return MASKED ? k + (k < head ? u0 : tail) : u0 + k; };     // the group's k-th unit
         auto some_hide = [&](int p0) { return p0 + kUnit - 1 > lim_min || (MASKED && p0 < begin_max && p0 + kUnit > a.sinks); };
         const int n = u0 + wave < u1 ? (u1 - u0 - wave + kWaves - 1) / kWaves : 0;   // the wave's units: wave + 4 j
-        // q, whose parts go to LDS once the first units' loads are on their way
-        constexpr int NT = 64 * kWaves, QN = (R * (D / 8) + NT - 1) / NT;
-        uint4 qw[QN];
-#pragma unroll
-        for (int i = 0; i < QN; ++i) {
-            const int r = r0 + (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
-            qw[i] = make_uint4(0, 0, 0, 0);
-            if (r < rows) qw[i] = *reinterpret_cast<const uint4*>(a.q + ((int64_t)b * a.M + r / G) * a.ldq + (int64_t)(g * G + r % G) * D + 8 * ch);
-        }
-        // the first head rows of units j, j = lane, tiles 0 and 1 (kNoRow: there is no such tile)
+        // the first head rows of units j, j = lane, tiles 0 and 1 (kv4::kNoRow: there is no such tile)
         uint32_t first[2];
         auto find_rows = [&](int j0) {
 #pragma unroll
@@ -124,11 +115,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                 int64_t u = (int64_t)u0 + wave + kWaves * (j0 + lane);
                 if constexpr (MASKED) u += wave + kWaves * (j0 + lane) < head ? 0 : tail - u0;
                 const int64_t pos = u * kUnit + 16 * t;
-                first[t] = kNoRow;
-                if (pos < a.c.max_pos && j0 + lane < n) {
-                    const int64_t row = kv4::head_row(a.c, b, g, (int)pos);
-                    first[t] = row < 0 ? kNoRow : (uint32_t)row;
-                }
+                first[t] = kv4::kNoRow;
+                if (pos < a.c.max_pos && j0 + lane < n) first[t] = kv4::head_row32(a.c, b, g, (int)pos);
             }
         };
         struct Unit {
@@ -138,7 +126,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         auto locate = [&](int j) {
             if ((j & 63) == 0) find_rows(j);
             const uint32_t x = __builtin_amdgcn_readlane(first[0], j & 63), y = __builtin_amdgcn_readlane(first[1], j & 63);
-            return Unit{x == kNoRow ? 0 : x, y == kNoRow ? 0 : y, (x == kNoRow ? 0 : 1) | (y == kNoRow ? 0 : 2), (MASKED ? real(wave + kWaves * j) : u0 + wave + kWaves * j) * kUnit};
+            return Unit{x == kv4::kNoRow ? 0 : x, y == kv4::kNoRow ? 0 : y, (x == kv4::kNoRow ? 0 : 1) | (y == kv4::kNoRow ? 0 : 2), (MASKED ? real(wave + kWaves * j) : u0 + wave + kWaves * j) * kUnit};
         };
         // a unit's bytes, in few and wide loads.  K: row l32, half lh; codes: those of K's (lane < 32) or V's position l32, one
         // word; V: D/8 bytes of row 16 t + lane / 4
@@ -216,6 +204,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         Unit ua = locate(0), ub = ua, uc = ua;
         load_k(ua);
         load_v(ua);
+        // q (rows past the last are the last)
+        constexpr int NT = 64 * kWaves, QN = (R * (D / 8) + NT - 1) / NT;
+        uint4 qw[QN];
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int r = min(r0 + (tid + NT * i) / (D / 8), rows - 1), ch = (tid + NT * i) % (D / 8), t = a.token(r);
+            qw[i] = *reinterpret_cast<const uint4*>(a.q + ((int64_t)b * a.M + t) * a.ldq + (int64_t)(g * G + r - t * G) * D + 8 * ch);
+        }
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
             const int r = (tid + NT * i) / (D / 8), ch = (tid + NT * i) % (D / 8);
@@ -228,9 +224,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         __syncthreads();
         // the lane's query is row r0 + l32; rows that are none see everything and write nothing.
         // zero: 0, or NaN where the row holds an infinity or a NaN (then so is its output)
-        const int lim = r0 + l32 < rows ? clamped(last_seen<MASKED>(a, base, (r0 + l32) / G)) : 1 << 30;
+        const int lim = r0 + l32 < rows ? clamped(last_seen<MASKED>(a, base, a.token(r0 + l32))) : 1 << 30;
         int begin = 0;
-        if constexpr (MASKED) begin = r0 + l32 < rows ? begin_of(a, b, base, (r0 + l32) / G) : 0;
+        if constexpr (MASKED) begin = r0 + l32 < rows ? begin_of(a, b, base, a.token(r0 + l32)) : 0;
         float zero = 0.0f, m = kNone, l = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&lds.in.qs[l32][(D / 2) * lh + 8 * kt]));
@@ -270,7 +266,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
                     if (!(u.there >> (i >> 3) & 1) || 8 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
                 if constexpr (MASKED) {
                     const int from = begin - u.p0 - 4 * lh, sinks = a.sinks - u.p0 - 4 * lh;
-                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min((r0 + l32) / G, a.M - 1), u.p0) >> (4 * lh) : ~0u;
+                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min(a.token(r0 + l32), a.M - 1), u.p0) >> (4 * lh) : ~0u;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int at = 8 * (i >> 2) + (i & 3);
@@ -346,10 +342,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             put_v(0, ua);
             load_v(ub);
             masked(ua, s);
-            float t[16], sum;
-            terms(s, a.scale, m, wide, t, sum);
-            parts(t, pa);
-            again(s, a.scale, m, l, wide, sum, pa, over, rescale);
+            first_terms(s, a.scale, m, l, wide, pa, over);
             ua = ub;
             ub = locate(2);
             if (n > 1) scores(1, ua, s);

@@ -38,6 +38,17 @@ __device__ __forceinline__ int64_t head_row(const Cache& c, int b, int g, int po
     return ((int64_t)pid * c.Hkv + g) * c.page + r;
 }
 
+// The same of the kernels that hold rows in 32 bits, which make_cache makes enough of; kNoRow for -1.
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t head_row32(const Cache& c, int b, int g, int pos) {
+    uint32_t pid = b, r = pos;
+    if (c.pages) {
+        pid = c.pages[(int64_t)b * c.max_pages + (pos >> c.lg)];
+        r = pos & (c.page - 1);
+    }
+    return c.pages && pid >= (uint32_t)c.n_pages ? kNoRow : (pid * (uint32_t)c.Hkv + (uint32_t)g) * (uint32_t)c.page + r;
+}
+
 // 2^(code - 127) for the packed conversions, which read the exponent field: 0
 // stands for 2^-127 there and 255 for NaN, as in E8M0.
 __device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_float(code << 23); }

@@ -23,7 +23,7 @@ def test_refusals():
     _refused(_attn(sinks=1), "without a window")
     _refused(_attn(window=2, tree=P), "for a tree of 3")
     _refused(_attn(tree=P + 2), "4-byte aligned")
-    for kw in (dict(), dict(window=100, sinks=4), dict(tree=P)):
+    for kw in (dict(), dict(window=4000, sinks=4), dict(tree=P)):
         _refused(_attn(**kw, ws=None), "workspace")
         _refused(_attn(**kw, wsb=16), "workspace")
         _refused(_attn(**kw, o=None), "no output")
@@ -43,6 +43,23 @@ def test_workspace_sizes():
     for a in ((1, 1, 32, 4, 128, 32768, -1, 0), (1, 1, 32, 4, 128, 32768, 5, -1), (1, 1 << 30, 128, 1, 128, 4096, 5, 0), (1, 1, 7, 4, 128, 64, 5, 0),
               (2 ** 31 - 1,) * 8):
         assert size(*a) == 0, a
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are never read: needs a machine without a GPU")
+@pytest.mark.parametrize("B,M,Hq,Hkv", [(1, 1, 32, 4), (8, 1, 32, 4), (8, 2, 16, 8), (100, 1, 8, 8), (1, 40, 32, 4), (3, 9, 8, 2)])
+@pytest.mark.parametrize("tree", [None, P])
+def test_the_workspace_that_a_call_asks_for(B, M, Hq, Hkv, tree):
+    """What the size function says is enough, and a byte less is not: at every window, also those that reach everything."""
+    page, size = 4096, _lib.load().mxfp4_attn_kv4_masked_workspace_size
+    for window in [0] + sorted({max(M, 1 << i) + j for i in range(14) for j in (0, 1)} | {page + j for j in (-70, -33, -1, 0, M - 1, M, M + 1)}):
+        for sinks in (0, 4) if window else (0,):
+            n = size(B, M, Hq, Hkv, 128, page, window, sinks)
+            kw = dict(window=window, sinks=sinks, tree=tree, B=B, M=M, Hq=Hq, Hkv=Hkv, page=page)
+            args = lambda wsb: _lib.load().mxfp4_attn_kv4_masked(P, 0, Hq * 128, P, P, P, P, None, B, page, 0, P, window, sinks, tree, P, 2, None, None, B, M,
+                                                                 Hq, Hkv, 128, P if wsb else None, wsb, None)
+            assert args(n) == 100, kw         # hipErrorNoDevice: it came to the launch
+            if n:
+                assert args(n - 1) == -1, kw
 
 
 def test_binding():
