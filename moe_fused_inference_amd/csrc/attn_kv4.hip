@@ -226,8 +226,10 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos, int room) {
         // 2048 16.5 / 18.5; but B = 8, 2048 15.4 / 11.8, B = 1, 1024 10.8 / 8.1.
         if (longest > 1 && max_pos <= 2048 && wgs >= 128 && wgs <= 256) p.waves = 16;
     }
-    // shares of the whole batch for one round of workgroups, four or two a CU, and none that starts a second round
-    const int64_t want = std::max<int64_t>(1, (p.many ? 512 : 1024) / ((int64_t)Hkv * p.groups));
+    // shares of the whole batch for one round of workgroups, four or two a CU (up to 16 rows with a window three: four / three,
+    // us: 8 sequences, 4096 positions 17.9 / 15.8, 32 of 8192 41.4 / 39.8, of 16384 67.6 / 62.1, one 10.1 / 10.1), and none that
+    // starts a second round
+    const int64_t want = std::max<int64_t>(1, (p.many ? 512 : window ? 768 : 1024) / ((int64_t)Hkv * p.groups));
     // A workgroup for a sequence, no shares and no merge, where there are many and short ones.  us, shares / one, one
     // token, sequences of one length and (in brackets) of 0 .. that: 512 workgroups, 2048 positions 43.9 / 31.1 (30.8 /
     // 26.0), 4096 63.5 / 57.3 (38.2 / 49.2); 2048 workgroups, 8192 positions 446 / 406 (238 / 247).  Nine tokens, 384
