@@ -167,12 +167,18 @@ class DecodeStep:
     runs in launches of its own: attn_front and attn_next, which put the FP8
     cache's into the MoE launch, do not apply.  us a layer (32 / 4 heads, hidden
     2048, 1/8 of the head with it; FP8 / MXFP4): one token, 4000 positions 38.6 /
-    43.4, 32000 57.7 / 47.2; four tokens 62.8 / 66.1, 80.3 / 74.1."""
+    43.4, 32000 57.7 / 47.2; four tokens 62.8 / 66.1, 80.3 / 74.1.
+
+    window, sinks (kv="mxfp4"): every layer's attention sees the last `window`
+    positions up to a token's own, and the first `sinks`."""
 
     def __init__(self, model, cfg, M=1, max_pos=4096, device="cuda", fused_router=True, qkv_tail=True,
-                 attn_front=True, attn_next=True, kv="fp8"):
+                 attn_front=True, attn_next=True, kv="fp8", window=None, sinks=0):
         if kv not in ("fp8", "mxfp4"):
             raise RuntimeError(f"kv must be 'fp8' or 'mxfp4', got {kv!r}")
+        if window is not None and (kv != "mxfp4" or window <= 0) or sinks < 0 or (sinks and window is None):
+            raise RuntimeError(f"a window is positive, sinks need one, and both the MXFP4 cache, got kv={kv!r} window={window} sinks={sinks}")
+        self.window, self.sinks = min(int(window or 0), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1)   # 0: none
         self.lib = _lib.load()
         self.model, self.cfg, self.M, self.max_pos = model, cfg, int(M), int(max_pos)
         self.kv_codec = 0 if self.M == 1 else 1   # kv_write's codec / torch float8_e4m3fn
@@ -227,7 +233,7 @@ class DecodeStep:
         buf("arg_ws", ((nb + 255) // 256 * 256,), u8)   # zero-filled once; each call leaves it so
         self.kv4 = None
         if kv == "mxfp4":
-            nb = self.lib.mxfp4_attn_kv4_workspace_size(1, M, Hq, Hkv, D, self.max_pos)
+            nb = self.lib.mxfp4_attn_kv4_masked_workspace_size(1, M, Hq, Hkv, D, self.max_pos, self.window, self.sinks)
             buf("attn_ws", (max(16, (nb + 15) // 16 * 16),), u8)
             buf("q", (M, Hq, D), bf16)
             self.kv4 = [kv4.empty_cache(1, self.max_pos, Hkv, D, device) for _ in range(c.n_layers)]
@@ -323,9 +329,9 @@ class DecodeStep:
             self._ck(lib.mxfp4_qk_norm_rope_kv4(qkv.data_ptr(), lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), c.rms_eps,
                                                 c.rope_theta, *cache, 1, M, Hq, Hkv, D, b.q.data_ptr(), s),
                      "qk_norm_rope_kv4")
-            self._ck(lib.mxfp4_attn_kv4(b.q.data_ptr(), _DT_BF16, Hq * D, *cache, None, _DT_F32, b.aq.data_ptr(),
-                                        b.as_.data_ptr(), 1, M, Hq, Hkv, D, b.attn_ws.data_ptr(), b.attn_ws.numel(),
-                                        s), "attn_kv4")
+            self._ck(lib.mxfp4_attn_kv4_masked(b.q.data_ptr(), _DT_BF16, Hq * D, *cache, self.window, self.sinks, None,
+                                               None, _DT_F32, b.aq.data_ptr(), b.as_.data_ptr(), 1, M, Hq, Hkv, D,
+                                               b.attn_ws.data_ptr(), b.attn_ws.numel(), s), "attn_kv4")
             self._lin(b.aq, b.as_, lw.o, H, Hq * D, b.oproj, s)
             return
         kvk, kvv = b.kvk[l], b.kvv[l]

@@ -127,8 +127,8 @@ def tree_masks(parents):
 def kv4_keep(caches, dpos, path, pages=None):
     """What stays of a verified tree moves together: the rows at positions dpos[b] + path[b, k] go to dpos[b] + k, in
     a cache or each of a list of them (a model's layers, one launch for 64).  path (int32 (B, A)): drafts in the
-    order of their line, so path[b, k] >= k (others stay where they are), -1 from its end on."""
-    if isinstance(caches[0], torch.Tensor):
+    order of their line, so path[b, k] >= k (others stay where they are), -1 from its end on.  Each cache is named once."""
+    if len(caches) and isinstance(caches[0], torch.Tensor):
         caches = [caches]
     _ext().keep(caches, dpos, path, pages)
 
