@@ -547,7 +547,8 @@ __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, 
 // How a call's work is laid out (attn_kv4.hip).
 struct Plan {
     bool many;       // rows for attn_rows
-    int groups, shares, most;   // shares of the batch (with `one` a sequence each), and one sequence may have
+    int groups, shares, most;   // shares of the batch (with `one` a sequence each), and one sequence has, about
+    int across;      // shares that a sequence may lie in, at most
     int records;     // of a row
     int waves;       // of a workgroup
     bool one;

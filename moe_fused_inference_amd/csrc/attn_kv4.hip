@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     store<CT>(a.out, ((int64_t)b * a.M + rs.token) * a.Hq + rs.g * a.G + rs.head, D, CT * tid, x);
 }
 
-// The same, to the same bits, where there are many rows of up to kFew records: 16 lanes a row, a lane D / 16 columns, with
+// The same, to the same bits, where there are many rows of up to kFew records (Plan::across): 16 lanes a row, a lane D / 16 columns, with
 // the four waves' sums of the kernel above as four in registers.
 template <int D, bool MASKED>
 __global__ __launch_bounds__(256) void attn_kv4_merge_rows_kernel(Args a) {
@@ -211,6 +211,7 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos, int room) {
     max_pos = room;
     const int64_t rows = (int64_t)M * (Hq / Hkv);
     int64_t longest = (max_pos + kMinShare * kUnit - 1) / (kMinShare * kUnit);   // shares a sequence may have (share_units)
+    const int64_t across = longest + (B > 1 ? 1 : 0);                            // where it begins within one, and others are short
     if (longest > kFew) longest = std::max<int64_t>(kFew, (longest + 1) / 2);
     const int64_t most = B * (longest + (B > 1 ? kPad / kMinShare : 0));   // with a share of whole pads
     p.waves = 4;
@@ -260,6 +261,7 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos, int room) {
     p.shares = p.one ? B : (int)std::min(want, most);
     p.records = p.shares + B - 1;
     p.most = (int)std::min<int64_t>(longest, p.shares);
+    p.across = (int)std::min<int64_t>(across, p.shares);
     return p;
 }
 
@@ -281,7 +283,7 @@ template <bool MASKED>
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
     // 16 lanes a row where there are many.  us, a workgroup / 16 lanes: 288 rows 12.9 / 18.5, 832 18.0 / 20.0, 1536 22.6 /
     // 23.2, 2048 23.6 / 22.8, 3328 28.3 / 26.4, 4096 47.9 / 44.1 (one sequence), 23.1 / 20.6 (eight).
-    if (p.most <= kFew && (int64_t)a.B * a.M * a.Hq >= 2048) {
+    if (p.across <= kFew && (int64_t)a.B * a.M * a.Hq >= 2048) {
         const dim3 grid((a.M * a.Hq + 15) / 16, a.B);
         if (D == 64) hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<64, MASKED>), grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<128, MASKED>), grid, dim3(256), 0, st, a);
