@@ -111,7 +111,7 @@ struct Args {
     Divisor by_G, by_rows, by_shares;   // by_rows: M * G
     __device__ __forceinline__ int token(int r) const { return (int)by_G((uint32_t)r); }    // of row r of a kv head
     float scale;                 // log2(e) / sqrt(D)
-    // Of the kernels with masks (MASKED) alone
+    // Of the kernels with masks (MASKS) alone
     int window, sinks;           // a token sees the last `window` positions up to its own (0: all), and the first `sinks`
     const uint32_t* tree;        // or null: (B, M, words), bit i of a token's words: it sees the call's i-th
     int words;
@@ -123,9 +123,11 @@ __device__ __forceinline__ uint32_t units_of(const Args& a, int base) {
     return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
 }
 
-// Masks.  With a window the units between the sinks and the first position that any
+// Masks, each kernel's a constant: with both as one that asks what there is, a call of trees took 3 to 9 % more (16 of 64
+// drafts over 16384 positions 488 us, 466; 7 of 5 drafts, 5 heads of 64, 10.9, 9.7).  With a window the units between the sinks and the first position that any
 // token's window reaches are no work: a sequence's units are counted without them (unit
 // v stands for v, or v + gap past the sinks), here, in the shares, and in the merge.
+constexpr int kWindow = 1, kTree = 2;      // MASKS: one, both, or 0
 struct Units {
     uint32_t n, sinks, gap;
     __device__ __forceinline__ uint32_t real(uint32_t v) const { return v < sinks ? v : v + gap; }
@@ -135,32 +137,29 @@ struct Units {
 // line: base + (what it sees of the call) - 1.  The first and the last begin of tokens
 // t0 .. t1 (with a tree of any; a token that sees none of the call is taken to stand at base - 1).
 __device__ __forceinline__ int clamp_pos(const Args& a, int64_t pos) { return (int)(pos < 0 ? 0 : pos < a.c.max_pos ? pos : a.c.max_pos); }
+template <int MASKS>
 __device__ __forceinline__ int first_begin(const Args& a, int base, int t0) {
-    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? 0 : t0 + 1)) : 0;
+    return MASKS & kWindow ? clamp_pos(a, (int64_t)base - a.window + (MASKS & kTree ? 0 : t0 + 1)) : 0;
 }
+template <int MASKS>
 __device__ __forceinline__ int last_begin(const Args& a, int base, int t1) {
-    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? a.M : t1 + 1)) : 0;
+    return MASKS & kWindow ? clamp_pos(a, (int64_t)base - a.window + (MASKS & kTree ? a.M : t1 + 1)) : 0;
 }
-template <bool MASKED>
+template <int MASKS>
 __device__ __forceinline__ Units units(const Args& a, int base) {
     Units u{units_of(a, base), 0, 0};
-    if constexpr (MASKED) {
-        if (a.window) {
-            const uint32_t from = min((uint32_t)first_begin(a, base, 0) / kUnit, u.n);
-            u.sinks = min((uint32_t)(a.sinks + kUnit - 1) / kUnit, u.n);
-            u.gap = from > u.sinks ? from - u.sinks : 0;
-            u.n -= u.gap;
-        }
+    if constexpr (MASKS & kWindow) {
+        const uint32_t from = min((uint32_t)first_begin<MASKS>(a, base, 0) / kUnit, u.n);
+        u.sinks = min((uint32_t)(a.sinks + kUnit - 1) / kUnit, u.n);
+        u.gap = from > u.sinks ? from - u.sinks : 0;
+        u.n -= u.gap;
     }
     return u;
 }
 // The last position that token t sees, if it is in the cache.
-template <bool MASKED>
+template <int MASKS>
 __device__ __forceinline__ int64_t last_seen(const Args& a, int base, int t) {
-    if constexpr (MASKED) {
-        if (a.tree) return min((int64_t)base + a.M, (int64_t)a.c.max_pos) - 1;
-    }
-    return (int64_t)base + t;
+    return MASKS & kTree ? min((int64_t)base + a.M, (int64_t)a.c.max_pos) - 1 : (int64_t)base + t;
 }
 // Words of token t of sequence b, and how many of the call it sees.
 __device__ __forceinline__ const uint32_t* tree_row(const Args& a, int b, int t) { return a.tree + ((int64_t)b * a.M + t) * a.words; }
@@ -181,8 +180,9 @@ __device__ __forceinline__ uint32_t tree_bits(const Args& a, int b, int base, in
     return __builtin_amdgcn_alignbit(hi, lo, (uint32_t)d & 31u);
 }
 // Where token t's window begins.
+template <int MASKS>
 __device__ __forceinline__ int begin_of(const Args& a, int b, int base, int t) {
-    return a.window ? clamp_pos(a, (int64_t)base - a.window + (a.tree ? tree_count(a, b, t) : t + 1)) : 0;
+    return MASKS & kWindow ? clamp_pos(a, (int64_t)base - a.window + (MASKS & kTree ? tree_count(a, b, t) : t + 1)) : 0;
 }
 // Inclusive prefix sums over the wave (every lane active).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
@@ -217,14 +217,14 @@ struct Place {
     uint64_t start;
 };
 // Share blockIdx.x's first sequence; false: it is past the line.
-template <bool MASKED>
+template <int MASKS>
 __device__ __forceinline__ bool find_share(const Args& a, Place& p) {
     const int lane = threadIdx.x & 63;
     auto places = [&](int b0, int& base) {
         base = 0;
         if (b0 + lane >= a.B) return 0u;
         base = a.dpos[b0 + lane];
-        const uint32_t n = units<MASKED>(a, base).n;
+        const uint32_t n = units<MASKS>(a, base).n;
         return n ? n + kPad : 0u;
     };
     int base;
@@ -273,7 +273,7 @@ enum class Work {
     kLine,       // a share of the line
 };
 // Its sequences in turn: segment(b, its dpos, its units u0 .. u1 - 1).
-template <Work W, bool MASKED, class Segment>
+template <Work W, int MASKS, class Segment>
 __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
     if constexpr (W == Work::kSequence) {
         segment(blockIdx.x, __builtin_amdgcn_readfirstlane(a.dpos[blockIdx.x]), 0, INT32_MAX);
@@ -282,18 +282,18 @@ __device__ __forceinline__ void each_segment(const Args& a, Segment segment) {
     if constexpr (W == Work::kShare) {      // (a kernel of its own: nine tokens over 23001 positions 25.1 us, in the loop 25.8)
         const int base = a.dpos[0];         // (in flight, where nothing here needs it)
         uint32_t per = a.per;
-        if (per == 0) per = share_units(units<MASKED>(a, __builtin_amdgcn_readfirstlane(base)).n, a);
+        if (per == 0) per = share_units(units<MASKS>(a, __builtin_amdgcn_readfirstlane(base)).n, a);
         if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.places[0] = make_int4(0, 0, (int)per, 0);
         const uint32_t u0 = blockIdx.x * per;
         segment(0, base, (int)u0, (int)(u0 + per));
         return;
     }
     Place p;
-    if (!find_share<MASKED>(a, p)) return;             // uniform
+    if (!find_share<MASKS>(a, p)) return;             // uniform
     const uint64_t from = (uint64_t)blockIdx.x * p.per;
     constexpr int pad = kPad;
     for (bool first = true;;) {
-        const int n = (int)units<MASKED>(a, p.base).n;
+        const int n = (int)units<MASKS>(a, p.base).n;
         // the share's beginning and end in units of the sequence, which ends past `from` (per < 2^28)
         const int u1 = (int)min((int64_t)n, (int64_t)(from + p.per - p.start) - pad);
         const int u0 = (int)max((int64_t)0, (int64_t)from - (int64_t)p.start - pad);
@@ -472,7 +472,7 @@ __device__ __forceinline__ void mark_not_finite(const Args& a, int b, int base, 
 
 // The same with masks: unit_at(k) is the k-th unit of the workgroup, of n; the wave has
 // every NW-th.  some_hide(first position): not all of the workgroup's rows see all of it.
-template <int D, int NW, class UnitAt, class SomeHide>
+template <int D, int NW, int MASKS, class UnitAt, class SomeHide>
 __device__ __forceinline__ void mark_not_finite_masked(const Args& a, int b, int base, int g, int r0, int rows, int wave, int n, int last,
                                                        UnitAt unit_at, SomeHide some_hide, float (*mo)[D + 4]) {
     asm volatile("" ::: "memory");
@@ -487,8 +487,9 @@ __device__ __forceinline__ void mark_not_finite_masked(const Args& a, int b, int
                 if (!(kv4::not_finite(w, a.c.vs[row * (D / 32) + col / 32]) & 1)) continue;
                 for (int r = 0; r < rows; ++r) {
                     const int t = (r0 + r) / a.G;
-                    const bool sees = pos <= last_seen<true>(a, base, t) && (pos >= begin_of(a, b, base, t) || pos < a.sinks) &&
-                                      (!a.tree || tree_bits(a, b, base, t, pos) & 1);
+                    const bool sees = pos <= last_seen<MASKS>(a, base, t) &&
+                                      (!(MASKS & kWindow) || pos >= begin_of<MASKS>(a, b, base, t) || pos < a.sinks) &&
+                                      (!(MASKS & kTree) || tree_bits(a, b, base, t, pos) & 1);
                     if (sees) mo[r][col] = __builtin_nanf("");
                 }
             }
@@ -499,15 +500,15 @@ __device__ __forceinline__ void mark_not_finite_masked(const Args& a, int b, int
 // The end of row r of kv head g of sequence b, a segment from unit u0 on: NW waves' (m, l,
 // columns) to one record, or with ONE the output.  16 neighbouring lanes a row (by
 // tid), which all call it, D / 16 columns a lane.
-template <int D, int NW, bool ONE, bool MASKED, class M, class L, class O>
+template <int D, int NW, bool ONE, int MASKS, class M, class L, class O>
 __device__ __forceinline__ void finish(const Args& a, int tid, int b, int base, int g, int r, int u0, M m_of, L l_of, O o_of) {
     constexpr int CT = D / 16;
     const int c0 = CT * (tid & 15);
     const int t = a.token(r);
     const int64_t pos = (int64_t)base + t;
     if (!ONE && (pos < 0 || pos >= a.c.max_pos)) return;                      // no record: the merge reads none
-    if constexpr (!ONE && MASKED) {
-        if ((uint32_t)u0 > units<true>(a, base).of_real((uint32_t)last_seen<true>(a, base, t) / kUnit)) return;
+    if constexpr (!ONE && MASKS != 0) {
+        if ((uint32_t)u0 > units<MASKS>(a, base).of_real((uint32_t)last_seen<MASKS>(a, base, t) / kUnit)) return;
     } else if (!ONE) {
         if ((int64_t)u0 * kUnit > pos) return;
     }
@@ -555,10 +556,14 @@ struct Plan {
 };
 
 // Up to 16 query rows of a kv head (attn_kv4_few.h); much: K by streaming loads.  And more (attn_kv4_rows.h), in groups of
-// 32; exact: p in three bf16 parts instead of two.  Without masks, and with.
+// 32; exact: p in three bf16 parts instead of two.  A file each for its masks.
 int attn_few(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
-int attn_few_masked(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
+int attn_few_window(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
+int attn_few_tree(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
+int attn_few_tree_window(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st);
 int attn_rows(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
-int attn_rows_masked(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
+int attn_rows_window(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
+int attn_rows_tree(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
+int attn_rows_tree_window(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st);
 
 }  // namespace mxa

@@ -55,13 +55,13 @@ struct Records {
     int g, token, head, n;
     const float* at;
 };
-template <int D, bool MASKED>
+template <int D, int MASKS>
 __device__ __forceinline__ Records records_of(const Args& a, int4 p, int base, int b, int row) {
     const int rows = a.M * a.G, g = (int)a.by_rows(row), r = row - g * rows, t = a.token(r);
     const int64_t pos = (int64_t)base + t;
     // those of the shares with its sequence's units up to the last that it sees
     uint32_t top = (uint32_t)(pos / kUnit);
-    if constexpr (MASKED) top = units<true>(a, base).of_real((uint32_t)(last_seen<true>(a, base, t) / kUnit));
+    if constexpr (MASKS != 0) top = units<MASKS>(a, base).of_real((uint32_t)(last_seen<MASKS>(a, base, t) / kUnit));
     const int n = pos < 0 || pos >= a.c.max_pos ? 0 : min((int)(((uint32_t)p.y + top) / (uint32_t)p.z) + 1, a.shares - p.x);
     return Records{g, t, r - t * a.G, n, a.part + ((int64_t)row * a.records + p.x + b) * (D + 4)};
 }
@@ -69,7 +69,7 @@ __device__ __forceinline__ Records records_of(const Args& a, int4 p, int base, i
 // Workgroup (row of kv head g: blockIdx.x = g * rows + r, sequence b): the row's
 // records dealt to NW waves, eight loaded at a time (one memory latency for up to
 // 8 NW), each with a running reference; a lane holds D / 64 columns.
-template <int D, int NW, bool MASKED>
+template <int D, int NW, int MASKS>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     constexpr int C = D / 64, CT = D / 16, N = 8;
     typedef float cvec __attribute__((ext_vector_type(C)));
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = blockIdx.y;
-    const Records rs = records_of<D, MASKED>(a, a.places[b], a.dpos[b], b, blockIdx.x);
+    const Records rs = records_of<D, MASKS>(a, a.places[b], a.dpos[b], b, blockIdx.x);
     const int ns = __builtin_amdgcn_readfirstlane(rs.n);
     const float* rec = rs.at;
     float m = kNone, l = 0.0f;
@@ -137,12 +137,12 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_merge_kernel(Args a) {
 
 // The same, to the same bits, where there are many rows of up to kFew records (Plan::across): 16 lanes a row, a lane D / 16 columns, with
 // the four waves' sums of the kernel above as four in registers.
-template <int D, bool MASKED>
+template <int D, int MASKS>
 __global__ __launch_bounds__(256) void attn_kv4_merge_rows_kernel(Args a) {
     constexpr int CT = D / 16, N = 4;
     const int tid = threadIdx.x, t = tid & 15, b = blockIdx.y;
     const int row = blockIdx.x * 16 + (tid >> 4), total = a.M * a.Hq;
-    const Records rs = records_of<D, MASKED>(a, a.places[b], a.dpos[b], b, min(row, total - 1));
+    const Records rs = records_of<D, MASKS>(a, a.places[b], a.dpos[b], b, min(row, total - 1));
     // the states of records t and t + 16, and the reference of those of t's class modulo 4
     float2 st[2];
     float ref = kNone;
@@ -279,22 +279,22 @@ bool takes(int B, int M, int Hq, int Hkv, int D, int max_pos) {
 // shares) 23.4 / 23.4 / 25.2; one token over 16000, 16 heads (64 shares) 15.8 / 15.3 / 16.3
 int merge_waves(const Plan& p, int B) { return p.shares <= kFew * B || p.most <= kFew ? 4 : p.most <= 2 * kFew ? 8 : 16; }
 
-template <bool MASKED>
+template <int MASKS>
 int merge(const Args& a, const Plan& p, int D, hipStream_t st) {
     // 16 lanes a row where there are many.  us, a workgroup / 16 lanes: 288 rows 12.9 / 18.5, 832 18.0 / 20.0, 1536 22.6 /
     // 23.2, 2048 23.6 / 22.8, 3328 28.3 / 26.4, 4096 47.9 / 44.1 (one sequence), 23.1 / 20.6 (eight).
     if (p.across <= kFew && (int64_t)a.B * a.M * a.Hq >= 2048) {
         const dim3 grid((a.M * a.Hq + 15) / 16, a.B);
-        if (D == 64) hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<64, MASKED>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<128, MASKED>), grid, dim3(256), 0, st, a);
+        if (D == 64) hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<64, MASKS>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attn_kv4_merge_rows_kernel<128, MASKS>), grid, dim3(256), 0, st, a);
         return mxh::launch_status("attn_kv4 (merge of rows)");
     }
     const int nw = merge_waves(p, a.B);
     const dim3 grid(a.M * a.Hq, a.B), block(64 * nw);
 #define MXH_M4(DD)                                                                                       \
-    if (nw == 4) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 4, MASKED>), grid, block, 0, st, a);      \
-    else if (nw == 8) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 8, MASKED>), grid, block, 0, st, a); \
-    else hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 16, MASKED>), grid, block, 0, st, a)
+    if (nw == 4) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 4, MASKS>), grid, block, 0, st, a);      \
+    else if (nw == 8) hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 8, MASKS>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((attn_kv4_merge_kernel<DD, 16, MASKS>), grid, block, 0, st, a)
     if (D == 64) { MXH_M4(64); } else { MXH_M4(128); }
 #undef MXH_M4
     return mxh::launch_status("attn_kv4 (merge)");
@@ -315,7 +315,7 @@ size_t workspace_of(const Plan& p, int B, int M, int Hq, int D) {
 }  // namespace
 
 int mxa::attn_few(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st) {
-    return launch_few<false>(a, q_dtype, p, D, much, st);
+    return launch_few<0>(a, q_dtype, p, D, much, st);
 }
 
 extern "C" size_t mxfp4_attn_kv4_workspace_size(int B, int M, int Hq, int Hkv, int D, int max_pos) {
@@ -367,7 +367,6 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     const bool exact = (o && o_dtype == MXFP4_DT_F32) || oq;
     if (window >= (int64_t)a.c.max_pos + (tree ? M : 0)) window = 0;      // it reaches every position
     if (window == 0) sinks = 0;
-    const bool masked = window != 0 || tree;
     const int room = room_of(M, a.c.max_pos, window, sinks);
     const Plan p = plan(B, M, Hq, Hkv, a.c.max_pos, room);
     // (the threads of a launch are counted in 32 bits)
@@ -398,8 +397,13 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     a.scale = (float)(1.4426950408889634 / sqrt((double)D));
     const hipStream_t st = mxh::as_stream(stream);
     const bool much = std::min((int64_t)B * room, (int64_t)n_pages * page) * Hkv * (D + D / 16) > kMuch;
-    const int rl = p.many ? (masked ? attn_rows_masked : attn_rows)(a, q_dtype, p, D, exact, st)
-                          : (masked ? attn_few_masked : attn_few)(a, q_dtype, p, D, much, st);
+    const int masks = (window ? kWindow : 0) | (tree ? kTree : 0);
+    using Few = decltype(&attn_few);
+    using Rows = decltype(&attn_rows);
+    static constexpr Few few[4] = {attn_few, attn_few_window, attn_few_tree, attn_few_tree_window};
+    static constexpr Rows rows[4] = {attn_rows, attn_rows_window, attn_rows_tree, attn_rows_tree_window};
+    const int rl = p.many ? rows[masks](a, q_dtype, p, D, exact, st) : few[masks](a, q_dtype, p, D, much, st);
     if (rl != MXFP4_OK || p.one) return rl;
-    return masked ? merge<true>(a, p, D, st) : merge<false>(a, p, D, st);
+    static constexpr decltype(&merge<0>) join[4] = {merge<0>, merge<kWindow>, merge<kTree>, merge<kWindow | kTree>};
+    return join[masks](a, p, D, st);
 }

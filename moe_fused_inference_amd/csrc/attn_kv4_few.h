@@ -1,6 +1,6 @@
 // attn_kv4_few.h -- the kernel of attention over the MXFP4 KV cache for up to 16 query rows
 // of a kv head (attn_kv4.hip has its contract, mathematics and figures), without masks
-// (attn_kv4.hip) and with (attn_kv4_masked.hip).
+// (attn_kv4.hip) and with (attn_kv4_window.hip, attn_kv4_tree.hip, attn_kv4_tree_window.hip).
 #pragma once
 #include "attn_kv4.h"
 #include "kv4.h"
@@ -99,9 +99,9 @@ __device__ __forceinline__ void decode_v(const uint32_t (&v)[8], const float (&s
     for (int c = 0; c < 4; ++c) vd[c] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
 }
 
-template <int D, int NQ, Work W, int NW, bool STREAM, bool MASKED>
+template <int D, int NQ, Work W, int NW, bool STREAM, int MASKS>
 __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
-    constexpr bool ONE = W == Work::kSequence;
+    constexpr bool ONE = W == Work::kSequence, WINDOW = MASKS & kWindow, TREE = MASKS & kTree;
     constexpr int R = 16, KT = D / 32, CT = D / 16;
     // q, and after the last unit the waves' sums
     __shared__ union Lds {
@@ -129,12 +129,12 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         }
         // the first head rows of the wave's units u0 + wave + NW j, j = lane, tiles 0 and 1 (kv4::kNoRow: there is no such tile)
         uint32_t first[2];
-        Units un{};      // (MASKED)
+        Units un{};      // (WINDOW)
         auto find_rows = [&](int j0) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 int64_t u = (int64_t)u0 + wave + NW * (j0 + lane);
-                if constexpr (MASKED) u += u < un.sinks ? 0 : un.gap;
+                if constexpr (WINDOW) u += u < un.sinks ? 0 : un.gap;
                 const int64_t pos = u * kUnit + 16 * t;
                 first[t] = kv4::kNoRow;
                 if (pos < a.c.max_pos) first[t] = kv4::head_row32(a.c, b, g, (int)pos);
@@ -157,25 +157,25 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
             load_k<STREAM>(r, a.c, row, off);
             load_v(r, a.c, row, off);
         };
-        if constexpr (W == Work::kShare && !MASKED) first_loads();        // of a share of fixed length before dpos is there: what no token sees is masked
+        if constexpr (W == Work::kShare && !WINDOW) first_loads();        // of a share of fixed length before dpos is there: what no token sees is masked
         base = __builtin_amdgcn_readfirstlane(base);
         // Positions fit 31 bits: a token before the cache is put at -1, one past it at its end
         auto clamped = [&](int64_t pos) { return (int)(pos < 0 ? -1 : pos < a.c.max_pos ? pos : a.c.max_pos); };
         const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
         int lim_min = clamped(base);                                  // the first token sees up to here
-        // (MASKED) where the first and the last window begin, and units that some row does not see whole
+        if constexpr (TREE) lim_min = clamped((int64_t)base - 1);     // (and of the drafts its own line)
+        // (WINDOW) where the first and the last window begin, and units that some row does not see whole
         int begin_min = 0, begin_max = 0;
-        if constexpr (MASKED) {
-            if (a.tree) lim_min = clamped((int64_t)base - 1);
-            un = units<true>(a, base);
-            begin_min = first_begin(a, base, 0);
-            begin_max = last_begin(a, base, a.M - 1);
+        if constexpr (WINDOW) {
+            un = units<MASKS>(a, base);
+            begin_min = first_begin<MASKS>(a, base, 0);
+            begin_max = last_begin<MASKS>(a, base, a.M - 1);
             u1 = min(u1, (int)un.n);
         } else {
             u1 = min(u1, (last + kUnit) / kUnit);
         }
-        auto some_hide = [&](int p0) { return p0 + kUnit - 1 > lim_min || (MASKED && p0 < begin_max && p0 + kUnit > a.sinks); };
-        if constexpr (W == Work::kShare && !MASKED) {
+        auto some_hide = [&](int p0) { return p0 + kUnit - 1 > lim_min || (WINDOW && p0 < begin_max && p0 + kUnit > a.sinks); };
+        if constexpr (W == Work::kShare && !WINDOW) {
             if (u0 >= u1) return;                               // no record: the merge reads none
         } else {
             if (W == Work::kShare && u0 >= u1) return;
@@ -197,9 +197,9 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&qs[l16][(D / 4) * lq + 8 * kt]));
         zero = over_lq<false>(zero);
         // the lane's query is row l16; rows that are none see everything and write nothing
-        const int lim = l16 < rows ? clamped(last_seen<MASKED>(a, base, a.token(l16))) : 1 << 30;
+        const int lim = l16 < rows ? clamped(last_seen<MASKS>(a, base, a.token(l16))) : 1 << 30;
         int begin = 0;
-        if constexpr (MASKED) begin = l16 < rows ? begin_of(a, b, base, a.token(l16)) : 0;
+        if constexpr (WINDOW) begin = l16 < rows ? begin_of<MASKS>(a, b, base, a.token(l16)) : 0;
         float m = kNone, l = 0.0f;
         bool wide = false;   // uniform: a row's reference is past kWide
         mx::v4f acc[CT];
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         // behind one the compiler waits for the older loads as if these had not been issued, that is for all)
         auto unit = [&](int u, int j, auto more_) {
             constexpr bool more = decltype(more_)::value;
-            const int p0 = (MASKED ? (int)un.real(u) : u) * kUnit;
+            const int p0 = (WINDOW ? (int)un.real(u) : u) * kUnit;
             uint32_t next[2];
             int there_next = 0;
             if constexpr (more) {
@@ -243,14 +243,19 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (!(there >> (i >> 2) & 1) || 16 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
-                if constexpr (MASKED) {
+                if constexpr (WINDOW) {
                     const int from = begin - p0 - 4 * lq, sinks = a.sinks - p0 - 4 * lq;
-                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min(a.token(l16), a.M - 1), p0) >> (4 * lq) : ~0u;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int at = 16 * (i >> 2) + (i & 3);
-                        if ((at < from && at >= sinks) || !(bits >> at & 1)) s[i] = -INFINITY;
+                        if (at < from && at >= sinks) s[i] = -INFINITY;
                     }
+                }
+                if constexpr (TREE) {
+                    const uint32_t bits = tree_bits(a, b, base, min(a.token(l16), a.M - 1), p0) >> (4 * lq);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!(bits >> (16 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
                 }
             }
             uint4 p[1][kParts];
@@ -277,7 +282,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                         r.v[i] = 0;
                         vs[i] = 1.0f;
                     }
-                if constexpr (MASKED) {      // or before the first window
+                if constexpr (WINDOW) {      // or before the first window
                     const int from = begin_min - p0 - 4 * lq, sinks = a.sinks - p0 - 4 * lq;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -289,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
                     }
                 }
                 // nor may what only some rows see reach the others'
-                if (MASKED ? (lim_min < last || begin_min < begin_max) && some_hide(p0) : p0 + kUnit - 1 > lim_min && lim_min < last) {
+                if (WINDOW ? (lim_min < last || begin_min < begin_max) && some_hide(p0) : p0 + kUnit - 1 > lim_min && lim_min < last) {
                     uint32_t large = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) large = max(large, __float_as_uint(vs[i]) & 0x7F800000u);
@@ -332,28 +337,28 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
             ml[wave][l16] = ls;
         }
         if (__builtin_amdgcn_readfirstlane(dirty)) {
-            if constexpr (MASKED)
-                mark_not_finite_masked<D, NW>(a, b, base, g, 0, rows, wave, u1 - u0, last, [&](int k) { return (int)un.real(u0 + k); }, some_hide, mo[wave]);
+            if constexpr (MASKS != 0)
+                mark_not_finite_masked<D, NW, MASKS>(a, b, base, g, 0, rows, wave, u1 - u0, last, [&](int k) { return WINDOW ? (int)un.real(u0 + k) : u0 + k; }, some_hide, mo[wave]);
             else
                 mark_not_finite<D, NW>(a, b, base, g, 0, rows, wave, u0, u1, lim_min, last, mo[wave]);
         }
         __syncthreads();
         // thread: CT columns of a row (8 of 128, 4 of 64)
         const int qr = tid >> 4;
-        if (tid < 256 && qr < rows) finish<D, NW, ONE, MASKED>(a, tid, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
+        if (tid < 256 && qr < rows) finish<D, NW, ONE, MASKS>(a, tid, b, base, g, qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; }, [&](int w, int c) { return *reinterpret_cast<const float4*>(&mo[w][qr][c]); });
     };
-    each_segment<W, MASKED>(a, segment);
+    each_segment<W, MASKS>(a, segment);
 }
 
-template <bool MASKED>
+template <int MASKS>
 int launch_few(const Args& a, int q_dtype, const Plan& p, int D, bool much, hipStream_t st) {
     const dim3 grid(p.shares, a.c.Hkv);
 #define MXH_W4(DD, QQ, W)                                                                                          \
-    if (much) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, true, MASKED>), grid, dim3(256), 0, st, a);  \
-    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, false, MASKED>), grid, dim3(256), 0, st, a)
+    if (much) hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, true, MASKS>), grid, dim3(256), 0, st, a);  \
+    else hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::W, 4, false, MASKS>), grid, dim3(256), 0, st, a)
 #define MXH_K4(DD, QQ)                                                                                                   \
     if (p.waves == 16)                                                                                                   \
-        hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 16, false, MASKED>), grid, dim3(1024), 0, st, a);   \
+        hipLaunchKernelGGL((attn_kv4_kernel<DD, QQ, Work::kSequence, 16, false, MASKS>), grid, dim3(1024), 0, st, a);   \
     else if (p.one) { MXH_W4(DD, QQ, kSequence); }                                                                       \
     else if (a.B == 1) { MXH_W4(DD, QQ, kShare); }                                                                       \
     else { MXH_W4(DD, QQ, kLine); }

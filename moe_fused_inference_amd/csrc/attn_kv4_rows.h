@@ -57,9 +57,9 @@ struct Stage {
     alignas(16) float scale[2][64][D / 32];   // K's of the unit's 32 positions, then V's (scale_at: a lane reads a position's as it is used)
 };
 
-template <int D, int NQ, int NP, Work W, bool MASKED>
+template <int D, int NQ, int NP, Work W, int MASKS>
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
-    constexpr bool ONE = W == Work::kSequence;
+    constexpr bool ONE = W == Work::kSequence, WINDOW = MASKS & kWindow, TREE = MASKS & kTree;
     constexpr int R = 32, KT = D / 16, CT = D / 32;    // rows, steps of S, column tiles (and a lane's columns)
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     typedef uint32_t hvec __attribute__((ext_vector_type(D / 32)));
@@ -86,14 +86,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         const int last = min(clamped((int64_t)base + a.M - 1), a.c.max_pos - 1);      // positions past it are no one's
         int lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base + a.token(r0)));        // the group's first token sees up to here
         const int t1 = a.token(min(r0 + R, rows) - 1);                                           // its last token
-        const int lim_max = __builtin_amdgcn_readfirstlane(min(clamped(last_seen<MASKED>(a, base, t1)), a.c.max_pos - 1));
-        // (MASKED) where the group's first and last window begin; its units: `head` of the sinks, then others
+        const int lim_max = __builtin_amdgcn_readfirstlane(min(clamped(last_seen<MASKS>(a, base, t1)), a.c.max_pos - 1));
+        if constexpr (TREE) lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base - 1));     // (and of the drafts its own line)
+        // (WINDOW) where the group's first and last window begin; its units: `head` of the sinks, then others
         int begin_min = 0, begin_max = 0, head = 0, tail = 0;
-        if constexpr (MASKED) {
-            if (a.tree) lim_min = __builtin_amdgcn_readfirstlane(clamped((int64_t)base - 1));
-            const Units un = units<true>(a, base);
-            begin_min = __builtin_amdgcn_readfirstlane(first_begin(a, base, a.token(r0)));
-            begin_max = __builtin_amdgcn_readfirstlane(last_begin(a, base, t1));
+        if constexpr (WINDOW) {
+            const Units un = units<MASKS>(a, base);
+            begin_min = __builtin_amdgcn_readfirstlane(first_begin<MASKS>(a, base, a.token(r0)));
+            begin_max = __builtin_amdgcn_readfirstlane(last_begin<MASKS>(a, base, t1));
             u1 = min(u1, lim_max < 0 ? 0 : min((int)un.n, (int)un.of_real(lim_max / kUnit) + 1));
             if (!ONE && u0 >= u1) return;                       // no row of the group sees the segment: no record
             const int from = max(u0, max((int)un.of_real(begin_min / kUnit), (int)un.sinks));
@@ -104,8 +104,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             u1 = min(u1, (lim_max + kUnit) / kUnit);
             if (!ONE && u0 >= u1) return;
         }
-        auto real = [&](int k) { return MASKED ? k + (k < head ? u0 : tail) : u0 + k; };     // the group's k-th unit
-        auto some_hide = [&](int p0) { return p0 + kUnit - 1 > lim_min || (MASKED && p0 < begin_max && p0 + kUnit > a.sinks); };
+        auto real = [&](int k) { return WINDOW ? k + (k < head ? u0 : tail) : u0 + k; };     // the group's k-th unit
+        auto some_hide = [&](int p0) { return p0 + kUnit - 1 > lim_min || (WINDOW && p0 < begin_max && p0 + kUnit > a.sinks); };
         const int n = u0 + wave < u1 ? (u1 - u0 - wave + kWaves - 1) / kWaves : 0;   // the wave's units: wave + 4 j
         // the first head rows of units j, j = lane, tiles 0 and 1 (kv4::kNoRow: there is no such tile)
         uint32_t first[2];
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 int64_t u = (int64_t)u0 + wave + kWaves * (j0 + lane);
-                if constexpr (MASKED) u += wave + kWaves * (j0 + lane) < head ? 0 : tail - u0;
+                if constexpr (WINDOW) u += wave + kWaves * (j0 + lane) < head ? 0 : tail - u0;
                 const int64_t pos = u * kUnit + 16 * t;
                 first[t] = kv4::kNoRow;
                 if (pos < a.c.max_pos && j0 + lane < n) first[t] = kv4::head_row32(a.c, b, g, (int)pos);
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         auto locate = [&](int j) {
             if ((j & 63) == 0) find_rows(j);
             const uint32_t x = __builtin_amdgcn_readlane(first[0], j & 63), y = __builtin_amdgcn_readlane(first[1], j & 63);
-            return Unit{x == kv4::kNoRow ? 0 : x, y == kv4::kNoRow ? 0 : y, (x == kv4::kNoRow ? 0 : 1) | (y == kv4::kNoRow ? 0 : 2), (MASKED ? real(wave + kWaves * j) : u0 + wave + kWaves * j) * kUnit};
+            return Unit{x == kv4::kNoRow ? 0 : x, y == kv4::kNoRow ? 0 : y, (x == kv4::kNoRow ? 0 : 1) | (y == kv4::kNoRow ? 0 : 2), (WINDOW ? real(wave + kWaves * j) : u0 + wave + kWaves * j) * kUnit};
         };
         // a unit's bytes, in few and wide loads.  K: row l32, half lh; codes: those of K's (lane < 32) or V's position l32, one
         // word; V: D/8 bytes of row 16 t + lane / 4
@@ -150,14 +150,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         Stage<D>& stage = lds.in.stage[wave];
         // rows past the last token, and of no page, may hold anything: 0 * NaN must not reach a sum
         auto ragged = [&](const Unit& u) {
-            return __builtin_amdgcn_readfirstlane(u.there != 3 || u.p0 + kUnit - 1 > last || (MASKED && u.p0 < begin_min && u.p0 + kUnit > a.sinks));
+            return __builtin_amdgcn_readfirstlane(u.there != 3 || u.p0 + kUnit - 1 > last || (WINDOW && u.p0 < begin_min && u.p0 + kUnit > a.sinks));
         };
         auto put_codes = [&](int j, const Unit& u) {
             if (ragged(u)) {
                 int sees = last - u.p0;
                 asm volatile("" : "+v"(sees));       // (nothing below is computed ahead of the branch)
                 if (!(u.there >> (l32 >> 4) & 1) || l32 > sees) rcodes = 0x7F7F7F7Fu;
-                if (MASKED && u.p0 + l32 < begin_min && u.p0 + l32 >= a.sinks) rcodes = 0x7F7F7F7Fu;
+                if (WINDOW && u.p0 + l32 < begin_min && u.p0 + l32 >= a.sinks) rcodes = 0x7F7F7F7Fu;
             }
             typedef float svec __attribute__((ext_vector_type(D / 32)));
             svec x;
@@ -169,14 +169,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         int dirty = 0;       // uniform: values that are not finite were taken out, among positions that not all rows see
         const int all_see = min(lim_min, last);      // up to here
         auto put_v = [&](int j, const Unit& u) {
-            const bool hide = MASKED ? some_hide(u.p0) : u.p0 + kUnit - 1 > all_see;
+            const bool hide = WINDOW ? some_hide(u.p0) : u.p0 + kUnit - 1 > all_see;
             if (__builtin_amdgcn_readfirstlane(u.there != 3 || hide)) {
                 int sees = last - u.p0;
                 asm volatile("" : "+v"(sees));
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
                     if (!(u.there >> t & 1) || 16 * t + v_row > sees ||
-                        (MASKED && u.p0 + 16 * t + v_row < begin_min && u.p0 + 16 * t + v_row >= a.sinks))
+                        (WINDOW && u.p0 + 16 * t + v_row < begin_min && u.p0 + 16 * t + v_row >= a.sinks))
                         rv[t] = 0;
                 // nor may what only some rows see reach the others'
                 float* scale[2];
@@ -224,9 +224,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         __syncthreads();
         // the lane's query is row r0 + l32; rows that are none see everything and write nothing.
         // zero: 0, or NaN where the row holds an infinity or a NaN (then so is its output)
-        const int lim = r0 + l32 < rows ? clamped(last_seen<MASKED>(a, base, a.token(r0 + l32))) : 1 << 30;
+        const int lim = r0 + l32 < rows ? clamped(last_seen<MASKS>(a, base, a.token(r0 + l32))) : 1 << 30;
         int begin = 0;
-        if constexpr (MASKED) begin = r0 + l32 < rows ? begin_of(a, b, base, a.token(r0 + l32)) : 0;
+        if constexpr (WINDOW) begin = r0 + l32 < rows ? begin_of<MASKS>(a, b, base, a.token(r0 + l32)) : 0;
         float zero = 0.0f, m = kNone, l = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) zero += not_finite(*reinterpret_cast<const uint4*>(&lds.in.qs[l32][(D / 2) * lh + 8 * kt]));
@@ -264,14 +264,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (!(u.there >> (i >> 3) & 1) || 8 * (i >> 2) + (i & 3) > sees) s[i] = -INFINITY;
-                if constexpr (MASKED) {
+                if constexpr (WINDOW) {
                     const int from = begin - u.p0 - 4 * lh, sinks = a.sinks - u.p0 - 4 * lh;
-                    const uint32_t bits = a.tree ? tree_bits(a, b, base, min(a.token(r0 + l32), a.M - 1), u.p0) >> (4 * lh) : ~0u;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int at = 8 * (i >> 2) + (i & 3);
-                        if ((at < from && at >= sinks) || !(bits >> at & 1)) s[i] = -INFINITY;
+                        if (at < from && at >= sinks) s[i] = -INFINITY;
                     }
+                }
+                if constexpr (TREE) {
+                    const uint32_t bits = tree_bits(a, b, base, min(a.token(r0 + l32), a.M - 1), u.p0) >> (4 * lh);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
                 }
             }
         };
@@ -375,8 +380,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
             ml[wave][l32] = ls;
         }
         if (__builtin_amdgcn_readfirstlane(dirty)) {
-            if constexpr (MASKED)
-                mark_not_finite_masked<D, kWaves>(a, b, base, g, r0, min(R, rows - r0), wave, u1 - u0, last, real, some_hide, lds.mo[wave]);
+            if constexpr (MASKS != 0)
+                mark_not_finite_masked<D, kWaves, MASKS>(a, b, base, g, r0, min(R, rows - r0), wave, u1 - u0, last, real, some_hide, lds.mo[wave]);
             else
                 mark_not_finite<D, kWaves>(a, b, base, g, r0, min(R, rows - r0), wave, u0, u1, all_see, last, lds.mo[wave]);
         }
@@ -384,30 +389,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
 #pragma unroll 1
         for (int qr = tid >> 4; qr < R; qr += NT / 16)
             if (r0 + qr < rows)
-                finish<D, kWaves, ONE, MASKED>(a, tid, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
+                finish<D, kWaves, ONE, MASKS>(a, tid, b, base, g, r0 + qr, u0, [&](int w) { return mm[w][qr]; }, [&](int w) { return ml[w][qr]; },
                                        [&](int w, int c) { return *reinterpret_cast<const float4*>(&lds.mo[w][qr][c]); });
     };
-    each_segment<W, MASKED>(a, segment);
+    each_segment<W, MASKS>(a, segment);
 }
 
-template <bool MASKED, int D, int NQ, int NP>
+template <int MASKS, int D, int NQ, int NP>
 void launch_rows(const Args& a, const Plan& p, hipStream_t st) {
     const dim3 grid(a.shares, a.c.Hkv, p.groups);
-    const auto kernel = p.one      ? attn_kv4_rows_kernel<D, NQ, NP, Work::kSequence, MASKED>
-                        : a.B == 1 ? attn_kv4_rows_kernel<D, NQ, NP, Work::kShare, MASKED>
-                                   : attn_kv4_rows_kernel<D, NQ, NP, Work::kLine, MASKED>;
+    const auto kernel = p.one      ? attn_kv4_rows_kernel<D, NQ, NP, Work::kSequence, MASKS>
+                        : a.B == 1 ? attn_kv4_rows_kernel<D, NQ, NP, Work::kShare, MASKS>
+                                   : attn_kv4_rows_kernel<D, NQ, NP, Work::kLine, MASKS>;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, st, a);
 }
-template <bool MASKED, int D>
+template <int MASKS, int D>
 void launch_rows(const Args& a, int q_dtype, const Plan& p, bool exact, hipStream_t st) {
     const bool half = q_dtype == MXFP4_DT_F16;
-    if (exact) half ? launch_rows<MASKED, D, 2, 3>(a, p, st) : launch_rows<MASKED, D, 1, 3>(a, p, st);
-    else half ? launch_rows<MASKED, D, 2, 2>(a, p, st) : launch_rows<MASKED, D, 1, 2>(a, p, st);
+    if (exact) half ? launch_rows<MASKS, D, 2, 3>(a, p, st) : launch_rows<MASKS, D, 1, 3>(a, p, st);
+    else half ? launch_rows<MASKS, D, 2, 2>(a, p, st) : launch_rows<MASKS, D, 1, 2>(a, p, st);
 }
-template <bool MASKED>
+template <int MASKS>
 int launch_rows(const Args& a, int q_dtype, const Plan& p, int D, bool exact, hipStream_t st) {
-    if (D == 64) launch_rows<MASKED, 64>(a, q_dtype, p, exact, st);
-    else launch_rows<MASKED, 128>(a, q_dtype, p, exact, st);
+    if (D == 64) launch_rows<MASKS, 64>(a, q_dtype, p, exact, st);
+    else launch_rows<MASKS, 128>(a, q_dtype, p, exact, st);
     return mxh::launch_status("attn_kv4 (rows)");
 }
 
