@@ -322,7 +322,7 @@ int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, const uint8_t
 
 /* mxfp4_kv4_write_slots: mxfp4_kv4_write of T tokens, token t at slots[t] (device
  * int64), the place page * (rows of a page) + row of the pool; others, -1 among them,
- * write nothing.  page: any multiple of 16. */
+ * write nothing.  A place that is named twice holds a mixture.  page: any multiple of 16. */
 int mxfp4_kv4_write_slots(const void* k, const void* v, int src_dtype, int64_t ldk, int64_t ldv, uint8_t* kq, uint8_t* ks,
                           uint8_t* vq, uint8_t* vs, int n_pages, int page, const int64_t* slots, int T, int Hkv, int D,
                           void* stream);
@@ -339,7 +339,7 @@ int mxfp4_tree_masks(const int32_t* parents, int32_t* tree, int32_t* depth, int 
  * A - 1 or the first negative path[b][k] (device int32 (B, A)), position dpos[b] +
  * path[b][k] goes to position dpos[b] + k, keys and values of every kv head, in every
  * one of n_layers caches of one shape (kq, ks, vq, vs: host arrays of their device
- * pointers); all are read before any is written.  path[b][k] = k stays where it is, and
+ * pointers, each cache once); all are read before any is written.  path[b][k] = k stays where it is, and
  * so does one below k (a path runs forward), one past the cache or on no page, or whose
  * goal is.  Pages that a table names twice, where they are written, hold a mixture. */
 int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* const* vq, uint8_t* const* vs, int n_layers,

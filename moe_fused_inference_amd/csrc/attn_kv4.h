@@ -123,10 +123,13 @@ __device__ __forceinline__ uint32_t units_of(const Args& a, int base) {
     return (uint32_t)(((int)(n < 0 ? 0 : n < a.c.max_pos ? n : a.c.max_pos) + kUnit - 1) / kUnit);
 }
 
-// Masks, each kernel's a constant: with both as one that asks what there is, a call of trees took 3 to 9 % more (16 of 64
-// drafts over 16384 positions 488 us, 466; 7 of 5 drafts, 5 heads of 64, 10.9, 9.7).  With a window the units between the sinks and the first position that any
+// Masks.  With a window the units between the sinks and the first position that any
 // token's window reaches are no work: a sequence's units are counted without them (unit
 // v stands for v, or v + gap past the sinks), here, in the shares, and in the merge.
+// Which masks there are is a constant of a kernel.  One kernel for all of them, asking at
+// run time, took trees 3 to 9 % longer (16 of 64 drafts over 16384 positions 488 us / 466,
+// 7 of 5 drafts with 5 heads of 64 10.9 / 9.7), which now cost what the plain call does
+// (459, 9.0).
 constexpr int kWindow = 1, kTree = 2;      // MASKS: one, both, or 0
 struct Units {
     uint32_t n, sinks, gap;

@@ -1,5 +1,7 @@
 // attn_kv4.hip -- attention over the MXFP4 KV cache (kv4.h): M tokens of each of
-// B sequences, token m of sequence b at dpos[b] + m over positions 0 .. dpos[b] + m.
+// B sequences, token m of sequence b at dpos[b] + m over positions 0 .. dpos[b] + m,
+// or of those the last ones and the first (a window with sinks), or with M drafts that
+// form a tree its ancestors among them (attn_kv4.h, Masks).
 //
 //   attn_kv4_kernel        workgroup (share of the batch, kv head g), up to 16 query
 //                          rows (tokens x heads of the kv head): a wave takes every
@@ -10,7 +12,7 @@
 //                          whole sequence.
 //   attn_kv4_rows_kernel   the same for more rows (attn_kv4_rows.hip).
 //   attn_kv4_merge_kernel  workgroup (kv head's row, sequence): the row's records
-//                          -> its output.
+//                          -> its output; attn_kv4_merge_rows_kernel, 16 rows.
 //
 // Shares.  dpos lives on the device, so the host fixes only how many shares there
 // may be (a round of workgroups); every workgroup adds up the batch's lengths, and
@@ -36,6 +38,13 @@
 // Rows are apart: a row's reference moves by its own terms, and values that are not finite
 // are kept from the tokens before them (mark_not_finite).  Both are code off the loop's
 // path; it costs 48 sequences 26.4 -> 26.5 us, 7 x 3 tokens of 5 heads 8.95 -> 9.1.
+// With a window a call is short, so the chains of latencies weigh more: 48 sequences, a
+// window of 2000, 16.9 us in one launch (2.8 TB/s: 192 workgroups of 16 waves, each with a
+// unit's loads ahead); one of 4096 9.7 (5.8 + 2.9: 1.4 until dpos is there, 2.1 for the
+// first unit's bytes).  A tree of 26 drafts over 4026 positions 16.0: two units a wave
+// behind 5 us of prologue, and the merge.  The second unit's K beside the first's was no
+// faster (17.0 / 17.0, a window's piece of 512 tokens 23.2 / 23.6): what a wave waits for
+// is the first bytes.
 #include "attn_kv4_few.h"
 
 #include <algorithm>

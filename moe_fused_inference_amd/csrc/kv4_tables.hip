@@ -9,12 +9,15 @@
 // page a, handed on by the thread that returns it, the others are from the stack as it was, and no
 // thread waits for another.
 //
-//   kv4_pages_kernel  every workgroup makes the sums of the whole batch (a few loads and a scan) and
-//                     moves the pages of some sequences.  Alone, it does everything.
-//   kv4_slots_kernel  otherwise: the tokens' places, and its first workgroup the ranges and the count,
+//   kv4_pages_kernel  every workgroup makes the sums of the whole batch (a few loads and a scan); the
+//                     pages that move are dealt out over all threads, which find a page's sequence
+//                     by search in the sums.  Alone, it does everything.
+//   kv4_slots_kernel  otherwise: the tokens' places, and its last workgroup the ranges and the count,
 //                     which the other launch's workgroups still read.
 //
 // Bound by the launch and by dependent loads: lengths, returned entries, the stack's, the tokens'.
+// 48 sequences of up to 125 pages, nine tokens each, 4.3 us (6.1 with a wave a sequence); 300 prompts
+// of up to 4000 tokens in pages of 16 4.4 + 4.4 us, and 2.6 TB/s of places written.
 #include "attn_kv4.h"
 #include "mx_host.h"
 

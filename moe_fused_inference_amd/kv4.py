@@ -1,4 +1,4 @@
-"""The KV cache in MXFP4: allocation, write, read-back and decode attention.
+"""The KV cache in MXFP4: allocation, write, read-back and decode attention; windows, trees of drafts, page tables.
 
 A head row of D (64 or 128) keys or values is D/2 bytes of E2M1 nibbles and
 D/32 E8M0 codes, the library's MXFP4 row, so a position of one head takes 68
@@ -12,6 +12,12 @@ one (``pages``, int32 (B, max_pages) on the device, a power-of-two page) the
 sequences share a pool, and entries outside [0, n_pages) are no page.  Token m
 of sequence b sits at ``dpos[b] + m`` (int32 (B,) on the device, so a captured
 graph follows it); a batch slot with dpos[b] <= -M is empty.
+
+A server's step over a pool, nothing of which needs the host: ``kv4_tables`` makes
+room for each sequence's new tokens and says where they go, ``kv4_write_slots``
+writes them, ``attn_decode4`` attends (``window=``, ``sinks=``; ``tree=`` from
+``tree_masks`` where the tokens are drafts); ``kv4_keep`` moves an accepted path's
+rows together, and ``kv4_tables`` with the lengths that stay takes the rest back.
 
 Every call checks its arguments (RuntimeError), allocates outputs and workspace
 with torch's caching allocator and queues its work on torch's current stream of
@@ -111,7 +117,7 @@ def kv4_tables(tables, lens, new=None, T=0):
 
 def kv4_write_slots(k, v, cache, slots):
     """kv4_write of tokens one after another: k, v (T, Hkv, D) -> the pool's rows slots (int64 (T,), those of
-    ``kv4_tables``); tokens whose slot is none write nothing."""
+    ``kv4_tables``, each of them once); tokens whose slot is none write nothing."""
     kq, ks, vq, vs = cache
     _ext().write_slots(k, v, kq, ks, vq, vs, slots)
 
