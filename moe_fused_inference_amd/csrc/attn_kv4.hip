@@ -39,7 +39,7 @@
 // are kept from the tokens before them (mark_not_finite).  Both are code off the loop's
 // path; it costs 48 sequences 26.4 -> 26.5 us, 7 x 3 tokens of 5 heads 8.95 -> 9.1.
 // With a window a call is short, so the chains of latencies weigh more: 48 sequences, a
-// window of 2000, 16.9 us in one launch (2.8 TB/s: 192 workgroups of 16 waves, each with a
+// window of 2000, 16.6 us in one launch (2.8 TB/s: 192 workgroups of 16 waves, each with a
 // unit's loads ahead); one of 4096 9.7 (5.8 + 2.9: 1.4 until dpos is there, 2.1 for the
 // first unit's bytes).  A tree of 26 drafts over 4026 positions 16.0: two units a wave
 // behind 5 us of prologue, and the merge.  The second unit's K beside the first's was no

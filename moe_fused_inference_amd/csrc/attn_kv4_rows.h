@@ -110,14 +110,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_rows_kernel(Args a) {
         // the first head rows of units j, j = lane, tiles 0 and 1 (kv4::kNoRow: there is no such tile)
         uint32_t first[2];
         auto find_rows = [&](int j0) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                int64_t u = (int64_t)u0 + wave + kWaves * (j0 + lane);
-                if constexpr (WINDOW) u += wave + kWaves * (j0 + lane) < head ? 0 : tail - u0;
-                const int64_t pos = u * kUnit + 16 * t;
-                first[t] = kv4::kNoRow;
-                if (pos < a.c.max_pos && j0 + lane < n) first[t] = kv4::head_row32(a.c, b, g, (int)pos);
-            }
+            int64_t u = (int64_t)u0 + wave + kWaves * (j0 + lane);
+            if constexpr (WINDOW) u += wave + kWaves * (j0 + lane) < head ? 0 : tail - u0;
+            kv4::unit_rows(a.c, b, g, u * kUnit, j0 + lane < n, first);
         };
         struct Unit {
             uint32_t x, y;    // its tiles' first head rows

@@ -38,15 +38,27 @@ __device__ __forceinline__ int64_t head_row(const Cache& c, int b, int g, int po
     return ((int64_t)pid * c.Hkv + g) * c.page + r;
 }
 
-// The same of the kernels that hold rows in 32 bits, which make_cache makes enough of; kNoRow for -1.
+// The same of the two tiles of a unit, those of positions pos and pos + kTile (0 on), for the kernels that hold rows in 32
+// bits, which make_cache makes enough of: kNoRow where there is none, or not `wanted`.  Both entries of the table at once:
+// a unit's rows are one memory latency.
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
-__device__ __forceinline__ uint32_t head_row32(const Cache& c, int b, int g, int pos) {
-    uint32_t pid = b, r = pos;
+__device__ __forceinline__ void unit_rows(const Cache& c, int b, int g, int64_t pos, bool wanted, uint32_t (&row)[2]) {
+    const bool there[2] = {wanted && pos < c.max_pos, wanted && pos + kTile < c.max_pos};
+    const int at[2] = {there[0] ? (int)pos : 0, there[1] ? (int)pos + kTile : 0};
+    uint32_t pid[2] = {(uint32_t)b, (uint32_t)b}, r[2] = {(uint32_t)at[0], (uint32_t)at[1]};
+    bool ok[2] = {there[0], there[1]};
     if (c.pages) {
-        pid = c.pages[(int64_t)b * c.max_pages + (pos >> c.lg)];
-        r = pos & (c.page - 1);
+        const int32_t* const table = c.pages + (int64_t)b * c.max_pages;
+        pid[0] = table[at[0] >> c.lg];
+        pid[1] = table[at[1] >> c.lg];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            ok[t] = ok[t] && pid[t] < (uint32_t)c.n_pages;
+            r[t] = at[t] & (c.page - 1);
+        }
     }
-    return c.pages && pid >= (uint32_t)c.n_pages ? kNoRow : (pid * (uint32_t)c.Hkv + (uint32_t)g) * (uint32_t)c.page + r;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) row[t] = ok[t] ? (pid[t] * (uint32_t)c.Hkv + (uint32_t)g) * (uint32_t)c.page + r[t] : kNoRow;
 }
 
 // 2^(code - 127) for the packed conversions, which read the exponent field: 0
