@@ -354,7 +354,8 @@ int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* const* vq, u
  *                  span[b][1]; zeros for a batch without pages
  *   free, state    int32 (n_pages), in place: state[0] free pages, the last of which is
  *                  taken first; state int32 (2), 8-byte aligned: that count, and how many
- *                  pages this call lacked
+ *                  pages the sequences need and have not after this call (2^30 at most):
+ *                  none was left for them, or they went back in an earlier call
  *   lens           int32 (B): positions that a sequence needs room for; 0 (or less): it
  *                  has ended and gives all its pages back
  *   news, starts   int32 (B) or NULL: of these the last news[b] are new tokens; int32
@@ -365,7 +366,12 @@ int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* const* vq, u
  *                  starts[B] on -1.  T = 0: may be NULL
  *   window, sinks  of the attention (mxfp4_attn_kv4_masked), the same in every call: pages
  *                  that no window from the first new token on (without new ones: the next)
- *                  reaches go back too, and once gone they stay gone.  0, 0: none
+ *                  reaches go back too, and once gone they stay gone: a sequence that steps
+ *                  back behind them has no place for what it needs there, and state[1]
+ *                  counts it.  But where every position is new (news[b] >= lens[b]) and
+ *                  pages are gone, it is another that begins in the place of the last, and
+ *                  those that are gone are taken again, before the others and from their
+ *                  end on.  0, 0: none
  * First the pages that are no longer needed go back, the r-th of R to place count + R -
  * 1 - r, then those that are needed are taken, both in the table's order; where there
  * are too few the first get them, and the same lengths ask for the others again.  So a

@@ -26,13 +26,13 @@
 namespace {
 
 constexpr int kMostSequences = 4096;
-constexpr int kMostTokens = 1 << 30;
+constexpr int kMostTokens = 1 << 30, kMostPages = 1 << 30;      // (sums of tokens, and of pages that lack, end there)
 
 struct Tables {
     int32_t* pages;
     int2* span;             // [lo, hi) of each sequence
     int32_t* free;
-    int32_t* state;         // free pages, and pages that the last call lacked
+    int32_t* state;         // free pages, and pages that the sequences lack after the last call
     const int32_t* lens;
     const int32_t* news;    // or null
     int32_t* starts;        // of the tokens; or null, with slots, seq, pos
@@ -42,21 +42,50 @@ struct Tables {
     int B, max_pages, n_pages, lg, window, sink_pages, T;
 };
 
-// A sequence's pages before the call and after it, and how many move.
+// A sequence's pages before the call and after it, and how many move.  No entry of the table is both returned and taken: the
+// threads that do either do not wait for each other.
+struct Range {
+    int s, w, hi;      // pages 0 .. s - 1 of the sinks, and w .. hi - 1
+};
 struct Move {
-    int lo, hi, lo2, hi2, s1, s2, w1, w2;      // ranges; the ends of the sinks' pages; where the windows' begin
-    __device__ __forceinline__ int back0() const { return max(0, s1 - s2); }
-    __device__ __forceinline__ int back1() const { return max(0, min(w2, hi) - w1); }
-    __device__ __forceinline__ int from2() const { return max(w1, max(w2, hi2)); }
-    __device__ __forceinline__ int back() const { return back0() + back1() + max(0, hi - from2()); }
+    Range has, needs;
+    int lo2;           // the new range's begin (needs.w, but for the sinks)
+    int gone;          // pages that it needs and that went back in an earlier call
+    __device__ __forceinline__ int back0() const { return max(0, has.s - needs.s); }
+    __device__ __forceinline__ int back1() const { return max(0, min(needs.w, has.hi) - has.w); }
+    __device__ __forceinline__ int from2() const { return max(has.w, max(needs.w, needs.hi)); }
+    __device__ __forceinline__ int back() const { return back0() + back1() + max(0, has.hi - from2()); }
     __device__ __forceinline__ int back_at(int r) const {     // the r-th returned
-        if (r < back0()) return s2 + r;
+        if (r < back0()) return needs.s + r;
         r -= back0();
-        return r < back1() ? w1 + r : from2() + r - back1();
+        return r < back1() ? has.w + r : from2() + r - back1();
     }
-    __device__ __forceinline__ int take0() const { return max(0, s2 - s1); }
-    __device__ __forceinline__ int take() const { return take0() + max(0, hi2 - max(w2, hi)); }
-    __device__ __forceinline__ int take_at(int a) const { return a < take0() ? s1 + a : max(w2, hi) + a - take0(); }
+    // Taken: of the sinks; before its range (where it begins anew), from its end on, so that what it gets is one range with
+    // what it has; behind it
+    __device__ __forceinline__ int take0() const { return max(0, needs.s - has.s); }
+    __device__ __forceinline__ int top1() const { return min(has.w, needs.hi); }
+    __device__ __forceinline__ int take1() const { return max(0, top1() - needs.w); }
+    __device__ __forceinline__ int from() const { return max(needs.w, has.hi); }
+    __device__ __forceinline__ int take() const { return take0() + take1() + max(0, needs.hi - from()); }
+    __device__ __forceinline__ int take_at(int a) const {
+        if (a < take0()) return has.s + a;
+        a -= take0();
+        return a < take1() ? top1() - 1 - a : from() + a - take1();
+    }
+    // Its range when it has got only the first `got` of them.
+    __device__ __forceinline__ int2 range(int got) const {
+        int lo = lo2, hi = needs.hi;
+        if (got < take()) {
+            const int rest = got - take0();
+            if (rest >= 0 && rest < take1()) {
+                lo = top1() - rest;
+                hi = min(has.hi, needs.hi);
+            } else {
+                hi = take_at(got);
+            }
+        }
+        return make_int2(min(lo, hi), hi);
+    }
 };
 // What a sequence's moves come from: its range, length and new tokens.
 struct Lengths {
@@ -68,18 +97,17 @@ __device__ __forceinline__ Lengths lengths_of(const Tables& t, int b) {
 }
 __device__ __forceinline__ Move move_of(const Tables& t, const Lengths& x) {
     Move m;
-    m.hi = min(max(x.hi, 0), t.max_pages);
-    m.lo = min(max(x.lo, 0), m.hi);
+    const int hi = min(max(x.hi, 0), t.max_pages), lo = min(max(x.lo, 0), hi), sinks = t.sink_pages;
     const int64_t room = (int64_t)t.max_pages << t.lg;
     const int64_t len = min((int64_t)max(x.len, 0), room);
-    m.hi2 = (int)((len + (1 << t.lg) - 1) >> t.lg);
-    int64_t first = 0;                                  // the first page that a window of the call's first token, or the next, reaches
-    if (t.window) first = max((int64_t)0, len - max(x.news, 0) - t.window + 1) >> t.lg;
-    m.lo2 = (int)min(max((int64_t)m.lo, first), (int64_t)m.hi2);
-    m.s1 = min(t.sink_pages, m.hi);
-    m.s2 = min(t.sink_pages, m.hi2);
-    m.w1 = max(m.lo, t.sink_pages);
-    m.w2 = max(m.lo2, t.sink_pages);
+    const int hi2 = (int)((len + (1 << t.lg) - 1) >> t.lg);
+    int first = 0;                                      // the first page that a window of the call's first token, or the next, reaches
+    if (t.window) first = (int)(max((int64_t)0, len - max(x.news, 0) - t.window + 1) >> t.lg);
+    const bool anew = x.len > 0 && x.news >= x.len && lo > sinks;      // every position is new, and pages are gone
+    m.lo2 = min(max(anew ? 0 : lo, first), hi2);
+    m.gone = max(0, m.lo2 - max(first, sinks));
+    m.has = Range{min(sinks, hi), max(lo, sinks), hi};
+    m.needs = Range{min(sinks, hi2), max(m.lo2, sinks), hi2};
     return m;
 }
 
@@ -91,6 +119,7 @@ struct Sums {
     int back[CAP], take[CAP], token[CAP];
     uint32_t wave[3][kWaves];
     int total[3];
+    unsigned long long gone;   // the pages that are, in all
     Lengths lengths[KEEP ? CAP : 1];
     __device__ __forceinline__ Lengths of(const Tables& t, int b) const {
         if constexpr (KEEP) return lengths[b];
@@ -111,9 +140,10 @@ template <int NT, int CAP, bool KEEP>
 __device__ __forceinline__ void sum_up(const Tables& t, Sums<NT, CAP, KEEP>& s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t before[3] = {0, 0, 0};
+    if (threadIdx.x == 0) s.gone = 0;
     for (int b0 = 0; b0 < t.B; b0 += NT) {
         const int b = b0 + threadIdx.x;
-        uint32_t n[3] = {0, 0, 0}, to[3];
+        uint32_t n[3] = {0, 0, 0}, to[3], gone = 0;
         if (b < t.B) {
             const Lengths x = lengths_of(t, b);
             const Move m = move_of(t, x);
@@ -121,6 +151,7 @@ __device__ __forceinline__ void sum_up(const Tables& t, Sums<NT, CAP, KEEP>& s) 
             n[0] = m.back();
             n[1] = m.take();
             n[2] = min(max(x.news, 0), kMostTokens);
+            gone = m.gone;
         }
         to[0] = mxa::wave_scan(n[0]);
         to[1] = mxa::wave_scan(n[1]);
@@ -128,6 +159,10 @@ __device__ __forceinline__ void sum_up(const Tables& t, Sums<NT, CAP, KEEP>& s) 
         if (lane == 63)
             for (int i = 0; i < 3; ++i) s.wave[i][wave] = to[i];
         __syncthreads();
+        if (__any(gone)) {                                       // seldom: no part of the sums
+            const uint32_t all = capped_scan(gone);
+            if (lane == 63) atomicAdd(&s.gone, (unsigned long long)all);
+        }
         uint32_t at[3], sum[3];
         for (int i = 0; i < 3; ++i) {
             at[i] = sum[i] = before[i];
@@ -193,16 +228,13 @@ __device__ __forceinline__ void move_pages(const Tables& t, const S& s, int i, i
 template <class S>
 __device__ __forceinline__ int2 new_span(const Tables& t, const S& s, int b, int count) {
     const Move m = move_of(t, s.of(t, b));
-    const int n = m.take(), got = (int)min((int64_t)n, max((int64_t)0, (int64_t)count + s.total[0] - s.take[b]));
-    int hi = m.hi2;
-    if (got < n) hi = got < m.take0() ? m.s1 + got : max(m.w2, m.hi) + got - m.take0();
-    return make_int2(min(m.lo2, hi), hi);
+    return m.range((int)min((int64_t)m.take(), max((int64_t)0, (int64_t)count + s.total[0] - s.take[b])));
 }
 __device__ __forceinline__ int free_count(const Tables& t) { return min(max(t.state[0], 0), t.n_pages); }
-// Free pages after the call, and how many lacked.
-__device__ __forceinline__ int2 new_state(const Tables& t, int count, int R, int A) {
-    const int64_t there = (int64_t)count + R;
-    return make_int2((int)min(there - min((int64_t)A, there), (int64_t)t.n_pages), (int)(A - min((int64_t)A, there)));
+// Free pages after the call, and how many are needed and not there: R and A returned and taken, `gone` gone.
+__device__ __forceinline__ int2 new_state(const Tables& t, int count, int R, int A, uint64_t gone) {
+    const int64_t there = (int64_t)count + R, got = min((int64_t)A, there);
+    return make_int2((int)min(there - got, (int64_t)t.n_pages), (int)min(A - got + gone, (uint64_t)kMostPages));
 }
 
 // Token `at`, of sequence b, at position p.
@@ -231,7 +263,7 @@ __global__ __launch_bounds__(NT) void kv4_pages_kernel(Tables t) {
     if constexpr (ALONE) {
         for (int b = threadIdx.x; b < t.B; b += NT) t.span[b] = new_span(t, s, b, count);
         __syncthreads();                                 // the table is written, and the count has been read
-        if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1]);
+        if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1], s.gone);
         for (int at = threadIdx.x; at < t.T; at += NT) {
             if (at >= s.total[2]) {
                 no_token(t, at);
@@ -276,7 +308,7 @@ __global__ __launch_bounds__(NT) void kv4_slots_kernel(Tables t) {
     const int count = free_count(t);
     sum_up(t, s);
     for (int q = threadIdx.x; q < t.B; q += NT) t.span[q] = new_span(t, s, q, count);      // (each reads its own alone)
-    if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1]);
+    if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1], s.gone);
 }
 
 // Entries of the table, and sequences, up to which one workgroup does everything.

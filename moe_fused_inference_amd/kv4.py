@@ -53,8 +53,8 @@ def empty_cache(n_pages, page, Hkv, D=128, device="cuda"):
 
 class PageTables(NamedTuple):
     """A batch's page table over a pool, and what is left of the pool (:func:`page_tables`).  ``pages`` is what the
-    calls here take as theirs; the others are ``kv4_tables``' own.  ``state``: free pages, and how many the last
-    call lacked."""
+    calls here take as theirs; the others are ``kv4_tables``' own.  ``state``: free pages, and how many the sequences
+    need and have not since the last call."""
     pages: torch.Tensor      # int32 (B, max_pages)
     span: torch.Tensor       # int32 (B, 2)
     free: torch.Tensor       # int32 (n_pages)
@@ -110,7 +110,11 @@ def kv4_tables(tables, lens, new=None, T=0):
     sequences get them, ``state[1]`` says how many lack, and the same call asks for them again.  A call and one with
     the lengths before it (drafts that are rejected) leave everything as it was.
 
-    new (int32 (B,)): the last new[b] positions are new tokens; -> their Slots, T places."""
+    new (int32 (B,)): the last new[b] positions are new tokens; -> their Slots, T places.
+
+    With a window, pages behind it that went back are not given again: a sequence that steps back to them has none
+    there, its new tokens' slots are -1, and ``state[1]`` counts them.  One that begins in the place of another, all
+    lens[b] positions of it new, has its pages from the first on, with or without a call of length 0 between."""
     got = _ext().tables(tables.pages, tables.span, tables.free, tables.state, tables.page, tables.window, tables.sinks, lens, new, T)
     return Slots(*got) if got else None
 

@@ -17,29 +17,36 @@ class Tables:
     def update(self, lens, news=None, T=0):
         B, max_pages = self.pages.shape
         room = max_pages * self.page
-        wants, spans = [], []
+        wants, spans, olds, firsts = [], [], [], []
+        self.lacked = 0
         for b in range(B):
             n = min(max(int(lens[b]), 0), room)
-            hi, lo = -(-n // self.page), 0
+            hi, lo, gone_to = -(-n // self.page), 0, int(self.span[b, 0])
+            olds.append(self.has(*self.span[b]))
+            # all its positions are new, and pages are gone: it begins in the place of another
+            anew = news is not None and 0 < n and int(lens[b]) <= int(news[b]) and gone_to > self.sink_pages
+            first_taken = [i for i in range(self.sink_pages, min(gone_to, hi))][::-1] if anew else []
+            if anew:
+                gone_to = 0
             if self.window is not None:
                 first = n - max(int(news[b]) if news is not None else 0, 0)        # the first position whose window counts
-                lo = min(max(int(self.span[b, 0]), max(0, first - self.window + 1) // self.page), hi)
+                needs = max(0, first - self.window + 1) // self.page
+                lo = min(max(gone_to, needs), hi)
+                self.lacked += len(set(self.has(needs, hi)) - set(self.has(lo, hi)))
             spans.append((lo, hi))
             wants.append(self.has(lo, hi))
-        olds = [self.has(*self.span[b]) for b in range(B)]
+            firsts.append(first_taken)
         back = []
         for b in range(B):
             for i in olds[b]:
-                if i not in set(wants[b]):
+                if i not in wants[b]:
                     back.append(int(self.pages[b, i]))
                     self.pages[b, i] = -1
         self.free += back[::-1]                      # the r-th to place count + R - 1 - r
-        self.lacked = 0
         for b in range(B):
-            had = set(olds[b])
             end = None
-            for i in wants[b]:
-                if i in had:
+            for i in firsts[b] + [i for i in wants[b] if i not in firsts[b]]:
+                if i in olds[b]:
                     continue
                 if self.free:
                     self.pages[b, i] = self.free.pop()
@@ -47,7 +54,10 @@ class Tables:
                     self.lacked += 1
                     end = i if end is None else end
             lo, hi = spans[b]
-            self.span[b] = (lo, hi) if end is None else (min(lo, end), end)
+            if end in firsts[b]:
+                self.span[b] = end + 1, min(self.span[b, 1], hi)
+            else:
+                self.span[b] = (lo, hi) if end is None else (min(lo, end), end)
         if news is None:
             return None
         slots, seq, pos = [], [], []
