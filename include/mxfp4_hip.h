@@ -355,7 +355,9 @@ int mxfp4_kv4_keep(uint8_t* const* kq, uint8_t* const* ks, uint8_t* const* vq, u
  *   free, state    int32 (n_pages), in place: state[0] free pages, the last of which is
  *                  taken first; state int32 (2), 8-byte aligned: that count, and how many
  *                  pages the sequences need and have not after this call (2^30 at most):
- *                  none was left for them, or they went back in an earlier call
+ *                  none was left for them, they went back in an earlier call, or their row
+ *                  of the table has no entry for them (positions from max_pages * page on,
+ *                  whose tokens get no place)
  *   lens           int32 (B): positions that a sequence needs room for; 0 (or less): it
  *                  has ended and gives all its pages back
  *   news, starts   int32 (B) or NULL: of these the last news[b] are new tokens; int32

@@ -50,7 +50,7 @@ struct Range {
 struct Move {
     Range has, needs;
     int lo2;           // the new range's begin (needs.w, but for the sinks)
-    int gone;          // pages that it needs and that went back in an earlier call
+    int gone;          // pages that it needs and no call gives: gone back in an earlier one, or past its row
     __device__ __forceinline__ int back0() const { return max(0, has.s - needs.s); }
     __device__ __forceinline__ int back1() const { return max(0, min(needs.w, has.hi) - has.w); }
     __device__ __forceinline__ int from2() const { return max(has.w, max(needs.w, needs.hi)); }
@@ -106,6 +106,11 @@ __device__ __forceinline__ Move move_of(const Tables& t, const Lengths& x) {
     const bool anew = x.len > 0 && x.news >= x.len && lo > sinks;      // every position is new, and pages are gone
     m.lo2 = min(max(anew ? 0 : lo, first), hi2);
     m.gone = max(0, m.lo2 - max(first, sinks));
+    if (x.len > room) {
+        const int all = (int)(((int64_t)x.len + (1 << t.lg) - 1) >> t.lg);
+        const int from = t.window ? (int)(max((int64_t)0, (int64_t)x.len - max(x.news, 0) - t.window + 1) >> t.lg) : 0;
+        m.gone += max(0, all - max(t.max_pages, from)) + max(0, min(min(sinks, from), all) - t.max_pages);
+    }
     m.has = Range{min(sinks, hi), max(lo, sinks), hi};
     m.needs = Range{min(sinks, hi2), max(m.lo2, sinks), hi2};
     return m;
@@ -119,7 +124,7 @@ struct Sums {
     int back[CAP], take[CAP], token[CAP];
     uint32_t wave[3][kWaves];
     int total[3];
-    unsigned long long gone;   // the pages that are, in all
+    unsigned long long gone;   // in all
     Lengths lengths[KEEP ? CAP : 1];
     __device__ __forceinline__ Lengths of(const Tables& t, int b) const {
         if constexpr (KEEP) return lengths[b];
@@ -337,7 +342,7 @@ extern "C" int mxfp4_kv4_tables(int32_t* pages, int32_t* span, int32_t* free, in
     while ((1 << lg) < page) ++lg;
     const int sink_pages = sinks > 0 ? (int)(((int64_t)sinks + page - 1) >> lg) : 0;
     const Tables t{pages, reinterpret_cast<int2*>(span), free, state, lens, news, starts, slots, seq, pos, B, max_pages, n_pages, lg,
-                   window, sink_pages < max_pages ? sink_pages : max_pages, T};
+                   window, sink_pages, T};
     const hipStream_t st = mxh::as_stream(stream);
     if (B <= kFewSequences && (int64_t)B * max_pages <= kFewEntries && T <= kFewTokens) {
         hipLaunchKernelGGL((kv4_pages_kernel<1024, kFewSequences, true>), dim3(1), dim3(1024), 0, st, t);

@@ -112,6 +112,9 @@ def kv4_tables(tables, lens, new=None, T=0):
 
     new (int32 (B,)): the last new[b] positions are new tokens; -> their Slots, T places.
 
+    ``state[1]`` also counts the pages of lengths past max_pages * page, which no later call can give: tokens there get
+    the slot -1.
+
     With a window, pages behind it that went back are not given again: a sequence that steps back to them has none
     there, its new tokens' slots are -1, and ``state[1]`` counts them.  One that begins in the place of another, all
     lens[b] positions of it new, has its pages from the first on, with or without a call of length 0 between."""

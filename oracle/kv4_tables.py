@@ -33,6 +33,15 @@ class Tables:
                 needs = max(0, first - self.window + 1) // self.page
                 lo = min(max(gone_to, needs), hi)
                 self.lacked += len(set(self.has(needs, hi)) - set(self.has(lo, hi)))
+            # pages past its row of the table
+            n = max(int(lens[b]), 0)
+            needs = 0
+            if self.window is not None:
+                needs = max(0, n - max(int(news[b]) if news is not None else 0, 0) - self.window + 1) // self.page
+            past = range(max_pages, -(-n // self.page))
+            if past:
+                seen = range(max(needs, past.start), past.stop), range(past.start, min(self.sink_pages, needs, past.stop))
+                self.lacked += sum(map(len, seen))
             spans.append((lo, hi))
             wants.append(self.has(lo, hi))
             firsts.append(first_taken)
