@@ -374,6 +374,7 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     // positions, two / three: 119 / 137 us; 0.23 % / 0.01 % of the bf16 outputs are the neighbour of the nearest (of fp32
     // torch operators 0.09 %), and the error against 64 bits, which is bf16's own, is 1.66e-3 of the norm for all three.
     const bool exact = (o && o_dtype == MXFP4_DT_F32) || oq;
+    const bool asked = window > 0;
     if (window >= (int64_t)a.c.max_pos + (tree ? M : 0)) window = 0;      // it reaches every position
     if (window == 0) sinks = 0;
     const int room = room_of(M, a.c.max_pos, window, sinks);
@@ -382,7 +383,8 @@ extern "C" int mxfp4_attn_kv4_masked(const void* q, int q_dtype, int64_t ldq, co
     MXH_REQUIRE(p.one || (int64_t)M * Hq * merge_waves(p, B) * 64 < (1ll << 32), "attn_kv4: M*Hq=%lld too large", (long long)M * Hq);
     const size_t need = workspace_of(p, B, M, Hq, D);
     MXH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
-                "attn_kv4: workspace must be 16-byte aligned and hold mxfp4_attn_kv4_workspace_size bytes");
+                "attn_kv4: a workspace of %zu bytes, must be 16-byte aligned and hold %zu, which %s says", workspace ? workspace_bytes : 0,
+                need, asked ? "mxfp4_attn_kv4_masked_workspace_size" : "mxfp4_attn_kv4_workspace_size");
     a.q = static_cast<const uint16_t*>(q);
     a.ldq = ldq;
     a.dpos = dpos;
