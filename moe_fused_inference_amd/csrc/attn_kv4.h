@@ -127,9 +127,11 @@ __device__ __forceinline__ uint32_t units_of(const Args& a, int base) {
 // token's window reaches are no work: a sequence's units are counted without them (unit
 // v stands for v, or v + gap past the sinks), here, in the shares, and in the merge.
 // Which masks there are is a constant of a kernel.  One kernel for all of them, asking at
-// run time, took trees 3 to 9 % longer (16 of 64 drafts over 16384 positions 488 us / 466,
-// 7 of 5 drafts with 5 heads of 64 10.9 / 9.7), which now cost what the plain call does
-// (459, 9.0).
+// run time, took trees 5 and 12 % longer (16 of 64 drafts over 16384 positions 488 us / 466,
+// 7 of 5 drafts with 5 heads of 64 10.9 / 9.7).  The plain call of as many tokens / a tree:
+// one sequence of 26 16.6 / 16.6, of four over 32000 17.7 / 17.7, a batch 16 x 64 467 / 473,
+// 24 x 2 (fp16) 20.9 / 21.9, 7 x 5 9.7 / 10.5.  A line's kernels hold a tree's addresses in
+// scalar registers that spill (56 to 89 of them; without a tree 22 to 27).
 constexpr int kWindow = 1, kTree = 2;      // MASKS: one, both, or 0
 struct Units {
     uint32_t n, sinks, gap;

@@ -258,6 +258,8 @@ Plan plan(int B, int M, int Hq, int Hkv, int max_pos, int room) {
         // More rows, shares / one: 4 workgroups, 128 positions 10.9 / 9.9, 256 10.9 / 11.7; 32, 256 12.4 / 11.8, 512 13.2 /
         // 14.7; 128, 1024 21.1 / 20.9 (one sequence), 22.9 / 20.5 (eight), 2048 25.6 / 30.7, 30.4 / 31.1; 256, 2048 33.1 / 31.2,
         // 39.9 / 31.6, 4096 48.0 / 50.1, 56.1 / 50.6; 400, 4096 78.3 / 69.0; 512, 8192 131 / 125, 145 / 127 (32 sequences).
+        // The bounds take the slower form in two places of these: 32 workgroups, 1024 (12.2 for 11.7), and more rows of eight
+        // sequences, 256, 4096 (56.1 for 50.6; of one 48.0 is the faster), as they do not ask how many sequences there are.
         const bool own = wgs <= 256;
         constexpr int few = 3 * kMinShare * kUnit;
         if (p.many) {

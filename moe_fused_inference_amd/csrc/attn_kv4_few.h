@@ -119,7 +119,7 @@ __global__ __launch_bounds__(64 * NW, 4) void attn_kv4_kernel(Args a) {
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int l16 = lane & 15, lq = lane >> 4;
         // q, whose parts go to LDS once the first units' loads are on their way.  Rows past the last load nothing: with the last
-        // row's in their place 32 sequences of up to 32768 positions took 60.4 us instead of 58.2.
+        // row's in their place 32 sequences of up to 32768 positions took 60.4 us where it took 58.2 on the same card (cards differ: 55 to 58).
         const uint16_t* qb = a.q + (int64_t)b * a.M * a.ldq + (int64_t)g * G * D;
         constexpr int NT = 64 * NW, QN = (R * (D / 8) + NT - 1) / NT;
         uint4 qw[QN];

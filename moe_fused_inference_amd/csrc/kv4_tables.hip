@@ -2,7 +2,7 @@
 // back to a stack of free ones, and the newest tokens get their places.
 //
 // A sequence holds its pages in one range of its row, [lo, hi) (`span`), and below it those of the
-// first `sinks` positions.  From old and new range it is plain how many it gives back and takes;
+// first `sinks` positions; what lies between went back behind its window.  From old and new range it is plain how many it gives back and takes;
 // sums over the sequences before it say which of the call's R returned and A taken pages these are.
 // Returned page r goes to place count + R - 1 - r of the stack and taken page a comes from place
 // count + R - 1 - a, as if all were returned before any is taken: so taken page a < R is returned
@@ -16,8 +16,9 @@
 //                     which the other launch's workgroups still read.
 //
 // Bound by the launch and by dependent loads: lengths, returned entries, the stack's, the tokens'.
-// 48 sequences of up to 125 pages, nine tokens each, 4.3 us (6.1 with a wave a sequence); 300 prompts
-// of up to 4000 tokens in pages of 16 4.4 + 4.4 us, and 2.6 TB/s of places written.
+// 48 sequences of up to 125 pages, nine tokens each, 4.7 us (6.1 with a wave a sequence), and 3.7 for
+// the shorter lengths after it; 300 prompts of up to 4000 tokens in pages of 16 4.3 + 7.0 us, 2.7 TB/s
+// of places written, and 4.5 + 2.8 for the pages' way back.
 #include "attn_kv4.h"
 #include "mx_host.h"
 
@@ -316,7 +317,12 @@ __global__ __launch_bounds__(NT) void kv4_slots_kernel(Tables t) {
     if (threadIdx.x == 0) *reinterpret_cast<int2*>(t.state) = new_state(t, count, s.total[0], s.total[1], s.gone);
 }
 
-// Entries of the table, and sequences, up to which one workgroup does everything.
+// Entries of the table, and sequences, up to which one workgroup does everything.  us for two calls, nine tokens or as many
+// as it says and the shorter lengths again, one workgroup / two launches, on the device: 48 sequences, 28800 entries 8.7 /
+// 11.3, 8160 tokens 14.3 / 11.5; 300, 30000 entries, 8100 tokens 17.1 / 14.0, 20100 29.5 / 14.3, 90000 entries, 2700 tokens
+// 12.3 / 14.2; 1000, 32000 entries, 2000 tokens 14.3 / 21.0, 8000 20.5 / 21.1, 20000 34.1 / 21.0, 100000 entries, 9000
+// tokens 21.6 / 20.7; one, 2000 tokens 8.0 / 11.0, 8000 10.2 / 11.1, 20000 15.1 / 11.4.  So tokens decide, between 4000 and
+// 8000 for most batches, and fewer launches are less for the host (9 / 17 us from Python); entries alone do not.
 constexpr int64_t kFewEntries = 32768;
 constexpr int kFewTokens = 8192, kFewSequences = 1024;
 constexpr int kThreads = 512;

@@ -9,7 +9,7 @@
 //   kv4_keep_kernel    row dpos[b] + path[b][k] -> dpos[b] + k of every layer's cache.
 //
 // Both are bound by the launch and a few dependent loads: one tree of 26 drafts 1.7 us, 64 of 500
-// 4.5; a path's five rows in 48 layers 4.4, 32 paths 7.5 (1.8 TB/s of rows that are 64 and 4 bytes).
+// 4.5; a path's five rows in 48 layers 4.4, 32 paths 7.5 (0.9 TB/s of rows, read and written, that are 64 and 4 bytes).
 #include "kv4.h"
 #include "mx_host.h"
 

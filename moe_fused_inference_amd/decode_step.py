@@ -170,7 +170,9 @@ class DecodeStep:
     43.4, 32000 57.7 / 47.2; four tokens 62.8 / 66.1, 80.3 / 74.1.
 
     window, sinks (kv="mxfp4"): every layer's attention sees the last `window`
-    positions up to a token's own, and the first `sinks`."""
+    positions up to a token's own, and the first `sinks`.  us a layer at 32000
+    positions, without a window / 4096 + 4 / 1024 + 4: one token 47.0 / 45.2 / 44.5,
+    four 74.3 / 70.1 / 67.1."""
 
     def __init__(self, model, cfg, M=1, max_pos=4096, device="cuda", fused_router=True, qkv_tail=True,
                  attn_front=True, attn_next=True, kv="fp8", window=None, sinks=0):
